@@ -1,4 +1,5 @@
-"""ctypes binding of libnflow_quant.so (include/nflow_quant.h, include/nflow_runtime.h).
+"""ctypes binding of libnflow_quant.so (include/nflow_quant.h, include/nflow_block.h,
+include/nflow_runtime.h).
 
 The library is loaded from neuroflow_amd/lib/ (built in-tree by
 `python -m neuroflow_amd.build`).  There is no fallback: if the library is
@@ -23,6 +24,7 @@ STATUS_NAMES = {0: "Ok", 1: "InvalidArg", 2: "FileNotFound", 3: "ParseError",
 
 ACT_NONE, ACT_RELU, ACT_GELU_TANH = 0, 1, 2
 FORMAT_INT8, FORMAT_FP8_E4M3 = 0, 1
+DTYPE_F32, DTYPE_BF16 = 0, 1
 
 
 class Int8LinearParamsC(C.Structure):
@@ -135,6 +137,23 @@ SIGNATURES = {
     "nflow_ir_layer_create": [_vp, C.c_char_p, C.c_char_p, C.POINTER(_vp)],
     "nflow_ir_fno_int8_dispatch": [_vp, _i32, C.POINTER(_i32), C.POINTER(C.c_float), C.POINTER(C.c_int32)],
     "nflow_ir_fno_x2_quant": [_vp, _i32, C.POINTER(X2QuantC)],
+    # include/nflow_block.h
+    "nflow_layer_norm_forward": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _f32, _vp, _i64, _vp, _vp, _vp],
+    "nflow_layer_norm_fp8_block": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _vp],
+    "nflow_layer_norm_backward": [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp,
+                                  C.c_size_t, _vp],
+    "nflow_layer_norm_backward_workspace": [_i64, _i64, C.POINTER(C.c_size_t)],
+    "nflow_fp8_block_quantise": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp],
+    "nflow_fp8_block_quantise_weight": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp],
+    "nflow_fp8_block_matmul": [_vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i64, _vp,
+                               C.c_size_t, _vp],
+    "nflow_fp8_block_matmul_workspace": [_i64, _i64, _i64, _i32, C.POINTER(C.c_size_t)],
+    "nflow_fp8_block_linear": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i64, _vp, C.c_size_t,
+                               _vp],
+    "nflow_fp8_block_linear_workspace": [_i64, _i64, _i64, _i32, C.POINTER(C.c_size_t)],
+    "nflow_fp8_block_linear_backward": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp,
+                                        _vp, C.c_size_t, _vp],
+    "nflow_fp8_block_linear_backward_workspace": [_i64, _i64, _i64, _i32, C.POINTER(C.c_size_t)],
     # include/nflow_runtime.h
     "nflow_runtime_create": [C.c_char_p, C.POINTER(_vp)],
     "nflow_runtime_create_memory": [_vp, C.c_size_t, C.POINTER(_vp)],

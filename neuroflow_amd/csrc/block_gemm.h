@@ -1,0 +1,30 @@
+// block_gemm.h -- arguments of the block-FP8 product, and the launchers its
+// translation units share.
+#pragma once
+
+#include "block_dev.h"
+
+namespace nfq {
+
+// C = act(A W^T + bias); codes in rows of 128 * blk_count(K) bytes, scales
+// (blk_count(K), M) and (blk_count(K), w_blocks ? blk_count(N) : N).
+struct BlockGemmArgs {
+    const uint8_t* A;
+    const float* sA;
+    const uint8_t* W;
+    const float* sW;
+    bool w_blocks;
+    int64_t M, N, K;
+    const float* bias;
+    int act;
+    void* C;
+    int out;            // nflow_dtype of C
+    int64_t ldc;
+};
+
+// x along its rows and / or columns (block_quantise.hip); arguments checked by
+// the caller, M, K > 0.
+int block_quantise(const char* what, const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* codes,
+                   float* scales, uint8_t* codes_t, float* scales_t, hipStream_t st);
+
+}  // namespace nfq
