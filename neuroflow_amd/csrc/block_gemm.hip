@@ -1,52 +1,9 @@
 // block_gemm.hip -- the product of 128-block FP8 codes and the linear layer
 // around it, forward and backward (include/nflow_block.h).
-#include "block_gemm.h"
+#include "block_gemm_kernel.h"
 
 namespace nfq {
 namespace {
-
-// 64 x 64 outputs per block of 256 threads, 4 x 4 a thread; the codes of 32
-// columns at a time decoded into LDS.
-template <typename TO>
-__global__ __launch_bounds__(256) void k_block_matmul(BlockGemmArgs a) {
-    constexpr int BT = 64, BK = 32;
-    __shared__ float As[BK][BT + 1], Ws[BK][BT + 1];
-    const int tid = threadIdx.x, tr = tid >> 4, tc = tid & 15;
-    const int64_t tn = (a.N + BT - 1) / BT;
-    const int64_t m0 = blockIdx.x / tn * BT, n0 = blockIdx.x % tn * BT;
-    const int64_t kb = blk_count(a.K), ld = kb * kBlk, nb = blk_count(a.N);
-    float acc[4][4] = {};
-    for (int64_t b = 0; b < kb; ++b) {
-        float sum[4][4] = {};
-        for (int k0 = 0; k0 < kBlk; k0 += BK) {
-            __syncthreads();
-            for (int i = tid; i < BT * BK; i += 256) {
-                const int r = i / BK, k = i % BK;
-                As[k][r] = m0 + r < a.M ? e4m3_decode(a.A[(m0 + r) * ld + b * kBlk + k0 + k]) : 0.0f;
-                Ws[k][r] = n0 + r < a.N ? e4m3_decode(a.W[(n0 + r) * ld + b * kBlk + k0 + k]) : 0.0f;
-            }
-            __syncthreads();
-            for (int k = 0; k < BK; ++k)
-                for (int i = 0; i < 4; ++i)
-                    for (int j = 0; j < 4; ++j)
-                        sum[i][j] = __builtin_fmaf(As[k][tr * 4 + i], Ws[k][tc * 4 + j], sum[i][j]);
-        }
-        for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) {
-                const int64_t m = m0 + tr * 4 + i, n = n0 + tc * 4 + j;
-                if (m >= a.M || n >= a.N) continue;
-                const float sw = a.w_blocks ? a.sW[b * nb + n / kBlk] : a.sW[b * a.N + n];
-                acc[i][j] = __builtin_fmaf(sum[i][j], a.sA[b * a.M + m] * sw, acc[i][j]);
-            }
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + tr * 4 + i, n = n0 + tc * 4 + j;
-            if (m >= a.M || n >= a.N) continue;
-            const float z = acc[i][j] + (a.bias ? a.bias[n] : 0.0f);
-            static_cast<TO*>(a.C)[m * a.ldc + n] = from_f32<TO>(activate_rt(z, a.act));
-        }
-}
 
 // Sum of the rows of x, a thread per column.
 template <typename T>
@@ -63,13 +20,93 @@ __global__ __launch_bounds__(256) void k_column_sums(const T* __restrict__ x, in
     out[n] = s;
 }
 
-int block_gemm(const char* what, const BlockGemmArgs& a, hipStream_t st) {
+// Sum of the splits' partial results, in their order, and the epilogue.
+template <typename TO>
+__global__ __launch_bounds__(256) void k_block_gemm_join(BlockGemmArgs a, const float* __restrict__ part, int splits) {
+    const int64_t n4 = (a.N + 3) / 4, total = a.M * n4;
+    const bool vec = a.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(a.C) & (4 * sizeof(TO) - 1)) == 0;
+    const bool vin = a.N % 4 == 0;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t m = i / n4, n = (i - m * n4) * 4;
+        v4f z{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < splits; ++s) {
+            const float* p = part + (s * a.M + m) * a.N + n;
+            if (vin) {
+                const v4f q = *reinterpret_cast<const v4f*>(p);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) z[v] += q[v];
+            } else {
+                for (int v = 0; v < 4; ++v)
+                    if (n + v < a.N) z[v] += p[v];
+            }
+        }
+        store4<TO>(a, m, n, z, vec);
+    }
+}
+
+using TileBig = BlockTile<2, 4, 8, 4, 2>;     // 256 x 256, eight waves
+using TileMid = BlockTile<2, 2, 4, 4, 2>;     // 128 x 128, four waves, two blocks per CU
+
+template <typename TO, bool BLOCKS, typename T>
+void launch_tiles(const BlockGemmArgs& a, int splits, float* part, hipStream_t st) {
+    auto k = k_block_gemm<TO, BLOCKS, T>;
+    static const bool once = [&] {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                  T::NS * T::STAGE);
+        return true;
+    }();
+    (void)once;
+    const int64_t tm = (a.M + T::BM - 1) / T::BM, tn = (a.N + T::BN - 1) / T::BN;
+    const int kb = static_cast<int>(blk_count(a.K)), per = splits > 1 ? (kb + splits - 1) / splits : kb;
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(tm * tn * splits)), dim3(T::THREADS), T::NS * T::STAGE, st, a,
+                       tm, tn, splits, per, part);
+}
+
+// How a product is cut: the tile and, where the tiles alone would leave CUs
+// idle, the number of runs of K blocks.
+struct GemmPlan {
+    bool big;
+    int splits;
+    size_t bytes;       // of the partial results
+};
+GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int out) {
+    const int64_t cus = num_cus(), kb = blk_count(K);
+    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
+    GemmPlan p{out == NFLOW_DTYPE_BF16 && big >= cus, 1, 0};
+    const int64_t tiles = p.big ? big : ((M + 127) / 128) * ((N + 127) / 128);
+    const int64_t room = p.big ? cus : 2 * cus;
+    if (tiles * 2 <= room && kb >= 8) {
+        p.splits = static_cast<int>(std::min<int64_t>(room / tiles, kb / 4));
+        if (p.splits > 1) p.bytes = static_cast<size_t>(p.splits) * M * N * sizeof(float);
+    }
+    return p;
+}
+
+template <typename TO, bool BLOCKS>
+void launch_gemm(const BlockGemmArgs& a, const GemmPlan& p, float* part, hipStream_t st) {
+    if constexpr (std::is_same_v<TO, bf16>) {
+        if (p.big) launch_tiles<TO, BLOCKS, TileBig>(a, p.splits, part, st);
+    }
+    if (!p.big) launch_tiles<TO, BLOCKS, TileMid>(a, p.splits, part, st);
+    if (p.splits > 1)
+        hipLaunchKernelGGL((k_block_gemm_join<TO>), dim3(grid_for(a.M * ((a.N + 3) / 4), 256, 8)), dim3(256), 0, st, a,
+                           part, p.splits);
+}
+
+int block_gemm(const char* what, const BlockGemmArgs& a, void* ws, hipStream_t st) {
     if (a.M == 0 || a.N == 0) return NFLOW_OK;
-    const int64_t tiles = ((a.M + 63) / 64) * ((a.N + 63) / 64);
-    if (tiles > INT32_MAX) return bad_arg(what, "more than 2^31 - 1 tiles");
-    const dim3 grid(static_cast<unsigned>(tiles)), block(256);
-    if (a.out == NFLOW_DTYPE_BF16) hipLaunchKernelGGL((k_block_matmul<bf16>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((k_block_matmul<float>), grid, block, 0, st, a);
+    const GemmPlan p = gemm_plan(a.M, a.N, a.K, a.out);
+    if (((a.M + 127) / 128) * ((a.N + 127) / 128) * p.splits > INT32_MAX)
+        return bad_arg(what, "more than 2^31 - 1 tiles");
+    float* part = static_cast<float*>(ws);
+    if (a.out == NFLOW_DTYPE_BF16) {
+        if (a.w_blocks) launch_gemm<bf16, true>(a, p, part, st);
+        else launch_gemm<bf16, false>(a, p, part, st);
+    } else {
+        if (a.w_blocks) launch_gemm<float, true>(a, p, part, st);
+        else launch_gemm<float, false>(a, p, part, st);
+    }
     return launch_status(what);
 }
 
@@ -109,6 +146,7 @@ int nflow_fp8_block_matmul_workspace(int64_t M, int64_t N, int64_t K, int c_dtyp
     *bytes = 0;
     if (M < 0 || N < 0 || K < 0) return bad_arg("fp8_block_matmul_workspace", "bad dims");
     if (!dtype_ok(c_dtype)) return bad_arg("fp8_block_matmul_workspace", "unknown dtype");
+    if (M > 0 && N > 0) *bytes = gemm_plan(M, N, K, c_dtype).bytes;
     return NFLOW_OK;
 }
 
@@ -123,7 +161,7 @@ int nflow_fp8_block_matmul(const uint8_t* A, const float* scale_A, const uint8_t
     size_t need = 0;
     if (int rc = nflow_fp8_block_matmul_workspace(M, N, K, c_dtype, &need)) return rc;
     if (int rc = check_workspace(what, workspace, workspace_bytes, need)) return rc;
-    return block_gemm(what, a, as_stream(stream));
+    return block_gemm(what, a, workspace, as_stream(stream));
 }
 
 int nflow_fp8_block_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
@@ -155,7 +193,7 @@ int nflow_fp8_block_linear(const void* x, int dtype, int64_t M, int64_t K, int64
         if (int rc = block_quantise(what, x, dtype, M, K, ldx, codes, scales, nullptr, nullptr, as_stream(stream)))
             return rc;
     }
-    return block_gemm(what, a, as_stream(stream));
+    return block_gemm(what, a, codes + xs.bytes(), as_stream(stream));
 }
 
 int nflow_fp8_block_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
@@ -205,9 +243,9 @@ int nflow_fp8_block_linear_backward(const void* dy, int dtype, int64_t M, int64_
         if (int rc = launch_status(what)) return rc;
     }
     if (dx)
-        if (int rc = block_gemm(what, ax, st)) return rc;
+        if (int rc = block_gemm(what, ax, t + cols.bytes(), st)) return rc;
     if (dW)
-        if (int rc = block_gemm(what, aw, st)) return rc;
+        if (int rc = block_gemm(what, aw, t + cols.bytes(), st)) return rc;
     return NFLOW_OK;
 }
 
