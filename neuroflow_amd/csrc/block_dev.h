@@ -25,6 +25,53 @@ __device__ __forceinline__ float to_f32(bf16 v) { return static_cast<float>(v); 
 template <typename T>
 __device__ __forceinline__ T from_f32(float v) { return static_cast<T>(v); }   // bf16: nearest, ties to even
 
+// Eight consecutive elements at p as floats, of which the first `left` exist
+// (the rest are 0).  One or two 16-byte loads at any element alignment.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int64_t left, float (&v)[8]) {
+    if (left >= 8) {
+        typedef T vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+        const vec q = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = to_f32(q[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < left ? to_f32(p[e]) : 0.0f;
+    }
+}
+
+// Up to eight elements in registers as they come from memory, converted where
+// they are used, so that a load can be in flight meanwhile.
+template <typename T>
+struct Raw8 {
+    typedef T vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    vec q;
+    __device__ __forceinline__ void load(const T* p, int64_t left) {
+        if (left >= 8) {
+            q = *reinterpret_cast<const vec*>(p);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[e] = e < left ? p[e] : T(0.0f);
+        }
+    }
+    __device__ __forceinline__ float operator[](int e) const { return to_f32(q[e]); }
+};
+
+// Eight floats at any element alignment, rounded to T; the first `left` of them.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int64_t left, const float (&v)[8]) {
+    if (left >= 8) {
+        typename Raw8<T>::vec q;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = from_f32<T>(v[e]);
+        *reinterpret_cast<typename Raw8<T>::vec*>(p) = q;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < left) p[e] = from_f32<T>(v[e]);
+    }
+}
+
 // ---- 128-block scale ----------------------------------------------------------
 
 // Below this a block's codes would need a subnormal scale, whose inverse
@@ -36,18 +83,42 @@ __device__ __forceinline__ float blk_scale(float amax) { return amax < kBlkTiny 
 // max that ignores a NaN in v (amax itself is never one).
 __device__ __forceinline__ float amax_of(float amax, float v) { return fmaxf(amax, fabsf(v)); }
 
-// ---- reductions over a wave -------------------------------------------------------
+// ---- reductions over L lanes (16 or 64, aligned) --------------------------------
+// Every lane gets the result, the same bits in each: within 16 lanes by DPP,
+// then the halves of row pairs and of the wave by the permlane swaps.
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+struct SumOp {
+    static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+struct MaxOp {
+    static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
+};
+
+template <typename Op>
+__device__ __forceinline__ float cross_rows(float v) {
+    const unsigned u = __float_as_uint(v);
+    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = Op::of(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    const unsigned w = __float_as_uint(v);
+    const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return Op::of(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+
+template <int L, typename Op>
+__device__ __forceinline__ float lanes_reduce(float v) {
+    static_assert(L == 16 || L == 64, "lanes");
+    v = Op::of(v, dpp_mov<0xB1>(v));     // quad_perm 1,0,3,2
+    v = Op::of(v, dpp_mov<0x4E>(v));     // quad_perm 2,3,0,1
+    v = Op::of(v, dpp_mov<0x141>(v));    // row_half_mirror
+    v = Op::of(v, dpp_mov<0x140>(v));    // row_mirror
+    if constexpr (L == 64) v = cross_rows<Op>(v);
     return v;
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
-}
+// Sum over the wave's four rows of 16 lanes.
+__device__ __forceinline__ float rows_sum(float v) { return cross_rows<SumOp>(v); }
+__device__ __forceinline__ float wave_sum(float v) { return lanes_reduce<64, SumOp>(v); }
+__device__ __forceinline__ float wave_max(float v) { return lanes_reduce<64, MaxOp>(v); }
+__device__ __forceinline__ float max16(float v) { return lanes_reduce<16, MaxOp>(v); }
 
 // ---- checks of the entry points ----------------------------------------------------
 

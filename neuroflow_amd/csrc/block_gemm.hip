@@ -5,21 +5,6 @@
 namespace nfq {
 namespace {
 
-// Sum of the rows of x, a thread per column.
-template <typename T>
-__global__ __launch_bounds__(256) void k_column_sums(const T* __restrict__ x, int64_t M, int64_t N, int64_t ld,
-                                                     float* __restrict__ out) {
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (n >= N) return;
-    float s = 0.0f;
-    for (int64_t m0 = 0; m0 < M; m0 += 256) {       // sums of 256 rows, then their sum
-        float p = 0.0f;
-        for (int64_t m = m0; m < m0 + 256 && m < M; ++m) p += to_f32(x[m * ld + n]);
-        s += p;
-    }
-    out[n] = s;
-}
-
 // Sum of the splits' partial results, in their order, and the epilogue.
 template <typename TO>
 __global__ __launch_bounds__(256) void k_block_gemm_join(BlockGemmArgs a, const float* __restrict__ part, int splits) {
@@ -96,6 +81,11 @@ void launch_gemm(const BlockGemmArgs& a, const GemmPlan& p, float* part, hipStre
 
 int block_gemm(const char* what, const BlockGemmArgs& a, void* ws, hipStream_t st) {
     if (a.M == 0 || a.N == 0) return NFLOW_OK;
+    if (few_rows(a.M)) {
+        if (a.N > INT32_MAX) return bad_arg(what, "more than 2^31 - 1 columns");
+        launch_block_few(a, st);
+        return launch_status(what);
+    }
     const GemmPlan p = gemm_plan(a.M, a.N, a.K, a.out);
     if (((a.M + 127) / 128) * ((a.N + 127) / 128) * p.splits > INT32_MAX)
         return bad_arg(what, "more than 2^31 - 1 tiles");
@@ -146,7 +136,7 @@ int nflow_fp8_block_matmul_workspace(int64_t M, int64_t N, int64_t K, int c_dtyp
     *bytes = 0;
     if (M < 0 || N < 0 || K < 0) return bad_arg("fp8_block_matmul_workspace", "bad dims");
     if (!dtype_ok(c_dtype)) return bad_arg("fp8_block_matmul_workspace", "unknown dtype");
-    if (M > 0 && N > 0) *bytes = gemm_plan(M, N, K, c_dtype).bytes;
+    if (N > 0 && !few_rows(M)) *bytes = gemm_plan(M, N, K, c_dtype).bytes;
     return NFLOW_OK;
 }
 
@@ -169,7 +159,7 @@ int nflow_fp8_block_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype,
     if (!bytes) return bad_arg("fp8_block_linear_workspace", "null output");
     *bytes = 0;
     if (int rc = nflow_fp8_block_matmul_workspace(M, N, K, dtype, bytes)) return rc;
-    *bytes = round16(*bytes) + BlockSpace(M, K).bytes();
+    if (!few_values(M)) *bytes = round16(*bytes) + BlockSpace(M, K).bytes();
     return NFLOW_OK;
 }
 
@@ -182,17 +172,27 @@ int nflow_fp8_block_linear(const void* x, int dtype, int64_t M, int64_t K, int64
     if (int rc = nflow_fp8_block_linear_workspace(M, N, K, dtype, &need)) return rc;
     if (int rc = check_workspace(what, workspace, workspace_bytes, need)) return rc;
     if (ldx < K) return bad_arg(what, "row stride smaller than a row");
+    // The codes the product reads: none where it quantises by itself.
+    const bool direct = few_values(M);
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     const BlockSpace xs(M, K);
     float* scales = reinterpret_cast<float*>(codes + xs.codes);
-    const BlockGemmArgs a{codes, scales, W, scale_W, true, M, N, K, bias, activation, y, dtype, ldy};
+    BlockGemmArgs a{codes, scales, W, scale_W, true, M, N, K, bias, activation, y, dtype, ldy};
+    if (direct) {
+        a.A = W;            // not read; check_gemm wants the operands' pointers
+        a.sA = scale_W;
+    }
     if (int rc = check_gemm(what, a)) return rc;
     if (M == 0 || N == 0) return NFLOW_OK;
-    if (K > 0) {
-        if (!x) return bad_arg(what, "null x");
-        if (int rc = block_quantise(what, x, dtype, M, K, ldx, codes, scales, nullptr, nullptr, as_stream(stream)))
-            return rc;
+    if (K > 0 && !x) return bad_arg(what, "null x");
+    if (direct) {
+        if (N > INT32_MAX) return bad_arg(what, "more than 2^31 - 1 columns");
+        launch_block_few_values(a, x, ldx, as_stream(stream));
+        return launch_status(what);
     }
+    if (K > 0)
+        if (int rc = block_quantise(what, x, dtype, M, K, ldx, codes, scales, nullptr, nullptr, nullptr, as_stream(stream)))
+            return rc;
     return block_gemm(what, a, codes + xs.bytes(), as_stream(stream));
 }
 
@@ -203,7 +203,8 @@ int nflow_fp8_block_linear_backward_workspace(int64_t M, int64_t N, int64_t K, i
     size_t dx = 0, dw = 0;
     if (int rc = nflow_fp8_block_matmul_workspace(M, K, N, dtype, &dx)) return rc;
     if (int rc = nflow_fp8_block_matmul_workspace(N, K, M, NFLOW_DTYPE_F32, &dw)) return rc;
-    *bytes = round16(std::max(dx, dw)) + BlockSpace(M, N).bytes() + BlockSpace(N, M).bytes();
+    *bytes = round16(std::max(dx, dw)) + BlockSpace(M, N).bytes() + BlockSpace(N, M).bytes() +
+             round16(static_cast<size_t>(blk_count(M)) * static_cast<size_t>(N) * sizeof(float));
     return NFLOW_OK;
 }
 
@@ -230,22 +231,19 @@ int nflow_fp8_block_linear_backward(const void* dy, int dtype, int64_t M, int64_
         if (int rc = check_gemm(what, ax)) return rc;
     if (dW)
         if (int rc = check_gemm(what, aw)) return rc;
-    if (M > 0 && N > 0 && (dx || dW))
+    float* sums = reinterpret_cast<float*>(t + cols.bytes());
+    const size_t sum_bytes = round16(static_cast<size_t>(blk_count(M)) * N * sizeof(float));
+    void* parts = t + cols.bytes() + sum_bytes;
+    if (M > 0 && N > 0 && (dx || dW || dbias))
         if (int rc = block_quantise(what, dy, dtype, M, N, lddy, dx ? q : nullptr, dx ? sq : nullptr,
-                                    dW ? t : nullptr, dW ? stt : nullptr, st))
+                                    dW ? t : nullptr, dW ? stt : nullptr, dbias ? sums : nullptr, st))
             return rc;
-    if (dbias && N > 0) {
-        const dim3 grid(static_cast<unsigned>((N + 255) / 256)), block(256);
-        if (dtype == NFLOW_DTYPE_BF16)
-            hipLaunchKernelGGL((k_column_sums<bf16>), grid, block, 0, st, static_cast<const bf16*>(dy), M, N, lddy, dbias);
-        else
-            hipLaunchKernelGGL((k_column_sums<float>), grid, block, 0, st, static_cast<const float*>(dy), M, N, lddy, dbias);
-        if (int rc = launch_status(what)) return rc;
-    }
+    if (dbias && N > 0)
+        if (int rc = sum_parts(what, sums, blk_count(M), N, dbias, st)) return rc;
     if (dx)
-        if (int rc = block_gemm(what, ax, t + cols.bytes(), st)) return rc;
+        if (int rc = block_gemm(what, ax, parts, st)) return rc;
     if (dW)
-        if (int rc = block_gemm(what, aw, t + cols.bytes(), st)) return rc;
+        if (int rc = block_gemm(what, aw, parts, st)) return rc;
     return NFLOW_OK;
 }
 

@@ -1,69 +1,191 @@
 // block_quantise.hip -- activations and weights to 128-block FP8
 // (include/nflow_block.h).
-#include "block_dev.h"
+#include <type_traits>
+
+#include "block_gemm.h"
 
 namespace nfq {
 namespace {
 
-// One wave per 128 values of a line: element e of line r at x[r * rs + e * cs],
-// so rows (rs = ld, cs = 1) and columns (rs = 1, cs = ld) are the same kernel.
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+// ---- rows ------------------------------------------------------------------
+// 16 lanes take a block of 128 values, 8 adjacent ones a lane: the largest
+// magnitude is a DPP reduction within the 16, the codes are 8 bytes a lane.
+// Sixteen neighbouring groups take the same blocks of neighbouring rows, so a
+// workgroup's scales (rows of the (blocks, M) array) leave as runs.  HBM
+// bound: each group has kRun blocks of its row in flight.
+constexpr int kRun = 4;
+
 template <typename T>
-__global__ __launch_bounds__(256) void k_block_quantise(const T* __restrict__ x, int64_t R, int64_t L, int64_t rs,
-                                                        int64_t cs, uint8_t* __restrict__ codes,
-                                                        float* __restrict__ scales) {
-    const int lane = threadIdx.x & 63;
-    const int64_t kb = blk_count(L), n = R * kb;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * 4;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); i < n; i += step) {
-        const int64_t r = i / kb, b = i % kb, e = b * kBlk + 2 * lane;
-        const float v0 = e < L ? to_f32(x[r * rs + e * cs]) : 0.0f;
-        const float v1 = e + 1 < L ? to_f32(x[r * rs + (e + 1) * cs]) : 0.0f;
-        const float sc = blk_scale(wave_max(amax_of(amax_of(0.0f, v0), v1)));
-        const float inv = 1.0f / sc;
-        // Past the line's end the byte is 0 whatever the scale.
-        const uint32_t w0 = e < L ? fp8_quant(v0, inv) : 0u, w1 = e + 1 < L ? fp8_quant(v1, inv) : 0u;
-        *reinterpret_cast<uint16_t*>(codes + r * kb * kBlk + e) = static_cast<uint16_t>(w0 | w1 << 8);
-        if (lane == 0) scales[b * R + r] = sc;
+__global__ __launch_bounds__(256) void k_quantise_rows_blk(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
+                                                           uint8_t* __restrict__ codes, float* __restrict__ scales) {
+    const int cl = threadIdx.x & 15;
+    const int64_t kb = blk_count(K), runs = (kb + kRun - 1) / kRun, n = M * runs;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+    if (i >= n) return;
+    const int64_t b0 = i / M * kRun, m = i % M;
+    const T* row = x + m * ldx;
+    float v[kRun][8];
+#pragma unroll
+    for (int u = 0; u < kRun; ++u) {
+        const int64_t c = (b0 + u) * kBlk + 8 * cl;
+        load8(row + c, K - c, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kRun; ++u) {
+        const int64_t b = b0 + u;
+        if (b >= kb) break;
+        float amax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = amax_of(amax, v[u][e]);
+        const float sc = blk_scale(max16(amax)), inv = 1.0f / sc;
+        *reinterpret_cast<v2u*>(codes + m * kb * kBlk + b * kBlk + 8 * cl) =
+            v2u{fp8_pack4(v4f{v[u][0], v[u][1], v[u][2], v[u][3]}, inv),
+                fp8_pack4(v4f{v[u][4], v[u][5], v[u][6], v[u][7]}, inv)};
+        if (cl == 0) scales[b * M + m] = sc;
     }
 }
 
-// One block of 256 threads per 128 x 128 block of a weight.
-template <typename T>
-__global__ __launch_bounds__(256) void k_block_quantise_weight(const T* __restrict__ W, int64_t N, int64_t K,
-                                                               int64_t ldw, uint8_t* __restrict__ codes,
-                                                               float* __restrict__ scales,
-                                                               uint8_t* __restrict__ codes_t,
-                                                               float* __restrict__ scales_t) {
-    __shared__ float part[4];
-    const int64_t nb = blk_count(N), kb = blk_count(K);
-    const int64_t n0 = blockIdx.x / kb * kBlk, k0 = blockIdx.x % kb * kBlk;
-    float amax = 0.0f;
-    for (int i = threadIdx.x; i < kBlk * kBlk; i += 256) {
-        const int64_t n = n0 + i / kBlk, k = k0 + i % kBlk;
-        if (n < N && k < K) amax = amax_of(amax, to_f32(W[n * ldw + k]));
+// ---- both axes, and weights ----------------------------------------------------
+// A workgroup takes 128 x 128 values, one read: 16 lanes cover a row, and
+// thread (rg, cl) holds the 8 x 8 values of rows 8 rg .. and columns 8 cl ...
+// Row maxima are a DPP reduction, column maxima a shuffle over the wave's four
+// row groups and LDS over the four waves.  The column codes are 8 bytes of a
+// column per thread and column; they cross to rows of the transposed array in
+// LDS (8-byte slot s of line c at s ^ (c / 8), which spreads the 16 lanes of
+// a write over the banks) and leave as whole 128-byte lines.
+struct TileOut {
+    uint8_t* codes;       // along rows, or null
+    float* scales;
+    uint8_t* codes_t;     // along columns, or null
+    float* scales_t;
+    float* col_sums;      // (row tiles, K) sums of 128 rows, or null
+};
+
+template <typename T, bool WEIGHT>
+__global__ __launch_bounds__(256) void k_quantise_tile(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
+                                                       TileOut o) {
+    __shared__ __attribute__((aligned(16))) uint8_t lt[kBlk * kBlk];
+    __shared__ __attribute__((aligned(16))) float cmax[4][kBlk];
+    __shared__ __attribute__((aligned(16))) float csum[4][kBlk];
+    const int tid = threadIdx.x, cl = tid & 15, rg = tid >> 4, wave = tid >> 6, lane = tid & 63;
+    const int64_t kb = blk_count(K), mb = blk_count(M);
+    const int64_t tm = blockIdx.x / kb, tk = blockIdx.x % kb;
+    const int64_t m0 = tm * kBlk + 8 * rg, c0 = tk * kBlk + 8 * cl;
+    float v[8][8];
+#pragma unroll
+    for (int p = 0; p < 8; ++p) load8(x + (m0 + p) * ldx + c0, m0 + p < M ? K - c0 : 0, v[p]);
+
+    float ca[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        ca[e] = 0.0f;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) ca[e] = amax_of(ca[e], v[p][e]);
+        ca[e] = fmaxf(ca[e], __shfl_xor(ca[e], 16));
+        ca[e] = fmaxf(ca[e], __shfl_xor(ca[e], 32));
     }
-    amax = wave_max(amax);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = amax;
+    if (lane < 16) {
+        *reinterpret_cast<v4f*>(&cmax[wave][8 * cl]) = v4f{ca[0], ca[1], ca[2], ca[3]};
+        *reinterpret_cast<v4f*>(&cmax[wave][8 * cl + 4]) = v4f{ca[4], ca[5], ca[6], ca[7]};
+    }
+    if (!WEIGHT && o.col_sums) {
+        float cs[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            cs[e] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < 8; ++p) cs[e] += v[p][e];
+            cs[e] += __shfl_xor(cs[e], 16);
+            cs[e] += __shfl_xor(cs[e], 32);
+        }
+        if (lane < 16) {
+            *reinterpret_cast<v4f*>(&csum[wave][8 * cl]) = v4f{cs[0], cs[1], cs[2], cs[3]};
+            *reinterpret_cast<v4f*>(&csum[wave][8 * cl + 4]) = v4f{cs[4], cs[5], cs[6], cs[7]};
+        }
+    }
     __syncthreads();
-    const float sc = blk_scale(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
-    const float inv = 1.0f / sc;
-    for (int i = threadIdx.x; i < kBlk * kBlk; i += 256) {
-        const int64_t n = n0 + i / kBlk, k = k0 + i % kBlk;
-        const uint32_t q = n < N && k < K ? fp8_quant(to_f32(W[n * ldw + k]), inv) : 0u;
-        if (n < N) codes[n * kb * kBlk + k] = static_cast<uint8_t>(q);
-        if (codes_t && k < K) codes_t[k * nb * kBlk + n] = static_cast<uint8_t>(q);
+    float cinv[8], sblk = 0.0f;
+    if constexpr (WEIGHT) {
+        float w = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) w = fmaxf(w, cmax[q >> 1][64 * (q & 1) + lane]);
+        sblk = blk_scale(wave_max(w));
+        const float inv = 1.0f / sblk;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cinv[e] = inv;
+        if (tid == 0) {
+            o.scales[tk * mb + tm] = sblk;
+            if (o.scales_t) o.scales_t[tm * kb + tk] = sblk;
+        }
+    } else {
+        if (tid < kBlk && tk * kBlk + tid < K) {
+            if (o.codes_t)
+                o.scales_t[tm * K + tk * kBlk + tid] =
+                    blk_scale(fmaxf(fmaxf(cmax[0][tid], cmax[1][tid]), fmaxf(cmax[2][tid], cmax[3][tid])));
+            if (o.col_sums)
+                o.col_sums[tm * K + tk * kBlk + tid] = (csum[0][tid] + csum[1][tid]) + (csum[2][tid] + csum[3][tid]);
+        }
+        if (o.codes_t) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int c = 8 * cl + e;
+                cinv[e] = 1.0f / blk_scale(fmaxf(fmaxf(cmax[0][c], cmax[1][c]), fmaxf(cmax[2][c], cmax[3][c])));
+            }
+        }
     }
-    if (threadIdx.x == 0) {
-        scales[(k0 / kBlk) * nb + n0 / kBlk] = sc;
-        if (scales_t) scales_t[(n0 / kBlk) * kb + k0 / kBlk] = sc;
+
+    if (o.codes) {
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            float inv = cinv[0];
+            if constexpr (!WEIGHT) {
+                float amax = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) amax = amax_of(amax, v[p][e]);
+                const float sc = blk_scale(max16(amax));
+                inv = 1.0f / sc;
+                if (cl == 0 && m0 + p < M) o.scales[tk * M + m0 + p] = sc;
+            }
+            if (m0 + p < M)
+                *reinterpret_cast<v2u*>(o.codes + (m0 + p) * kb * kBlk + c0) =
+                    v2u{fp8_pack4(v4f{v[p][0], v[p][1], v[p][2], v[p][3]}, inv),
+                        fp8_pack4(v4f{v[p][4], v[p][5], v[p][6], v[p][7]}, inv)};
+        }
+    }
+    if (o.codes_t) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<v2u*>(lt + (8 * cl + e) * kBlk + 8 * (rg ^ cl)) =
+                v2u{fp8_pack4(v4f{v[0][e], v[1][e], v[2][e], v[3][e]}, cinv[e]),
+                    fp8_pack4(v4f{v[4][e], v[5][e], v[6][e], v[7][e]}, cinv[e])};
+        __syncthreads();
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            const int c = 32 * it + (tid >> 3), s = 2 * (tid & 7), x = c >> 3;
+            const v2u lo = *reinterpret_cast<const v2u*>(lt + c * kBlk + 8 * (s ^ x));
+            const v2u hi = *reinterpret_cast<const v2u*>(lt + c * kBlk + 8 * ((s + 1) ^ x));
+            if (tk * kBlk + c < K)
+                *reinterpret_cast<v4u*>(o.codes_t + (tk * kBlk + c) * mb * kBlk + tm * kBlk + 8 * s) =
+                    v4u{lo[0], lo[1], hi[0], hi[1]};
+        }
     }
 }
 
-template <typename T>
-void launch_lines(const T* x, int64_t R, int64_t L, int64_t rs, int64_t cs, uint8_t* codes, float* scales,
-                  hipStream_t st) {
-    hipLaunchKernelGGL((k_block_quantise<T>), dim3(grid_for(R * blk_count(L), 4, 8)), dim3(256), 0, st, x, R, L, rs,
-                       cs, codes, scales);
+// out[n] = the sum of parts (P, N) over P: 64 columns a workgroup, its four
+// waves a quarter of the parts each.
+__global__ __launch_bounds__(256) void k_sum_parts(const float* __restrict__ part, int64_t P, int64_t N,
+                                                   float* __restrict__ out) {
+    __shared__ float s[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+    float v = 0.0f;
+    if (n < N)
+        for (int64_t p = wave; p < P; p += 4) v += part[p * N + n];
+    s[wave][lane] = v;
+    __syncthreads();
+    if (wave == 0 && n < N) out[n] = (s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]);
 }
 
 int check_matrix(const char* what, const void* x, int dtype, int64_t M, int64_t K, int64_t ldx) {
@@ -77,13 +199,27 @@ int check_matrix(const char* what, const void* x, int dtype, int64_t M, int64_t 
 }  // namespace
 
 int block_quantise(const char* what, const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* codes,
-                   float* scales, uint8_t* codes_t, float* scales_t, hipStream_t st) {
+                   float* scales, uint8_t* codes_t, float* scales_t, float* col_sums, hipStream_t st) {
+    const int64_t kb = blk_count(K);
+    const bool tile = codes_t || col_sums;
+    const int64_t blocks = tile ? blk_count(M) * kb : (M * ((kb + kRun - 1) / kRun) + 15) / 16;
+    if (blocks > INT32_MAX) return bad_arg(what, "more than 2^31 - 1 blocks");
+    const dim3 grid(static_cast<unsigned>(blocks)), block(256);
     auto run = [&](auto* p) {
-        if (codes) launch_lines(p, M, K, ldx, int64_t{1}, codes, scales, st);
-        if (codes_t) launch_lines(p, K, M, int64_t{1}, ldx, codes_t, scales_t, st);
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+        if (tile)
+            hipLaunchKernelGGL((k_quantise_tile<T, false>), grid, block, 0, st, p, M, K, ldx,
+                               TileOut{codes, scales, codes_t, scales_t, col_sums});
+        else
+            hipLaunchKernelGGL((k_quantise_rows_blk<T>), grid, block, 0, st, p, M, K, ldx, codes, scales);
     };
     if (dtype == NFLOW_DTYPE_BF16) run(static_cast<const bf16*>(x));
     else run(static_cast<const float*>(x));
+    return launch_status(what);
+}
+
+int sum_parts(const char* what, const float* part, int64_t P, int64_t N, float* out, hipStream_t st) {
+    hipLaunchKernelGGL(k_sum_parts, dim3(static_cast<unsigned>((N + 63) / 64)), dim3(256), 0, st, part, P, N, out);
     return launch_status(what);
 }
 
@@ -102,7 +238,7 @@ int nflow_fp8_block_quantise(const void* x, int dtype, int64_t M, int64_t K, int
     if (!codes && !codes_t) return bad_arg(what, "no output asked for");
     if (!codes != !scales || !codes_t != !scales_t) return bad_arg(what, "codes and scales come in pairs");
     if (!aligned(codes, 16) || !aligned(codes_t, 16)) return bad_arg(what, "codes must be 16-byte aligned");
-    return block_quantise(what, x, dtype, M, K, ldx, codes, scales, codes_t, scales_t, as_stream(stream));
+    return block_quantise(what, x, dtype, M, K, ldx, codes, scales, codes_t, scales_t, nullptr, as_stream(stream));
 }
 
 int nflow_fp8_block_quantise_weight(const void* W, int dtype, int64_t N, int64_t K, int64_t ldw, uint8_t* codes,
@@ -117,12 +253,13 @@ int nflow_fp8_block_quantise_weight(const void* W, int dtype, int64_t N, int64_t
     const int64_t blocks = blk_count(N) * blk_count(K);
     if (blocks > INT32_MAX) return bad_arg(what, "more than 2^31 - 1 blocks");
     const dim3 grid(static_cast<unsigned>(blocks)), block(256);
+    const TileOut o{codes, scales, codes_t, scales_t, nullptr};
     if (dtype == NFLOW_DTYPE_BF16)
-        hipLaunchKernelGGL((k_block_quantise_weight<bf16>), grid, block, 0, as_stream(stream),
-                           static_cast<const bf16*>(W), N, K, ldw, codes, scales, codes_t, scales_t);
+        hipLaunchKernelGGL((k_quantise_tile<bf16, true>), grid, block, 0, as_stream(stream),
+                           static_cast<const bf16*>(W), N, K, ldw, o);
     else
-        hipLaunchKernelGGL((k_block_quantise_weight<float>), grid, block, 0, as_stream(stream),
-                           static_cast<const float*>(W), N, K, ldw, codes, scales, codes_t, scales_t);
+        hipLaunchKernelGGL((k_quantise_tile<float, true>), grid, block, 0, as_stream(stream),
+                           static_cast<const float*>(W), N, K, ldw, o);
     return launch_status(what);
 }
 
