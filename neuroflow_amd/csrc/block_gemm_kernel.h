@@ -160,12 +160,14 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
             const int q = wid + T::WAVES * c;
             wide_dma(q < BM / 8 ? dA : dW, st + 1024 * q, voff[c], kBlk * k);
         }
-        // Scales: wave w takes 64 of them, A's rows first, then W's; a wave
-        // with none left fills its 256 bytes with zeros.
+        // Scales: wave w takes 64 of them, A's rows first, then W's (with BLOCKS
+        // those of the tile's 128-blocks of columns, all by one wave); a wave with
+        // none left fills its 256 bytes with zeros.
         const bool of_a = wid < BM / 64;
         const int w = of_a ? wid : wid - BM / 64;
-        const int64_t left = of_a ? rows_a - 64 * w : (BLOCKS ? 0 : rows_w - 64 * w);
-        const float* src = of_a ? a.sA + k * a.M + m0 + 64 * w : a.sW + k * a.N + n0 + 64 * w;
+        const int64_t left = of_a ? rows_a - 64 * w : BLOCKS ? (w == 0 ? nb - n0 / kBlk : 0) : rows_w - 64 * w;
+        const float* src = of_a ? a.sA + k * a.M + m0 + 64 * w
+                                : BLOCKS ? a.sW + k * nb + n0 / kBlk : a.sW + k * a.N + n0 + 64 * w;
         dma_dword(wide_desc(src, on ? (left < 64 ? left : 64) * 4 : 0), st + T::CODES + 256 * wid, 4 * lane, 0);
     };
 
@@ -175,10 +177,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
 #pragma unroll
         for (int j = 0; j < TJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-    // The wave's weight scale is uniform (one 128-block of columns); a block
-    // past the last column's is never stored, so it may be any.
     const int64_t ncol = n0 + 16 * TJ * wn;
-    const int64_t nblk = ncol < a.N ? ncol / kBlk : 0;
 
     auto fragment = [&](const uint8_t* st, int row) {
         const uint8_t* p = st + row * kBlk;
@@ -191,8 +190,15 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
 #pragma unroll
     for (int s = 0; s < LEAD; ++s) load(k0 + s, s);
     int stage = 0;
+    // One K block: row tile i's products are issued while row tile i - 1's sums
+    // join the accumulators (four FMAs behind each product) and row tile i + 1's
+    // codes come from LDS.  With a weight's scales the last row tile's sums wait
+    // in registers for the next block, past the barrier and its LDS latency.
+    v4f d[2][TJ];
+    float pend = 0.0f;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) d[1][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     for (int k = k0; k < k1; ++k) {
-        const float sw = BLOCKS ? a.sW[k * nb + nblk] : 1.0f;
         wait_barrier<(LEAD - 1) * T::LOADS>();
         {
             const int ns = stage + LEAD;
@@ -202,45 +208,89 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
         const float* sc = reinterpret_cast<const float*>(st + T::CODES);
         stage = stage + 1 == T::NS ? 0 : stage + 1;
 
-        v8i wf[TJ];
+        // Fragments run ahead of the products: one row tile for the FP8
+        // instruction, two for the bf16 one, whose operands are converted a row
+        // tile ahead.
+        constexpr int AHEAD = FP8 ? 1 : 2;
+        v8i wf[TJ], xf[2];
         v4f swv[TJ];
+        float sa[TI];
+        auto xfrag = [&](int i) { return fragment(st, 16 * TI * wm + 16 * i + r); };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) xf[i] = xfrag(i);
 #pragma unroll
         for (int j = 0; j < TJ; ++j) {
             wf[j] = fragment(st + BM * kBlk, 16 * TJ * wn + 16 * j + r);
             if constexpr (!BLOCKS) swv[j] = *reinterpret_cast<const v4f*>(sc + BM + 16 * TJ * wn + 16 * j + 4 * g);
         }
-        Bf16x32 wb[FP8 ? 1 : TJ];
+        const float sw = BLOCKS ? sc[BM + 16 * TJ * wn / kBlk] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) sa[i] = sc[16 * TI * wm + 16 * i + r];
+        auto join = [&](int i, const v4f (&dd)[TJ], int j, float s) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                acc[i][j][v] = __builtin_fmaf(BLOCKS ? dd[j][v] : dd[j][v] * swv[j][v], s, acc[i][j][v]);
+        };
+        Bf16x32 wb[FP8 ? 1 : TJ], xb[FP8 ? 1 : 2];
         if constexpr (!FP8) {
 #pragma unroll
             for (int j = 0; j < TJ; ++j) wb[j] = to_bf16(wf[j]);
+            xb[0] = to_bf16(xf[0]);
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < TI; ++i) {
-            const int row = 16 * TI * wm + 16 * i + r;
-            const v8i xf = fragment(st, row);
-            const float sa = sc[row] * sw;
-            v4f d[TJ];
+            const int pi = (i + TI - 1) % TI;
+            const bool joins = i > 0 || BLOCKS, reads = i + AHEAD < TI;
             if constexpr (FP8) {
+                if (reads) xf[(i + 1) & 1] = xfrag(i + 1);
 #pragma unroll
-                for (int j = 0; j < TJ; ++j)
-                    d[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], xf, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0,
-                                                                            0, 0, 0, 0);
+                for (int j = 0; j < TJ; ++j) {
+                    d[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        wf[j], xf[i & 1], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0, 0, 0);
+                    if (joins) join(pi, d[(i + 1) & 1], j, pend);
+                }
+                if (reads) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);     // LDS reads
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // a product
+                    if (joins) __builtin_amdgcn_sched_group_barrier(0x002, BLOCKS ? 4 : 8, 0);
+                }
             } else {
-                const Bf16x32 xb = to_bf16(xf);
-#pragma unroll
-                for (int j = 0; j < TJ; ++j) d[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                if (i + 1 < TI) xb[(i + 1) & 1] = to_bf16(xf[(i + 1) & 1]);
+                if (reads) xf[i & 1] = xfrag(i + 2);
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
 #pragma unroll
                     for (int j = 0; j < TJ; ++j)
-                        d[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j].q[q], xb.q[q], d[j], 0, 0, 0);
+                        d[i & 1][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            wb[j].q[q], xb[i & 1].q[q], q ? d[i & 1][j] : v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                if (joins) {
+#pragma unroll
+                    for (int j = 0; j < TJ; ++j) join(pi, d[(i + 1) & 1], j, pend);
+                }
+                if (reads) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+                for (int j = 0; j < 4 * TJ; ++j) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if (i + 1 < TI) __builtin_amdgcn_sched_group_barrier(0x002, 4 / TJ, 0);   // a conversion
+                    if (joins) __builtin_amdgcn_sched_group_barrier(0x002, BLOCKS ? 1 : 2, 0);
+                }
             }
-#pragma unroll
-            for (int j = 0; j < TJ; ++j)
-#pragma unroll
-                for (int v = 0; v < 4; ++v)
-                    acc[i][j][v] = __builtin_fmaf(BLOCKS ? d[j][v] : d[j][v] * swv[j][v], sa, acc[i][j][v]);
+            pend = sa[i] * sw;
+            __builtin_amdgcn_sched_barrier(0);
         }
+        static_assert(TI % 2 == 0, "the pending sums are those of an odd row tile");
+        if constexpr (!BLOCKS) {
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) join(TI - 1, d[1], j, pend);
+        }
+    }
+    if constexpr (BLOCKS) {
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) acc[TI - 1][j][v] = __builtin_fmaf(d[1][j][v], pend, acc[TI - 1][j][v]);
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // the empty loads past the last block
 
