@@ -56,6 +56,8 @@ struct BlockTile {
     static constexpr int BM = 16 * TI * WM, BN = 16 * TJ * WN;
     static constexpr int CODES = (BM + BN) * kBlk;                 // bytes of a stage's codes
     static constexpr int STAGE = CODES + 256 * WAVES;              // and of its scales, 64 a wave
+    static constexpr int STRIP_ROW = 16 * TJ + 4, STRIP = 16 * STRIP_ROW;   // floats of a wave's 16 rows on their way out
+    static_assert(WAVES * STRIP * 4 <= NS * STAGE, "the strips fit the stages");
     static constexpr int NL = (BM + BN) / 8 / WAVES;               // 1 KB code loads per wave and step
     static constexpr int LOADS = NL + 1;                           // and one 64-scale load
     static_assert((BM + BN) / 8 % WAVES == 0, "code loads spread evenly");
@@ -91,7 +93,8 @@ __device__ __forceinline__ void store4(const BlockGemmArgs& a, int64_t m, int64_
     }
     if (vec && n + 3 < a.N) {
         typedef TO v4t __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<v4t*>(c) = v4t{from_f32<TO>(y[0]), from_f32<TO>(y[1]), from_f32<TO>(y[2]), from_f32<TO>(y[3])};
+        const v4t q{from_f32<TO>(y[0]), from_f32<TO>(y[1]), from_f32<TO>(y[2]), from_f32<TO>(y[3])};
+        *reinterpret_cast<v4t*>(c) = q;
         return;
     }
 #pragma unroll
@@ -108,6 +111,68 @@ __device__ __forceinline__ Bf16x32 to_bf16(v8i c) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o.q[i] = fp8x8_to_bf16(c[2 * i], c[2 * i + 1]);
     return o;
+}
+
+// A wave's TI x TJ tiles of sums to rows m0 .., columns n0 .. of C, with bias
+// and activation, through its strip of LDS.
+// STREAM: non-temporal stores, for results that the caller's next launch reads,
+// if at all, from beyond the L2 (65536 x 1024 x 1024: bf16 95 -> 88 us, fp32 172
+// -> 156 us; 8192 x 8192 x 8192 515 -> 504 us).
+template <typename TO, typename T, bool STREAM, int TI, int TJ>
+__device__ __forceinline__ void store_tiles(const v4f (&acc)[TI][TJ], float* strip, TO* C, int64_t M, int64_t N,
+                                            int64_t ldc, const float* bias, int act, int64_t m0, int64_t n0) {
+    constexpr int V = 16 / sizeof(TO), LPR = 16 * TJ / V, RPI = 64 / LPR;   // values a lane, lanes a row, rows a store
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int row = lane / LPR, col = V * (lane % LPR);
+    const int64_t n = n0 + col;
+    const bool vec = n + V <= N && ldc % V == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0;
+    float b[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) b[v] = bias && n + v < N ? bias[n + v] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) *reinterpret_cast<v4f*>(strip + r * T::STRIP_ROW + 16 * j + 4 * g) = acc[i][j];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int q = 0; q < 16 / RPI; ++q) {
+            const int64_t m = m0 + 16 * i + RPI * q + row;
+            const float* p = strip + (RPI * q + row) * T::STRIP_ROW + col;
+            float y[V];
+#pragma unroll
+            for (int v = 0; v < V; v += 4) {
+                const v4f z = *reinterpret_cast<const v4f*>(p + v);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) y[v + u] = z[u] + b[v + u];
+            }
+            if (act == NFLOW_ACT_RELU) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) y[v] = activate<ACT_RELU>(y[v]);
+            } else if (act == NFLOW_ACT_GELU_TANH) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) y[v] = activate<ACT_GELU_TANH>(y[v]);
+            }
+            if (m >= M) continue;
+            TO* c = C + m * ldc + n;
+            if (vec) {
+                typedef TO vt __attribute__((ext_vector_type(V)));
+                vt o;
+#pragma unroll
+                for (int v = 0; v < V; ++v) o[v] = from_f32<TO>(y[v]);
+                if constexpr (STREAM) __builtin_nontemporal_store(o, reinterpret_cast<vt*>(c));
+                else *reinterpret_cast<vt*>(c) = o;
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (n + v < N) c[v] = from_f32<TO>(y[v]);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
 }
 
 // TO: type of C, and with it the instruction.  BLOCKS: a weight's scales (one
@@ -138,37 +203,40 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
     // 8 q .. 8 q + 7 (q = wid + WAVES c; A's rows, then W's): lane l fills slot
     // l % 8 of row 8 q + l / 8, which holds 16-byte group (l % 8) ^ ((row >> 1) & 7),
     // so that the 16 rows a fragment read takes at once lie in different banks.
-    // A block past the last gets an empty range: it fetches nothing, and every
+    // A load's rows are in its range's base, so one offset register serves all.
+    // A block past the last gets empty ranges: it fetches nothing, and every
     // step issues the same number of loads.
     const uint32_t lds0 = wide_lds_addr(lds);
-    int voff[T::NL];
-#pragma unroll
-    for (int c = 0; c < T::NL; ++c) {
-        const int row = 8 * (wid + T::WAVES * c) + (lane >> 3);
-        const int grp = (lane & 7) ^ ((row >> 1) & 7);
-        voff[c] = static_cast<int>((row < BM ? row : row - BM) * ld) + 16 * grp;
-    }
+    constexpr int ROWS = 8 * T::WAVES, NLA = BM / ROWS;      // rows per round of loads, rounds of A's
+    static_assert(BM % ROWS == 0 && BN % ROWS == 0 && ROWS % 16 == 0, "rounds of A's and of W's rows");
+    const int lrow = 8 * wid + (lane >> 3);
+    const int voff = static_cast<int>(lrow * ld) + 16 * ((lane & 7) ^ ((lrow >> 1) & 7));
     const uint8_t* baseA = a.A + m0 * ld;
     const uint8_t* baseW = a.W + n0 * ld;
+    auto load_codes = [&](int k, int s, int c) {
+        const int64_t left = c < NLA ? rows_a - ROWS * c : rows_w - ROWS * (c - NLA);
+        const uint8_t* base = c < NLA ? baseA + ROWS * c * ld : baseW + ROWS * (c - NLA) * ld;
+        wide_dma(wide_desc(base, k < k1 ? left * ld : 0), lds0 + s * T::STAGE + 1024 * (wid + T::WAVES * c), voff,
+                 kBlk * k);
+    };
+    // Scales: wave w takes 64 of them, A's rows first, then W's (with BLOCKS
+    // those of the tile's 128-blocks of columns, all by one wave); a wave with
+    // none left fills its 256 bytes with zeros.
+    const bool of_a = wid < BM / 64;
+    const int sw_at = of_a ? wid : wid - BM / 64;
+    const int64_t s_left = of_a ? rows_a - 64 * sw_at
+                                : BLOCKS ? (sw_at == 0 ? nb - n0 / kBlk : 0) : rows_w - 64 * sw_at;
+    const int64_t s_bytes = (s_left < 64 ? s_left : 64) * 4, s_step = of_a ? a.M : BLOCKS ? nb : a.N;
+    const float* s_src = of_a ? a.sA + m0 + 64 * sw_at : BLOCKS ? a.sW + n0 / kBlk : a.sW + n0 + 64 * sw_at;
+    s_src += k0 * s_step;                                    // of the block whose turn is next
+    auto load_scales = [&](int k, int s) {
+        dma_dword(wide_desc(s_src, k < k1 ? s_bytes : 0), lds0 + s * T::STAGE + T::CODES + 256 * wid, 4 * lane, 0);
+        s_src += s_step;
+    };
     auto load = [&](int k, int s) {
-        const bool on = k < k1;
-        const v4u dA = wide_desc(baseA, on ? rows_a * ld : 0);
-        const v4u dW = wide_desc(baseW, on ? rows_w * ld : 0);
-        const uint32_t st = lds0 + s * T::STAGE;
 #pragma unroll
-        for (int c = 0; c < T::NL; ++c) {
-            const int q = wid + T::WAVES * c;
-            wide_dma(q < BM / 8 ? dA : dW, st + 1024 * q, voff[c], kBlk * k);
-        }
-        // Scales: wave w takes 64 of them, A's rows first, then W's (with BLOCKS
-        // those of the tile's 128-blocks of columns, all by one wave); a wave with
-        // none left fills its 256 bytes with zeros.
-        const bool of_a = wid < BM / 64;
-        const int w = of_a ? wid : wid - BM / 64;
-        const int64_t left = of_a ? rows_a - 64 * w : BLOCKS ? (w == 0 ? nb - n0 / kBlk : 0) : rows_w - 64 * w;
-        const float* src = of_a ? a.sA + k * a.M + m0 + 64 * w
-                                : BLOCKS ? a.sW + k * nb + n0 / kBlk : a.sW + k * a.N + n0 + 64 * w;
-        dma_dword(wide_desc(src, on ? (left < 64 ? left : 64) * 4 : 0), st + T::CODES + 256 * wid, 4 * lane, 0);
+        for (int c = 0; c < T::NL; ++c) load_codes(k, s, c);
+        load_scales(k, s);
     };
 
     v4f acc[TI][TJ];
@@ -179,25 +247,98 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
 
     const int64_t ncol = n0 + 16 * TJ * wn;
 
-    auto fragment = [&](const uint8_t* st, int row) {
-        const uint8_t* p = st + row * kBlk;
-        const int x = (row >> 1) & 7;
-        const v4i lo = *reinterpret_cast<const v4i*>(p + 16 * (g ^ x));
-        const v4i hi = *reinterpret_cast<const v4i*>(p + 16 * ((g + 4) ^ x));
+    // Fragments of 16-row tile i (of A) or j (of W) of a stage: two reads at an
+    // immediate offset from a lane's place in the first tile, whose swizzle is
+    // that of every tile (16 rows on).
+    const int flo = r * kBlk + 16 * (g ^ ((r >> 1) & 7)), fhi = flo ^ 64;
+    const int xat = 16 * TI * wm, wat = BM + 16 * TJ * wn;   // first rows in the stage
+    auto fragment = [&](const uint8_t* st, int row0, int i) {
+        const v4i lo = *reinterpret_cast<const v4i*>(st + (row0 * kBlk + flo) + 16 * kBlk * i);
+        const v4i hi = *reinterpret_cast<const v4i*>(st + (row0 * kBlk + fhi) + 16 * kBlk * i);
         return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
+    auto xscale_of = [&](const uint8_t* st, int i) {
+        return reinterpret_cast<const float*>(st + T::CODES + 4 * (xat + r))[16 * i];
+    };
 
-#pragma unroll
-    for (int s = 0; s < LEAD; ++s) load(k0 + s, s);
-    int stage = 0;
-    // One K block: row tile i's products are issued while row tile i - 1's sums
-    // join the accumulators (four FMAs behind each product) and row tile i + 1's
-    // codes come from LDS.  With a weight's scales the last row tile's sums wait
-    // in registers for the next block, past the barrier and its LDS latency.
     v4f d[2][TJ];
     float pend = 0.0f;
 #pragma unroll
     for (int j = 0; j < TJ; ++j) d[1][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    static_assert(TI % 2 == 0, "the pending sums are those of an odd row tile");
+
+    if constexpr (FP8 && BLOCKS) {
+        // One K block: row tile i's products are issued while row tile i - 1's sums
+        // join the accumulators (four FMAs behind each product) and row tile i + 1's
+        // codes come from LDS.  The block's barrier stands before its last row
+        // tile, whose codes are in registers by then: past it the stage is free
+        // for the block after next, the next block's stage is complete, and its
+        // first fragments arrive under the last row tile's products.  The last
+        // sums join in the next block.
+        static_assert(T::NS == 2, "two stages");
+        load(k0, 0);
+        load(k0 + 1, 1);
+        wait_barrier<T::LOADS>();
+        const uint8_t* st = lds;
+        auto xfrag = [&](int i) { return fragment(st, xat, i); };
+        auto wfrag = [&](int j) { return fragment(st, wat, j); };
+        auto xscale = [&](int i) { return xscale_of(st, i); };
+        auto wscale = [&] { return reinterpret_cast<const float*>(st + T::CODES)[BM + 16 * TJ * wn / kBlk]; };
+        v8i wf[TJ], xf[2];
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) wf[j] = wfrag(j);
+        xf[0] = xfrag(0);
+        float sx = xscale(0), sw = wscale();
+        auto product = [&](int i, int j) {
+            d[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], xf[i & 1], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0,
+                                                                          0, 0, 0, 0, 0);
+            const int pi = (i + TI - 1) % TI;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) acc[pi][j][v] = __builtin_fmaf(d[(i + 1) & 1][j][v], pend, acc[pi][j][v]);
+        };
+        int s = 0;
+        for (int k = k0; k < k1; ++k) {
+#pragma unroll
+            for (int i = 0; i < TI - 1; ++i) {
+                xf[(i + 1) & 1] = xfrag(i + 1);
+                const float sn = xscale(i + 1);
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) product(i, j);
+                __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);            // LDS reads
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);        // a product
+                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);        // four FMAs
+                }
+                pend = sx * sw;
+                sx = sn;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            wait_barrier<0>();
+            st = lds + (s ^ 1) * T::STAGE;
+            __builtin_amdgcn_sched_barrier(0);
+            xf[0] = xfrag(0);
+            const float sn = xscale(0), swn = wscale();
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) {
+                product(TI - 1, j);
+                wf[j] = wfrag(j);
+#pragma unroll
+                for (int c = j; c < T::NL; c += TJ) load_codes(k + 2, s, c);
+                if (j == TJ - 1) load_scales(k + 2, s);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            pend = sx * sw;
+            sx = sn;
+            sw = swn;
+            s ^= 1;
+        }
+    } else {
+#pragma unroll
+    for (int s = 0; s < LEAD; ++s) load(k0 + s, s);
+    int stage = 0;
+    // As above, with one barrier at the block's start, and the sums of the last
+    // row tile joined at its end.
     for (int k = k0; k < k1; ++k) {
         wait_barrier<(LEAD - 1) * T::LOADS>();
         {
@@ -215,17 +356,17 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
         v8i wf[TJ], xf[2];
         v4f swv[TJ];
         float sa[TI];
-        auto xfrag = [&](int i) { return fragment(st, 16 * TI * wm + 16 * i + r); };
+        auto xfrag = [&](int i) { return fragment(st, xat, i); };
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) xf[i] = xfrag(i);
 #pragma unroll
         for (int j = 0; j < TJ; ++j) {
-            wf[j] = fragment(st + BM * kBlk, 16 * TJ * wn + 16 * j + r);
+            wf[j] = fragment(st, wat, j);
             if constexpr (!BLOCKS) swv[j] = *reinterpret_cast<const v4f*>(sc + BM + 16 * TJ * wn + 16 * j + 4 * g);
         }
         const float sw = BLOCKS ? sc[BM + 16 * TJ * wn / kBlk] : 1.0f;
 #pragma unroll
-        for (int i = 0; i < TI; ++i) sa[i] = sc[16 * TI * wm + 16 * i + r];
+        for (int i = 0; i < TI; ++i) sa[i] = xscale_of(st, i);
         auto join = [&](int i, const v4f (&dd)[TJ], int j, float s) {
 #pragma unroll
             for (int v = 0; v < 4; ++v)
@@ -280,11 +421,11 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
             pend = sa[i] * sw;
             __builtin_amdgcn_sched_barrier(0);
         }
-        static_assert(TI % 2 == 0, "the pending sums are those of an odd row tile");
         if constexpr (!BLOCKS) {
 #pragma unroll
             for (int j = 0; j < TJ; ++j) join(TI - 1, d[1], j, pend);
         }
+    }
     }
     if constexpr (BLOCKS) {
 #pragma unroll
@@ -294,26 +435,16 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // the empty loads past the last block
 
-    if (splits > 1) {
-        BlockGemmArgs p = a;
-        p.C = part + split * a.M * a.N;
-        p.ldc = a.N;
-        p.bias = nullptr;
-        p.act = NFLOW_ACT_NONE;
-        const bool vec = a.N % 4 == 0;
-#pragma unroll
-        for (int i = 0; i < TI; ++i)
-#pragma unroll
-            for (int j = 0; j < TJ; ++j)
-                store4<float>(p, m0 + 16 * TI * wm + 16 * i + r, ncol + 16 * j + 4 * g, acc[i][j], vec);
-        return;
-    }
-    const bool vec = a.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(a.C) & (4 * sizeof(TO) - 1)) == 0;
-#pragma unroll
-    for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int j = 0; j < TJ; ++j)
-            store4<TO>(a, m0 + 16 * TI * wm + 16 * i + r, ncol + 16 * j + 4 * g, acc[i][j], vec);
+    // Results leave through LDS (the stages' memory), a row tile at a time: a
+    // wave writes its 16 rows as the products hold them and reads them back along
+    // the rows, so that its stores are whole 128-byte lines.
+    __syncthreads();
+    float* strip = reinterpret_cast<float*>(lds) + wid * T::STRIP;
+    if (splits > 1)
+        store_tiles<float, T, false>(acc, strip, part + split * a.M * a.N, a.M, a.N, a.N, nullptr, NFLOW_ACT_NONE,
+                              m0 + xat, ncol);
+    else
+        store_tiles<TO, T, true>(acc, strip, static_cast<TO*>(a.C), a.M, a.N, a.ldc, a.bias, a.act, m0 + xat, ncol);
 }
 
 }  // namespace nfq
