@@ -80,6 +80,21 @@ constexpr float kBlkTiny = 448.0f * 0x1p-126f;
 
 __device__ __forceinline__ float blk_scale(float amax) { return amax < kBlkTiny ? 1.0f : amax / 448.0f; }
 
+// The four bytes fp8_quant(x[e], inv) under a block's own scale.  There
+// |x inv| <= 448 (1 + 2^-22), which the conversion rounds to 448, so no clamp
+// is needed; the codec's cap below 2^-6 is (fp8_prerounded); and a NaN keeps
+// through, its byte 0x7F or 0xFF (no number's byte) stripped of the sign.
+__device__ __forceinline__ uint32_t blk_pack4(float x0, float x1, float x2, float x3, float inv) {
+    auto capped = [](float v) {
+        const float sub = __builtin_amdgcn_fmed3f(v, -7.0f * 0x1p-9f, 7.0f * 0x1p-9f);
+        return fabsf(v) < 0x1p-6f ? sub : v;
+    };
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(capped(x0 * inv), capped(x1 * inv), 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(capped(x2 * inv), capped(x3 * inv), w, true);
+    const uint32_t u = static_cast<uint32_t>(w);
+    return u & ~(((u & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u);
+}
+
 // max that ignores a NaN in v (amax itself is never one).
 __device__ __forceinline__ float amax_of(float amax, float v) { return fmaxf(amax, fabsf(v)); }
 

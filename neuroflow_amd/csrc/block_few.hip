@@ -9,12 +9,15 @@
 // the workgroup joins them in LDS in the waves' order.  Bound by reading the
 // weight: N K bytes, plus the launch and one load's latency.
 //
-// Rows come as codes (a lane's row r = l % 16), or as values which the wave
-// quantises itself: the four lanes of a row hold a block's 128 values, so the
-// block's largest magnitude is two permlane swaps away.  That spares a launch,
-// and repeats the quantise in every workgroup, so it is for the fewest rows.
+// Rows come as codes, or as values, which every workgroup then quantises by
+// itself into LDS while its first weight loads are in flight: 16 lanes a block
+// of 128 values, as in block_quantise.hip. That spares a launch and repeats the
+// quantise in each workgroup, so it is for few values (few_values).
 #include "block_gemm_kernel.h"
 
+#ifndef FEWV
+#define FEWV 32768
+#endif
 namespace nfq {
 namespace {
 
@@ -49,17 +52,38 @@ __global__ __launch_bounds__(64 * W) void k_block_few(BlockGemmArgs a, const X* 
         return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
 
-    v8i wn[CT];
-    auto fetch_w = [&](int k) {
+    v8i wn[2][CT];
+    auto fetch_w = [&](int k, v8i (&w)[CT]) {
+        const int64_t at = static_cast<int64_t>(k < kb ? k : 0) * kBlk;      // past the last: any, never used
 #pragma unroll
-        for (int j = 0; j < CT; ++j) wn[j] = load_codes(wrow[j] + static_cast<int64_t>(k) * kBlk);
+        for (int j = 0; j < CT; ++j) w[j] = load_codes(wrow[j] + at);
     };
-    if (wid < kb) fetch_w(wid);
-    for (int k = wid; k < kb; k += W) {
-        v8i wf[CT];
+    if (kb > 0) {
+        fetch_w(wid, wn[0]);
+        fetch_w(wid + W, wn[1]);
+    }
+    // Values to codes and scales in LDS, rows of ldx_lds bytes (16 more than the
+    // codes, against bank conflicts between rows).
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int ldl = static_cast<int>(ld) + 16;
+    float* lds_scale = reinterpret_cast<float*>(lds + (CODES ? 0 : a.M * ldl));
+    if constexpr (!CODES) {
+        const int items = static_cast<int>(a.M) * kb, cl = threadIdx.x & 15;
+        for (int i = threadIdx.x >> 4; i < items; i += 4 * W) {
+            const int m = i / kb, b = i - m * kb, c = b * kBlk + 8 * cl;
+            float v[8], amax = 0.0f;
+            load8(x + m * ldx + c, a.K - c, v);
 #pragma unroll
-        for (int j = 0; j < CT; ++j) wf[j] = wn[j];
-        if (k + W < kb) fetch_w(k + W);
+            for (int e = 0; e < 8; ++e) amax = amax_of(amax, v[e]);
+            const float sc = blk_scale(max16(amax)), inv = 1.0f / sc;
+            typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+            *reinterpret_cast<v2u*>(lds + m * ldl + c) = v2u{blk_pack4(v[0], v[1], v[2], v[3], inv),
+                                                             blk_pack4(v[4], v[5], v[6], v[7], inv)};
+            if (cl == 0) lds_scale[i] = sc;
+        }
+        __syncthreads();
+    }
+    auto step = [&](int k, const v8i (&wf)[CT]) {
         v4f sw[CT];
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
@@ -74,29 +98,15 @@ __global__ __launch_bounds__(64 * W) void k_block_few(BlockGemmArgs a, const X* 
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            const int64_t m = 16 * i + r;
+            const int64_t m = 16 * i + r, mm = m < a.M ? m : 0;
             v8i xf;
             float sa;
             if constexpr (CODES) {
-                xf = load_codes(x + (m < a.M ? m : 0) * ld + static_cast<int64_t>(k) * kBlk + 16 * g);
-                sa = m < a.M ? a.sA[k * a.M + m] : 0.0f;
+                xf = load_codes(x + mm * ld + static_cast<int64_t>(k) * kBlk + 16 * g);
+                sa = a.sA[k * a.M + mm];
             } else {
-                // 16 values from 16 g and 16 from 64 + 16 g on: the codes' places.
-                float v[4][8], amax = 0.0f;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int64_t c = static_cast<int64_t>(k) * kBlk + 16 * g + 64 * (q >> 1) + 8 * (q & 1);
-                    load8(x + m * ldx + c, m < a.M ? a.K - c : 0, v[q]);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) amax = amax_of(amax, v[q][e]);
-                }
-                sa = blk_scale(cross_rows<MaxOp>(amax));
-                const float inv = 1.0f / sa;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    xf[2 * q] = static_cast<int>(fp8_pack4(v4f{v[q][0], v[q][1], v[q][2], v[q][3]}, inv));
-                    xf[2 * q + 1] = static_cast<int>(fp8_pack4(v4f{v[q][4], v[q][5], v[q][6], v[q][7]}, inv));
-                }
+                xf = load_codes(lds + mm * ldl + k * kBlk + 16 * g);
+                sa = lds_scale[mm * kb + k];
             }
 #pragma unroll
             for (int j = 0; j < CT; ++j) {
@@ -113,6 +123,15 @@ __global__ __launch_bounds__(64 * W) void k_block_few(BlockGemmArgs a, const X* 
                     acc[i][j][v] = __builtin_fmaf(BLOCKS ? d[v] : d[v] * sw[j][v], BLOCKS ? sa * sw[j][v] : sa, acc[i][j][v]);
             }
         }
+    };
+    // Blocks in pairs, each pair's codes asked for two of the wave's turns ahead.
+    for (int k = wid; k < kb; k += 2 * W) {
+        step(k, wn[0]);
+        fetch_w(k + 2 * W, wn[0]);
+        if (k + W < kb) {
+            step(k + W, wn[1]);
+            fetch_w(k + 3 * W, wn[1]);
+        }
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i)
@@ -128,10 +147,16 @@ __global__ __launch_bounds__(64 * W) void k_block_few(BlockGemmArgs a, const X* 
     }
 }
 
+// LDS of the quantised rows.
+size_t few_lds(int64_t M, int64_t K) {
+    return static_cast<size_t>(M * (blk_count(K) * kBlk + 16) + 4 * M * blk_count(K));
+}
+
 template <typename TO, typename X, bool BLOCKS, int RT, int CT, int W>
 void launch_w(const BlockGemmArgs& a, const X* x, int64_t ldx, hipStream_t st) {
     const unsigned grid = static_cast<unsigned>((a.N + 16 * CT - 1) / (16 * CT));
-    hipLaunchKernelGGL((k_block_few<TO, X, BLOCKS, RT, CT, W>), dim3(grid), dim3(64 * W), 0, st, a, x, ldx);
+    const size_t lds = std::is_same_v<X, uint8_t> ? 0 : few_lds(a.M, a.K);
+    hipLaunchKernelGGL((k_block_few<TO, X, BLOCKS, RT, CT, W>), dim3(grid), dim3(64 * W), lds, st, a, x, ldx);
 }
 
 // Waves per workgroup: 16 while that is at most 16 waves a CU, fewer for wide
@@ -166,7 +191,7 @@ void launch_block_few(const BlockGemmArgs& a, hipStream_t st) {
     }
 }
 
-bool few_values(int64_t M) { return M <= 16; }
+bool few_values(int64_t M, int64_t K) { return M <= 16 && M * blk_count(K) * kBlk <= FEWV; }
 
 void launch_block_few_values(const BlockGemmArgs& a, const void* x, int64_t ldx, hipStream_t st) {
     if (a.out == NFLOW_DTYPE_BF16) launch_few<bf16, bf16, true, 1, 1>(a, static_cast<const bf16*>(x), ldx, st);

@@ -159,7 +159,7 @@ int nflow_fp8_block_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype,
     if (!bytes) return bad_arg("fp8_block_linear_workspace", "null output");
     *bytes = 0;
     if (int rc = nflow_fp8_block_matmul_workspace(M, N, K, dtype, bytes)) return rc;
-    if (!few_values(M)) *bytes = round16(*bytes) + BlockSpace(M, K).bytes();
+    if (!few_values(M, K)) *bytes = round16(*bytes) + BlockSpace(M, K).bytes();
     return NFLOW_OK;
 }
 
@@ -173,7 +173,7 @@ int nflow_fp8_block_linear(const void* x, int dtype, int64_t M, int64_t K, int64
     if (int rc = check_workspace(what, workspace, workspace_bytes, need)) return rc;
     if (ldx < K) return bad_arg(what, "row stride smaller than a row");
     // The codes the product reads: none where it quantises by itself.
-    const bool direct = few_values(M);
+    const bool direct = few_values(M, K);
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     const BlockSpace xs(M, K);
     float* scales = reinterpret_cast<float*>(codes + xs.codes);

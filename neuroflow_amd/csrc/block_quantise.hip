@@ -41,8 +41,8 @@ __global__ __launch_bounds__(256) void k_quantise_rows_blk(const T* __restrict__
         for (int e = 0; e < 8; ++e) amax = amax_of(amax, v[u][e]);
         const float sc = blk_scale(max16(amax)), inv = 1.0f / sc;
         *reinterpret_cast<v2u*>(codes + m * kb * kBlk + b * kBlk + 8 * cl) =
-            v2u{fp8_pack4(v4f{v[u][0], v[u][1], v[u][2], v[u][3]}, inv),
-                fp8_pack4(v4f{v[u][4], v[u][5], v[u][6], v[u][7]}, inv)};
+            v2u{blk_pack4(v[u][0], v[u][1], v[u][2], v[u][3], inv),
+                blk_pack4(v[u][4], v[u][5], v[u][6], v[u][7], inv)};
         if (cl == 0) scales[b * M + m] = sc;
     }
 }
@@ -150,16 +150,16 @@ __global__ __launch_bounds__(256) void k_quantise_tile(const T* __restrict__ x, 
             }
             if (m0 + p < M)
                 *reinterpret_cast<v2u*>(o.codes + (m0 + p) * kb * kBlk + c0) =
-                    v2u{fp8_pack4(v4f{v[p][0], v[p][1], v[p][2], v[p][3]}, inv),
-                        fp8_pack4(v4f{v[p][4], v[p][5], v[p][6], v[p][7]}, inv)};
+                    v2u{blk_pack4(v[p][0], v[p][1], v[p][2], v[p][3], inv),
+                        blk_pack4(v[p][4], v[p][5], v[p][6], v[p][7], inv)};
         }
     }
     if (o.codes_t) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             *reinterpret_cast<v2u*>(lt + (8 * cl + e) * kBlk + 8 * (rg ^ cl)) =
-                v2u{fp8_pack4(v4f{v[0][e], v[1][e], v[2][e], v[3][e]}, cinv[e]),
-                    fp8_pack4(v4f{v[4][e], v[5][e], v[6][e], v[7][e]}, cinv[e])};
+                v2u{blk_pack4(v[0][e], v[1][e], v[2][e], v[3][e], cinv[e]),
+                    blk_pack4(v[4][e], v[5][e], v[6][e], v[7][e], cinv[e])};
         __syncthreads();
 #pragma unroll
         for (int it = 0; it < 4; ++it) {

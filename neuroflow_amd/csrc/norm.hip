@@ -78,11 +78,10 @@ __device__ __forceinline__ void load_param(const float* p, int c, int D, float n
 }
 
 template <typename T, bool FP8, int L, int NV>
-__global__ __launch_bounds__(row_threads<L>()) void k_norm(NormArgs a) {
+__global__ __launch_bounds__(row_threads<L>()) void k_norm(NormArgs a, int64_t per) {
     constexpr int G = row_threads<L>() / L;              // rows a workgroup holds
     __shared__ float part[2][L <= 64 ? 1 : L / 64];
     const int t = threadIdx.x % L;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * G;
     const int D = static_cast<int>(a.D);
     const float fd = static_cast<float>(D);
     float w[NV][8], b[NV][8];
@@ -101,9 +100,15 @@ __global__ __launch_bounds__(row_threads<L>()) void k_norm(NormArgs a) {
             next[j].load(x + c, m < a.M ? D - c : 0);
         }
     };
-    int64_t m = static_cast<int64_t>(blockIdx.x) * G + threadIdx.x / L;
-    fetch(m);
-    for (; m < a.M; m += step) {
+    // A workgroup takes a run of rows, G at a time: neighbouring rows' scales
+    // (and statistics) then meet in one L2 on their way out.
+    int64_t m = blockIdx.x * per + threadIdx.x / L;
+    const int64_t end = blockIdx.x * per + per < a.M ? blockIdx.x * per + per : a.M;
+    fetch(m < end ? m : a.M);
+    for (int64_t i = 0; i < per; i += G, m += G) {
+        // Beyond a partial last round the lanes of absent rows work on zeros and
+        // store nothing: the workgroup's barriers and the DPP reductions stay whole.
+        const bool on = m < end;
         float v[NV][8], s = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -112,42 +117,48 @@ __global__ __launch_bounds__(row_threads<L>()) void k_norm(NormArgs a) {
                 v[j][e] = next[j][e];
                 s += v[j][e];
             }
-        fetch(m + step);
+        fetch(i + G < per && m + G < end ? m + G : a.M);
         const float mean = row_sum<L>(s, part, 0) / fd;
         float q = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            const int left = D - 8 * (t + L * j);          // only a row's last vector is partial
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[j][e] = 8 * (t + L * j) + e < D ? v[j][e] - mean : 0.0f;
-                q = __builtin_fmaf(v[j][e], v[j][e], q);
+            for (int e = 0; e < 8; ++e) v[j][e] -= mean;
+            if (left < 8) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = e < left ? v[j][e] : 0.0f;
             }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q = __builtin_fmaf(v[j][e], v[j][e], q);
+        }
         const float rstd = 1.0f / sqrtf(row_sum<L>(q, part, 1) / fd + a.eps);
-        if (t == 0) {
+        if (on && t == 0) {
             if (a.mean) a.mean[m] = mean;
             if (a.rstd) a.rstd[m] = rstd;
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = 8 * (t + L * j);
+            const int c = 8 * (t + L * j), left = D - c;
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = norm_value(v[j][e], rstd, w[j][e], b[j][e]);
             if constexpr (!FP8) {
-                store8(static_cast<T*>(a.y) + m * a.ldy + c, D - c, y);
+                store8(static_cast<T*>(a.y) + m * a.ldy + c, on ? left : 0, y);
             } else {
                 // 16 threads hold a block of 128; columns past D count as 0.
                 const int kb = static_cast<int>(blk_count(D)), blk = c / kBlk;
+                if (left < 8) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = e < left ? y[e] : 0.0f;
+                }
                 float amax = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    y[e] = c + e < D ? y[e] : 0.0f;
-                    amax = amax_of(amax, y[e]);
-                }
+                for (int e = 0; e < 8; ++e) amax = amax_of(amax, y[e]);
                 const float sc = blk_scale(max16(amax)), inv = 1.0f / sc;
-                if (blk < kb) {
+                if (on && blk < kb) {
                     *reinterpret_cast<v2u*>(a.codes + m * kb * kBlk + c) =
-                        v2u{fp8_pack4(v4f{y[0], y[1], y[2], y[3]}, inv), fp8_pack4(v4f{y[4], y[5], y[6], y[7]}, inv)};
+                        v2u{blk_pack4(y[0], y[1], y[2], y[3], inv), blk_pack4(y[4], y[5], y[6], y[7], inv)};
                     if (t % 16 == 0) a.scales[blk * a.M + m] = sc;
                 }
             }
@@ -423,8 +434,9 @@ template <typename T, bool FP8, int L, int NV>
 void launch_norm(const NormArgs& a, hipStream_t st) {
     constexpr int threads = row_threads<L>(), G = threads / L;
     static const int64_t most = resident(k_norm<T, FP8, L, NV>, threads);
-    const int64_t grid = std::min((a.M + G - 1) / G, most);
-    hipLaunchKernelGGL((k_norm<T, FP8, L, NV>), dim3(static_cast<unsigned>(grid)), dim3(threads), 0, st, a);
+    const int64_t groups = (a.M + G - 1) / G, per = (groups + most - 1) / most * G;
+    hipLaunchKernelGGL((k_norm<T, FP8, L, NV>), dim3(static_cast<unsigned>((a.M + per - 1) / per)), dim3(threads), 0, st,
+                       a, per);
 }
 
 // The fewest threads that hold a row in 8 NV values each: fewer threads a row

@@ -27,8 +27,8 @@ def _params(D: int, weight, bias) -> None:
 def _stats(M: int, like: torch.Tensor, wanted: bool):
     if not wanted:
         return None, None
-    return (torch.empty(M, dtype=torch.float32, device=like.device),
-            torch.empty(M, dtype=torch.float32, device=like.device))
+    mean = torch.empty(M, dtype=torch.float32, device=like.device)
+    return mean, torch.empty_like(mean)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -38,8 +38,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     pass takes.  out may be x."""
     M, D, ldx = _matrix(x, "x")
     _params(D, weight, bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else _activation(out, "out", like=x)
-    ldy = _matrix(y, "out")[2]
+    if out is None:
+        y, ldy = torch.empty_like(x, memory_format=torch.contiguous_format), D
+    else:
+        y, ldy = out, _matrix(_activation(out, "out", like=x), "out")[2]
     mean, rstd = _stats(M, x, return_stats)
     check(_lib.lib().nflow_layer_norm_forward(_p(x), _dtype(x), M, D, ldx, _p(weight), _p(bias), float(eps), _p(y),
                                               ldy, _p(mean), _p(rstd), _stream()), "layer_norm")
