@@ -53,11 +53,12 @@ def _activation(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None)
 def _matrix(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
     """(rows, columns, row stride) of an activation."""
     _activation(t, name)
-    if t.dim() == 0:
+    shape = t.shape
+    if len(shape) == 0:
         raise ValueError(f"{name} needs an axis")
-    K = t.shape[-1]
+    K = shape[-1]
     if t.is_contiguous():
-        return (t.numel() // K if K else math.prod(t.shape[:-1])), K, K
+        return (shape[0] if len(shape) == 2 else math.prod(shape[:-1])), K, K
     if t.dim() > 2 or t.stride(-1) != 1 or t.stride(0) < K:
         raise ValueError(f"{name} must be contiguous, or 2-D with a contiguous last axis")
     return t.shape[0], K, t.stride(0)
@@ -68,6 +69,8 @@ def _param(t: Optional[torch.Tensor], n: int, name: str, required: bool = False)
         if required:
             raise TypeError(f"{name} is required")
         return
+    if type(t) is torch.Tensor and t.dtype is torch.float32 and t.is_cuda and t.shape == (n,) and t.is_contiguous():
+        return
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
     if t.dtype != torch.float32:
@@ -77,7 +80,7 @@ def _param(t: Optional[torch.Tensor], n: int, name: str, required: bool = False)
 
 
 def _block(q: BlockFp8, name: str, weight: bool = False) -> int:
-    """Rows of q; whether its scales are a weight's is returned by _is_weight."""
+    """Rows of q, whose scales are a weight's (128 x 128 blocks) or not."""
     codes, scales, k = q
     kb = (k + 127) >> 7
     if not codes.is_cuda or not scales.is_cuda:

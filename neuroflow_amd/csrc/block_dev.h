@@ -95,6 +95,38 @@ __device__ __forceinline__ uint32_t blk_pack4(float x0, float x1, float x2, floa
     return u & ~(((u & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u);
 }
 
+// Scale and inverse of C blocks whose largest magnitudes every one of 16 lanes
+// holds: lane l divides for block l % C (C a power of two), and a lane's value
+// goes to the 16 by DPP, instead of 2 C divisions (a dozen instructions each) in
+// every lane.
+// v[l % C], a bit of l at a time by masks: a conditional of two array elements
+// would send the array through LDS.
+template <int C>
+__device__ __forceinline__ float pick(const float (&v)[C], unsigned l) {
+    if constexpr (C == 1) {
+        return v[0];
+    } else {
+        const unsigned odd = 0u - (l & 1u);
+        float h[C / 2];
+#pragma unroll
+        for (int k = 0; k < C / 2; ++k)
+            h[k] = __uint_as_float((__float_as_uint(v[2 * k + 1]) & odd) | (__float_as_uint(v[2 * k]) & ~odd));
+        return pick<C / 2>(h, l >> 1);
+    }
+}
+template <int C, int K = 0>
+__device__ __forceinline__ void spread(float v, float (&out)[C]) {
+    if constexpr (K < C) {
+        out[K] = dpp_mov<0x150 + K>(v);      // row_newbcast: lane K of the 16
+        spread<C, K + 1>(v, out);
+    }
+}
+template <int C>
+__device__ __forceinline__ void blk_scales(const float (&amax)[C], float& own_scale, float (&inv)[C]) {
+    own_scale = blk_scale(pick<C>(amax, threadIdx.x));
+    spread<C>(1.0f / own_scale, inv);
+}
+
 // max that ignores a NaN in v (amax itself is never one).
 __device__ __forceinline__ float amax_of(float amax, float v) { return fmaxf(amax, fabsf(v)); }
 

@@ -33,7 +33,6 @@ int sum_parts(const char* what, const float* part, int64_t P, int64_t N, float* 
 
 // The product for few rows (block_few.hip): from codes, and from the values of
 // x (of C's type, row stride ldx) quantised on the way, W in 128 x 128 blocks.
-bool few_rows(int64_t M);
 void launch_block_few(const BlockGemmArgs& a, hipStream_t st);
 bool few_values(int64_t M, int64_t K);
 void launch_block_few_values(const BlockGemmArgs& a, const void* x, int64_t ldx, hipStream_t st);

@@ -1,5 +1,7 @@
 // block_gemm.hip -- the product of 128-block FP8 codes and the linear layer
 // around it, forward and backward (include/nflow_block.h).
+#include <cmath>
+
 #include "block_gemm_kernel.h"
 
 namespace nfq {
@@ -30,8 +32,9 @@ __global__ __launch_bounds__(256) void k_block_gemm_join(BlockGemmArgs a, const 
     }
 }
 
-using TileBig = BlockTile<2, 4, 8, 4, 2>;     // 256 x 256, eight waves
-using TileMid = BlockTile<2, 2, 4, 4, 2>;     // 128 x 128, four waves, two blocks per CU
+using TileBig = BlockTile<2, 4, 8, 4, 2>;     // 256 x 256, eight waves, a workgroup per CU
+using TileMid = BlockTile<2, 2, 4, 4, 2>;     // 128 x 128, four waves, two workgroups per CU
+using TileSmall = BlockTile<2, 2, 2, 2, 4>;   // 64 x 64, four waves, two workgroups per CU, loads three steps ahead
 
 template <typename TO, bool BLOCKS, typename T>
 void launch_tiles(const BlockGemmArgs& a, int splits, float* part, hipStream_t st) {
@@ -48,32 +51,67 @@ void launch_tiles(const BlockGemmArgs& a, int splits, float* part, hipStream_t s
                        tm, tn, splits, per, part);
 }
 
-// How a product is cut: the tile and, where the tiles alone would leave CUs
-// idle, the number of runs of K blocks.
+// How a product is cut: the kernel or tile, and the number of runs of K blocks
+// that its tiles are split into (joined by a second launch).
+enum GemmKind { GEMM_FEW, GEMM_SMALL, GEMM_MID, GEMM_BIG };
 struct GemmPlan {
-    bool big;
+    GemmKind kind;
     int splits;
     size_t bytes;       // of the partial results
 };
+
+// The cut with the least estimated time, in us.  With n workgroups on the
+// busiest CU a K block costs each tile max(alone, n each): alone is what one
+// workgroup takes for it by itself (its loads' latency), each what a further
+// one adds.  Fitted to MI355X times at 65 to 2048 rows and (N, K) from 1024 to
+// 8192, where the cut it picks is within 10% of the best of 15: e.g. bf16 4096 x
+// 4096 at 256 rows 22.0 -> 15.2 us by 64 x 64 tiles in place of 128 x 128 ones
+// in 8 splits, 1024 x 1024 at 1024 rows 15.7 -> 8.8 us unsplit; at 2048 rows
+// 128 x 128 tiles are ahead of 64 x 64, 39 against 68 us, and of 256 x 256, 39
+// against 52 us, which win from one for every CU on (8192 x 8192 x 8192 460
+// against 560 us).  A split pays a launch and its partial results' way through
+// the caches; the few-row kernel a CU's rate of reading fragments from L2
+// (36 GB/s), or the weight's from HBM.
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int out) {
-    const int64_t cus = num_cus(), kb = blk_count(K);
-    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-    GemmPlan p{out == NFLOW_DTYPE_BF16 && big >= cus, 1, 0};
-    const int64_t tiles = p.big ? big : ((M + 127) / 128) * ((N + 127) / 128);
-    const int64_t room = p.big ? cus : 2 * cus;
-    if (tiles * 2 <= room && kb >= 8) {
-        p.splits = static_cast<int>(std::min<int64_t>(room / tiles, kb / 4));
-        if (p.splits > 1) p.bytes = static_cast<size_t>(p.splits) * M * N * sizeof(float);
+    const bool f32 = out == NFLOW_DTYPE_F32;
+    const double cus = num_cus(), kb = static_cast<double>(blk_count(K)), m = static_cast<double>(M),
+                 n = static_cast<double>(N);
+    struct Cut {
+        GemmKind kind;
+        double edge, alone, each;
+    };
+    const Cut cuts[] = {{GEMM_SMALL, 64, f32 ? 0.50 : 0.35, f32 ? 0.39 : 0.25},
+                        {GEMM_MID, 128, f32 ? 1.08 : 0.72, f32 ? 0.90 : 0.54},
+                        {GEMM_BIG, 256, 1.75, 1.75}};
+    GemmPlan best{GEMM_MID, 1, 0};
+    double least = HUGE_VAL;
+    if (M <= 64) {
+        const double groups = std::ceil(n / 16), per_cu = std::ceil(groups / cus), rows = 16 + m;
+        least = std::max(n * kb * kBlk / 5.2e6, per_cu * kb * kBlk * rows / 36e3);
+        best.kind = GEMM_FEW;
     }
-    return p;
+    for (const Cut& c : cuts) {
+        if (c.kind == GEMM_BIG && f32) continue;        // its accumulators and operands do not fit the registers
+        const double tiles = std::ceil(m / c.edge) * std::ceil(n / c.edge);
+        for (int s = 1; s <= 16 && (s == 1 || 2 * s <= kb); s *= 2) {
+            const double per = std::ceil(tiles * s / cus), steps = std::ceil(kb / s);
+            const double t = steps * std::max(c.alone, per * c.each) + (s > 1 ? 5.0 + s * m * n * 8 / 8e6 : 0.0);
+            if (t < least) {
+                least = t;
+                best = GemmPlan{c.kind, s, s > 1 ? static_cast<size_t>(s) * M * N * sizeof(float) : 0};
+            }
+        }
+    }
+    return best;
 }
 
 template <typename TO, bool BLOCKS>
 void launch_gemm(const BlockGemmArgs& a, const GemmPlan& p, float* part, hipStream_t st) {
     if constexpr (std::is_same_v<TO, bf16>) {
-        if (p.big) launch_tiles<TO, BLOCKS, TileBig>(a, p.splits, part, st);
+        if (p.kind == GEMM_BIG) launch_tiles<TO, BLOCKS, TileBig>(a, p.splits, part, st);
     }
-    if (!p.big) launch_tiles<TO, BLOCKS, TileMid>(a, p.splits, part, st);
+    if (p.kind == GEMM_MID) launch_tiles<TO, BLOCKS, TileMid>(a, p.splits, part, st);
+    if (p.kind == GEMM_SMALL) launch_tiles<TO, BLOCKS, TileSmall>(a, p.splits, part, st);
     if (p.splits > 1)
         hipLaunchKernelGGL((k_block_gemm_join<TO>), dim3(grid_for(a.M * ((a.N + 3) / 4), 256, 8)), dim3(256), 0, st, a,
                            part, p.splits);
@@ -81,14 +119,11 @@ void launch_gemm(const BlockGemmArgs& a, const GemmPlan& p, float* part, hipStre
 
 int block_gemm(const char* what, const BlockGemmArgs& a, void* ws, hipStream_t st) {
     if (a.M == 0 || a.N == 0) return NFLOW_OK;
-    if (few_rows(a.M)) {
-        if (a.N > INT32_MAX) return bad_arg(what, "more than 2^31 - 1 columns");
+    const GemmPlan p = gemm_plan(a.M, a.N, a.K, a.out);
+    if (p.kind == GEMM_FEW) {
         launch_block_few(a, st);
         return launch_status(what);
     }
-    const GemmPlan p = gemm_plan(a.M, a.N, a.K, a.out);
-    if (((a.M + 127) / 128) * ((a.N + 127) / 128) * p.splits > INT32_MAX)
-        return bad_arg(what, "more than 2^31 - 1 tiles");
     float* part = static_cast<float*>(ws);
     if (a.out == NFLOW_DTYPE_BF16) {
         if (a.w_blocks) launch_gemm<bf16, true>(a, p, part, st);
@@ -100,6 +135,11 @@ int block_gemm(const char* what, const BlockGemmArgs& a, void* ws, hipStream_t s
     return launch_status(what);
 }
 
+// Whether linear is one launch of the few-row kernel on x's values.
+bool linear_direct(int64_t M, int64_t N, int64_t K, int dtype) {
+    return few_values(M, K) && gemm_plan(M, N, K, dtype).kind == GEMM_FEW;
+}
+
 int check_gemm(const char* what, const BlockGemmArgs& a) {
     if (!dtype_ok(a.out)) return bad_arg(what, "unknown dtype");
     if (a.M < 0 || a.N < 0 || a.K < 0) return bad_arg(what, "bad dims");
@@ -108,6 +148,7 @@ int check_gemm(const char* what, const BlockGemmArgs& a) {
         return bad_arg(what, "unknown activation");
     if (a.ldc < a.N) return bad_arg(what, "row stride smaller than a row");
     if (a.M == 0 || a.N == 0) return NFLOW_OK;
+    if (((a.M + 63) / 64) * ((a.N + 63) / 64) > INT32_MAX / 16) return bad_arg(what, "too many results for one launch");
     if (!a.C) return bad_arg(what, "null output");
     if (a.K > 0 && (!a.A || !a.sA || !a.W || !a.sW)) return bad_arg(what, "null codes or scales");
     if (!aligned(a.A, 16) || !aligned(a.W, 16)) return bad_arg(what, "codes must be 16-byte aligned");
@@ -136,7 +177,7 @@ int nflow_fp8_block_matmul_workspace(int64_t M, int64_t N, int64_t K, int c_dtyp
     *bytes = 0;
     if (M < 0 || N < 0 || K < 0) return bad_arg("fp8_block_matmul_workspace", "bad dims");
     if (!dtype_ok(c_dtype)) return bad_arg("fp8_block_matmul_workspace", "unknown dtype");
-    if (N > 0 && !few_rows(M)) *bytes = gemm_plan(M, N, K, c_dtype).bytes;
+    if (M > 0 && N > 0) *bytes = gemm_plan(M, N, K, c_dtype).bytes;
     return NFLOW_OK;
 }
 
@@ -159,7 +200,7 @@ int nflow_fp8_block_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype,
     if (!bytes) return bad_arg("fp8_block_linear_workspace", "null output");
     *bytes = 0;
     if (int rc = nflow_fp8_block_matmul_workspace(M, N, K, dtype, bytes)) return rc;
-    if (!few_values(M, K)) *bytes = round16(*bytes) + BlockSpace(M, K).bytes();
+    if (!linear_direct(M, N, K, dtype)) *bytes = round16(*bytes) + BlockSpace(M, K).bytes();
     return NFLOW_OK;
 }
 
@@ -173,7 +214,7 @@ int nflow_fp8_block_linear(const void* x, int dtype, int64_t M, int64_t K, int64
     if (int rc = check_workspace(what, workspace, workspace_bytes, need)) return rc;
     if (ldx < K) return bad_arg(what, "row stride smaller than a row");
     // The codes the product reads: none where it quantises by itself.
-    const bool direct = few_values(M, K);
+    const bool direct = linear_direct(M, N, K, dtype);
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     const BlockSpace xs(M, K);
     float* scales = reinterpret_cast<float*>(codes + xs.codes);
@@ -186,7 +227,6 @@ int nflow_fp8_block_linear(const void* x, int dtype, int64_t M, int64_t K, int64
     if (M == 0 || N == 0) return NFLOW_OK;
     if (K > 0 && !x) return bad_arg(what, "null x");
     if (direct) {
-        if (N > INT32_MAX) return bad_arg(what, "more than 2^31 - 1 columns");
         launch_block_few_values(a, x, ldx, as_stream(stream));
         return launch_status(what);
     }

@@ -267,7 +267,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
     for (int j = 0; j < TJ; ++j) d[1][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     static_assert(TI % 2 == 0, "the pending sums are those of an odd row tile");
 
-    if constexpr (FP8 && BLOCKS) {
+    if constexpr (FP8 && BLOCKS && T::NS == 2) {
         // One K block: row tile i's products are issued while row tile i - 1's sums
         // join the accumulators (four FMAs behind each product) and row tile i + 1's
         // codes come from LDS.  The block's barrier stands before its last row
@@ -275,7 +275,6 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
         // for the block after next, the next block's stage is complete, and its
         // first fragments arrive under the last row tile's products.  The last
         // sums join in the next block.
-        static_assert(T::NS == 2, "two stages");
         load(k0, 0);
         load(k0 + 1, 1);
         wait_barrier<T::LOADS>();
@@ -414,7 +413,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
 #pragma unroll
                 for (int j = 0; j < 4 * TJ; ++j) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    if (i + 1 < TI) __builtin_amdgcn_sched_group_barrier(0x002, 4 / TJ, 0);   // a conversion
+                    if (i + 1 < TI) __builtin_amdgcn_sched_group_barrier(0x002, TJ >= 4 ? 1 : 4 / TJ, 0);   // conversions
                     if (joins) __builtin_amdgcn_sched_group_barrier(0x002, BLOCKS ? 1 : 2, 0);
                 }
             }

@@ -32,18 +32,23 @@ __global__ __launch_bounds__(256) void k_quantise_rows_blk(const T* __restrict__
         const int64_t c = (b0 + u) * kBlk + 8 * cl;
         load8(row + c, K - c, v[u]);
     }
+    float amax[kRun], inv[kRun], sc;
+#pragma unroll
+    for (int u = 0; u < kRun; ++u) {
+        amax[u] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax[u] = amax_of(amax[u], v[u][e]);
+        amax[u] = max16(amax[u]);
+    }
+    blk_scales<kRun>(amax, sc, inv);
+    if (cl < kRun && b0 + cl < kb) scales[(b0 + cl) * M + m] = sc;
 #pragma unroll
     for (int u = 0; u < kRun; ++u) {
         const int64_t b = b0 + u;
         if (b >= kb) break;
-        float amax = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax = amax_of(amax, v[u][e]);
-        const float sc = blk_scale(max16(amax)), inv = 1.0f / sc;
         *reinterpret_cast<v2u*>(codes + m * kb * kBlk + b * kBlk + 8 * cl) =
-            v2u{blk_pack4(v[u][0], v[u][1], v[u][2], v[u][3], inv),
-                blk_pack4(v[u][4], v[u][5], v[u][6], v[u][7], inv)};
-        if (cl == 0) scales[b * M + m] = sc;
+            v2u{blk_pack4(v[u][0], v[u][1], v[u][2], v[u][3], inv[u]),
+                blk_pack4(v[u][4], v[u][5], v[u][6], v[u][7], inv[u])};
     }
 }
 
@@ -69,6 +74,7 @@ __global__ __launch_bounds__(256) void k_quantise_tile(const T* __restrict__ x, 
     __shared__ __attribute__((aligned(16))) uint8_t lt[kBlk * kBlk];
     __shared__ __attribute__((aligned(16))) float cmax[4][kBlk];
     __shared__ __attribute__((aligned(16))) float csum[4][kBlk];
+    __shared__ __attribute__((aligned(16))) float colinv[kBlk];
     const int tid = threadIdx.x, cl = tid & 15, rg = tid >> 4, wave = tid >> 6, lane = tid & 63;
     const int64_t kb = blk_count(K), mb = blk_count(M);
     const int64_t tm = blockIdx.x / kb, tk = blockIdx.x % kb;
@@ -106,13 +112,12 @@ __global__ __launch_bounds__(256) void k_quantise_tile(const T* __restrict__ x, 
         }
     }
     __syncthreads();
-    float cinv[8], sblk = 0.0f;
+    float cinv[8];
     if constexpr (WEIGHT) {
         float w = 0.0f;
 #pragma unroll
         for (int q = 0; q < 8; ++q) w = fmaxf(w, cmax[q >> 1][64 * (q & 1) + lane]);
-        sblk = blk_scale(wave_max(w));
-        const float inv = 1.0f / sblk;
+        const float sblk = blk_scale(wave_max(w)), inv = 1.0f / sblk;
 #pragma unroll
         for (int e = 0; e < 8; ++e) cinv[e] = inv;
         if (tid == 0) {
@@ -120,39 +125,47 @@ __global__ __launch_bounds__(256) void k_quantise_tile(const T* __restrict__ x, 
             if (o.scales_t) o.scales_t[tm * kb + tk] = sblk;
         }
     } else {
-        if (tid < kBlk && tk * kBlk + tid < K) {
-            if (o.codes_t)
-                o.scales_t[tm * K + tk * kBlk + tid] =
-                    blk_scale(fmaxf(fmaxf(cmax[0][tid], cmax[1][tid]), fmaxf(cmax[2][tid], cmax[3][tid])));
-            if (o.col_sums)
-                o.col_sums[tm * K + tk * kBlk + tid] = (csum[0][tid] + csum[1][tid]) + (csum[2][tid] + csum[3][tid]);
-        }
-        if (o.codes_t) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = 8 * cl + e;
-                cinv[e] = 1.0f / blk_scale(fmaxf(fmaxf(cmax[0][c], cmax[1][c]), fmaxf(cmax[2][c], cmax[3][c])));
+        // A thread per column divides; all read the inverses past the rows' part.
+        if (tid < kBlk) {
+            const float m4 = fmaxf(fmaxf(cmax[0][tid], cmax[1][tid]), fmaxf(cmax[2][tid], cmax[3][tid]));
+            const float sc = blk_scale(m4);
+            if (o.codes_t) {
+                colinv[tid] = 1.0f / sc;
+                if (tk * kBlk + tid < K) o.scales_t[tm * K + tk * kBlk + tid] = sc;
             }
+            if (o.col_sums && tk * kBlk + tid < K)
+                o.col_sums[tm * K + tk * kBlk + tid] = (csum[0][tid] + csum[1][tid]) + (csum[2][tid] + csum[3][tid]);
         }
     }
 
     if (o.codes) {
+        float rinv[8];
+        if constexpr (WEIGHT) {
 #pragma unroll
-        for (int p = 0; p < 8; ++p) {
-            float inv = cinv[0];
-            if constexpr (!WEIGHT) {
-                float amax = 0.0f;
+            for (int p = 0; p < 8; ++p) rinv[p] = cinv[0];
+        } else {
+            float ra[8], sc;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) amax = amax_of(amax, v[p][e]);
-                const float sc = blk_scale(max16(amax));
-                inv = 1.0f / sc;
-                if (cl == 0 && m0 + p < M) o.scales[tk * M + m0 + p] = sc;
+            for (int p = 0; p < 8; ++p) {
+                ra[p] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ra[p] = amax_of(ra[p], v[p][e]);
+                ra[p] = max16(ra[p]);
             }
+            blk_scales<8>(ra, sc, rinv);
+            if (cl < 8 && m0 + cl < M) o.scales[tk * M + m0 + cl] = sc;
+        }
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
             if (m0 + p < M)
                 *reinterpret_cast<v2u*>(o.codes + (m0 + p) * kb * kBlk + c0) =
-                    v2u{blk_pack4(v[p][0], v[p][1], v[p][2], v[p][3], inv),
-                        blk_pack4(v[p][4], v[p][5], v[p][6], v[p][7], inv)};
-        }
+                    v2u{blk_pack4(v[p][0], v[p][1], v[p][2], v[p][3], rinv[p]),
+                        blk_pack4(v[p][4], v[p][5], v[p][6], v[p][7], rinv[p])};
+    }
+    if (!WEIGHT && o.codes_t) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cinv[e] = colinv[8 * cl + e];
     }
     if (o.codes_t) {
 #pragma unroll

@@ -137,29 +137,39 @@ __global__ __launch_bounds__(row_threads<L>()) void k_norm(NormArgs a, int64_t p
             if (a.mean) a.mean[m] = mean;
             if (a.rstd) a.rstd[m] = rstd;
         }
+        float y[NV][8];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int c = 8 * (t + L * j), left = D - c;
-            float y[8];
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = norm_value(v[j][e], rstd, w[j][e], b[j][e]);
-            if constexpr (!FP8) {
-                store8(static_cast<T*>(a.y) + m * a.ldy + c, on ? left : 0, y);
-            } else {
-                // 16 threads hold a block of 128; columns past D count as 0.
-                const int kb = static_cast<int>(blk_count(D)), blk = c / kBlk;
+            for (int e = 0; e < 8; ++e) y[j][e] = norm_value(v[j][e], rstd, w[j][e], b[j][e]);
+        if constexpr (!FP8) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = 8 * (t + L * j);
+                store8(static_cast<T*>(a.y) + m * a.ldy + c, on ? D - c : 0, y[j]);
+            }
+        } else {
+            // 16 threads hold a block of 128; columns past D count as 0.  (Sharing
+            // the blocks' divisions among the lanes, as the quantise does, is
+            // slower here, 54.0 against 51.5 us at 16384 x 4096 bf16: a row is a
+            // chain of reductions, and this lengthens it.)
+            const int kb = static_cast<int>(blk_count(D));
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = 8 * (t + L * j), left = D - c;
                 if (left < 8) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = e < left ? y[e] : 0.0f;
+                    for (int e = 0; e < 8; ++e) y[j][e] = e < left ? y[j][e] : 0.0f;
                 }
                 float amax = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) amax = amax_of(amax, y[e]);
+                for (int e = 0; e < 8; ++e) amax = amax_of(amax, y[j][e]);
                 const float sc = blk_scale(max16(amax)), inv = 1.0f / sc;
-                if (on && blk < kb) {
+                if (on && c / kBlk < kb) {
                     *reinterpret_cast<v2u*>(a.codes + m * kb * kBlk + c) =
-                        v2u{blk_pack4(y[0], y[1], y[2], y[3], inv), blk_pack4(y[4], y[5], y[6], y[7], inv)};
-                    if (t % 16 == 0) a.scales[blk * a.M + m] = sc;
+                        v2u{blk_pack4(y[j][0], y[j][1], y[j][2], y[j][3], inv),
+                            blk_pack4(y[j][4], y[j][5], y[j][6], y[j][7], inv)};
+                    if (t % 16 == 0) a.scales[c / kBlk * a.M + m] = sc;
                 }
             }
         }
@@ -401,8 +411,10 @@ __global__ __launch_bounds__(1024) void k_norm_grad_join(const float* __restrict
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * 64 + lane;
     float v = 0.0f;
-    if (n < 2 * D)
+    if (n < 2 * D) {
+#pragma unroll 8
         for (int64_t p = wave; p < P; p += 16) v += part[p * 2 * D + n];
+    }
     s[wave][lane] = v;
     __syncthreads();
     if (wave == 0 && n < 2 * D) {
