@@ -36,19 +36,34 @@ using TileBig = BlockTile<2, 4, 8, 4, 2>;     // 256 x 256, eight waves, a workg
 using TileMid = BlockTile<2, 2, 4, 4, 2>;     // 128 x 128, four waves, two workgroups per CU
 using TileSmall = BlockTile<2, 2, 2, 2, 4>;   // 64 x 64, four waves, two workgroups per CU, loads three steps ahead
 
+template <typename T>
+GemmShare gemm_share(const BlockGemmArgs& a, int splits, float* part) {
+    const int64_t tm = (a.M + T::BM - 1) / T::BM, tn = (a.N + T::BN - 1) / T::BN;
+    const int kb = static_cast<int>(blk_count(a.K));
+    return GemmShare{tm, tn, splits, (kb + splits - 1) / splits, part, static_cast<int>(tm * tn * splits)};
+}
+
+// A kernel with T's stages as its dynamic LDS.
+template <typename T, auto k, typename... Args>
+void launch_staged(int blocks, hipStream_t st, Args... args) {
+    constexpr int bytes = T::NS * T::STAGE;
+    static const hipError_t once =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    (void)once;
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(T::THREADS), bytes, st, args...);
+}
+
 template <typename TO, bool BLOCKS, typename T>
 void launch_tiles(const BlockGemmArgs& a, int splits, float* part, hipStream_t st) {
-    auto k = k_block_gemm<TO, BLOCKS, T>;
-    static const bool once = [&] {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                  T::NS * T::STAGE);
-        return true;
-    }();
-    (void)once;
-    const int64_t tm = (a.M + T::BM - 1) / T::BM, tn = (a.N + T::BN - 1) / T::BN;
-    const int kb = static_cast<int>(blk_count(a.K)), per = splits > 1 ? (kb + splits - 1) / splits : kb;
-    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(tm * tn * splits)), dim3(T::THREADS), T::NS * T::STAGE, st, a,
-                       tm, tn, splits, per, part);
+    const GemmShare sh = gemm_share<T>(a, splits, part);
+    launch_staged<T, &k_block_gemm<TO, BLOCKS, T>>(sh.blocks, st, a, sh);
+}
+
+template <typename TO>
+void launch_join(const BlockGemmArgs& a, int splits, const float* part, hipStream_t st) {
+    if (splits > 1)
+        hipLaunchKernelGGL((k_block_gemm_join<TO>), dim3(grid_for(a.M * ((a.N + 3) / 4), 256, 8)), dim3(256), 0, st, a,
+                           part, splits);
 }
 
 // How a product is cut: the kernel or tile, and the number of runs of K blocks
@@ -112,9 +127,7 @@ void launch_gemm(const BlockGemmArgs& a, const GemmPlan& p, float* part, hipStre
     }
     if (p.kind == GEMM_MID) launch_tiles<TO, BLOCKS, TileMid>(a, p.splits, part, st);
     if (p.kind == GEMM_SMALL) launch_tiles<TO, BLOCKS, TileSmall>(a, p.splits, part, st);
-    if (p.splits > 1)
-        hipLaunchKernelGGL((k_block_gemm_join<TO>), dim3(grid_for(a.M * ((a.N + 3) / 4), 256, 8)), dim3(256), 0, st, a,
-                           part, p.splits);
+    launch_join<TO>(a, p.splits, part, st);
 }
 
 int block_gemm(const char* what, const BlockGemmArgs& a, void* ws, hipStream_t st) {
@@ -133,6 +146,25 @@ int block_gemm(const char* what, const BlockGemmArgs& a, void* ws, hipStream_t s
         else launch_gemm<float, false>(a, p, part, st);
     }
     return launch_status(what);
+}
+
+// The two products of the fp32 backward pass, a (row scales) and b (block
+// scales), in one launch where both take 128 x 128 tiles.
+int block_gemm_both(const char* what, const BlockGemmArgs& a, const BlockGemmArgs& b, void* ws_a, void* ws_b,
+                    hipStream_t st) {
+    if (a.M > 0 && a.N > 0 && b.M > 0 && b.N > 0 && a.out == NFLOW_DTYPE_F32 && b.out == NFLOW_DTYPE_F32) {
+        const GemmPlan pa = gemm_plan(a.M, a.N, a.K, a.out), pb = gemm_plan(b.M, b.N, b.K, b.out);
+        if (pa.kind == GEMM_MID && pb.kind == GEMM_MID) {
+            float *fa = static_cast<float*>(ws_a), *fb = static_cast<float*>(ws_b);
+            const GemmShare sa = gemm_share<TileMid>(a, pa.splits, fa), sb = gemm_share<TileMid>(b, pb.splits, fb);
+            launch_staged<TileMid, &k_block_gemm_pair<TileMid>>(sa.blocks + sb.blocks, st, a, sa, b, sb);
+            launch_join<float>(a, pa.splits, fa, st);
+            launch_join<float>(b, pb.splits, fb, st);
+            return launch_status(what);
+        }
+    }
+    if (int rc = block_gemm(what, a, ws_a, st)) return rc;
+    return block_gemm(what, b, ws_b, st);
 }
 
 // Whether linear is one launch of the few-row kernel on x's values.
@@ -243,7 +275,7 @@ int nflow_fp8_block_linear_backward_workspace(int64_t M, int64_t N, int64_t K, i
     size_t dx = 0, dw = 0;
     if (int rc = nflow_fp8_block_matmul_workspace(M, K, N, dtype, &dx)) return rc;
     if (int rc = nflow_fp8_block_matmul_workspace(N, K, M, NFLOW_DTYPE_F32, &dw)) return rc;
-    *bytes = round16(std::max(dx, dw)) + BlockSpace(M, N).bytes() + BlockSpace(N, M).bytes() +
+    *bytes = round16(dw) + round16(dx) + BlockSpace(M, N).bytes() + BlockSpace(N, M).bytes() +
              round16(static_cast<size_t>(blk_count(M)) * static_cast<size_t>(N) * sizeof(float));
     return NFLOW_OK;
 }
@@ -273,18 +305,17 @@ int nflow_fp8_block_linear_backward(const void* dy, int dtype, int64_t M, int64_
         if (int rc = check_gemm(what, aw)) return rc;
     float* sums = reinterpret_cast<float*>(t + cols.bytes());
     const size_t sum_bytes = round16(static_cast<size_t>(blk_count(M)) * N * sizeof(float));
-    void* parts = t + cols.bytes() + sum_bytes;
+    uint8_t* parts = t + cols.bytes() + sum_bytes;      // dW's partial results, then dx's
+    const size_t part_dw = round16(gemm_plan(N, K, M, NFLOW_DTYPE_F32).bytes);
     if (M > 0 && N > 0 && (dx || dW || dbias))
         if (int rc = block_quantise(what, dy, dtype, M, N, lddy, dx ? q : nullptr, dx ? sq : nullptr,
                                     dW ? t : nullptr, dW ? stt : nullptr, dbias ? sums : nullptr, st))
             return rc;
     if (dbias && N > 0)
         if (int rc = sum_parts(what, sums, blk_count(M), N, dbias, st)) return rc;
-    if (dx)
-        if (int rc = block_gemm(what, ax, parts, st)) return rc;
-    if (dW)
-        if (int rc = block_gemm(what, aw, parts, st)) return rc;
-    return NFLOW_OK;
+    if (dx && dW) return block_gemm_both(what, aw, ax, parts, parts + part_dw, st);
+    if (dx) return block_gemm(what, ax, parts + part_dw, st);
+    return dW ? block_gemm(what, aw, parts, st) : NFLOW_OK;
 }
 
 }  // extern "C"

@@ -179,9 +179,14 @@ __device__ __forceinline__ void store_tiles(const v4f (&acc)[TI][TJ], float* str
 // per 128 x 128), else one per row of W.  With splits > 1 the K blocks are
 // dealt out in runs of `per`, and split s writes its fp32 sums, unscaled by
 // anything further, to part[s] (M, N).
+struct GemmShare {
+    int64_t tiles_m, tiles_n;
+    int splits, per;
+    float* part;
+    int blocks;         // workgroups of the product
+};
 template <typename TO, bool BLOCKS, typename T>
-__global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, int64_t tiles_m, int64_t tiles_n,
-                                                              int splits, int per, float* part) {
+__device__ __forceinline__ void gemm_tile(const BlockGemmArgs& a, const GemmShare& sh, int bid) {
     constexpr bool FP8 = std::is_same_v<TO, bf16>;
     constexpr int TI = T::TI, TJ = T::TJ, BM = T::BM, BN = T::BN, LEAD = T::NS - 1;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -189,9 +194,10 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wid / T::WN, wn = wid % T::WN;
     const int r = lane & 15, g = lane >> 4;
-    const int64_t t = gemm_tile_of_block(blockIdx.x, gridDim.x, 8);
+    const int64_t t = gemm_tile_of_block(bid, sh.blocks, 8);
+    const int splits = sh.splits, per = sh.per;
     const int split = splits > 1 ? static_cast<int>(t % splits) : 0;
-    const TilePos pos = tile_pos(splits > 1 ? t / splits : t, tiles_m, tiles_n, 4);
+    const TilePos pos = tile_pos(splits > 1 ? t / splits : t, sh.tiles_m, sh.tiles_n, 4);
     const int64_t m0 = pos.tm * BM, n0 = pos.tn * BN;
     const int kb = static_cast<int>(blk_count(a.K));
     const int k0 = split * per, k1 = k0 + per < kb ? k0 + per : kb;
@@ -440,10 +446,25 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, i
     __syncthreads();
     float* strip = reinterpret_cast<float*>(lds) + wid * T::STRIP;
     if (splits > 1)
-        store_tiles<float, T, false>(acc, strip, part + split * a.M * a.N, a.M, a.N, a.N, nullptr, NFLOW_ACT_NONE,
+        store_tiles<float, T, false>(acc, strip, sh.part + split * a.M * a.N, a.M, a.N, a.N, nullptr, NFLOW_ACT_NONE,
                               m0 + xat, ncol);
     else
         store_tiles<TO, T, true>(acc, strip, static_cast<TO*>(a.C), a.M, a.N, a.ldc, a.bias, a.act, m0 + xat, ncol);
+}
+
+template <typename TO, bool BLOCKS, typename T>
+__global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm(BlockGemmArgs a, GemmShare sh) {
+    gemm_tile<TO, BLOCKS, T>(a, sh, blockIdx.x);
+}
+
+// Two independent fp32 products in one launch, a's workgroups first: where
+// neither fills the chip evenly by itself, one's workgroups run in the CUs that
+// the other leaves idle at its end.
+template <typename T>
+__global__ __launch_bounds__(T::THREADS, 2) void k_block_gemm_pair(BlockGemmArgs a, GemmShare sa, BlockGemmArgs b,
+                                                                   GemmShare sb) {
+    if (static_cast<int>(blockIdx.x) < sa.blocks) gemm_tile<float, false, T>(a, sa, blockIdx.x);
+    else gemm_tile<float, true, T>(b, sb, blockIdx.x - sa.blocks);
 }
 
 }  // namespace nfq
