@@ -18,7 +18,7 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .quant import _act, _p, _stream
+from .quant import _act, _p
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
@@ -106,6 +106,14 @@ def _empty_block(R: int, K: int, device) -> BlockFp8:
                     torch.empty(kb, R, dtype=torch.float32, device=device), K)
 
 
+def _stream(t: torch.Tensor) -> int:
+    """The current stream's handle, on t's device, which has to be the current one."""
+    i = t.get_device()
+    if i != torch._C._cuda_getDevice():
+        raise ValueError(f"the tensors are on cuda:{i}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return torch._C._cuda_getCurrentRawStream(i)
+
+
 def _workspace(n: int, device) -> Optional[torch.Tensor]:
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
@@ -117,7 +125,7 @@ def quantise(x: torch.Tensor) -> BlockFp8:
     M, K, ldx = _matrix(x, "x")
     q = _empty_block(M, K, x.device)
     check(_lib.lib().nflow_fp8_block_quantise(_p(x), _dtype(x), M, K, ldx, _p(q.codes), _p(q.scales), None, None,
-                                              _stream()), "fp8_block_quantise")
+                                              _stream(x)), "fp8_block_quantise")
     return q
 
 
@@ -127,7 +135,7 @@ def quantise_columns(x: torch.Tensor) -> BlockFp8:
     M, K, ldx = _matrix(x, "x")
     t = _empty_block(K, M, x.device)
     check(_lib.lib().nflow_fp8_block_quantise(_p(x), _dtype(x), M, K, ldx, None, None, _p(t.codes), _p(t.scales),
-                                              _stream()), "fp8_block_quantise")
+                                              _stream(x)), "fp8_block_quantise")
     return t
 
 
@@ -137,7 +145,7 @@ def quantise_both(x: torch.Tensor) -> Tuple[BlockFp8, BlockFp8]:
     M, K, ldx = _matrix(x, "x")
     q, t = _empty_block(M, K, x.device), _empty_block(K, M, x.device)
     check(_lib.lib().nflow_fp8_block_quantise(_p(x), _dtype(x), M, K, ldx, _p(q.codes), _p(q.scales), _p(t.codes),
-                                              _p(t.scales), _stream()), "fp8_block_quantise")
+                                              _p(t.scales), _stream(x)), "fp8_block_quantise")
     return q, t
 
 
@@ -154,7 +162,7 @@ def quantise_weight(W: torch.Tensor, transposed: bool = False):
                      torch.empty(nb, kb, dtype=torch.float32, device=W.device), N)
     check(_lib.lib().nflow_fp8_block_quantise_weight(_p(W), _dtype(W), N, K, ldw, _p(w.codes), _p(w.scales),
                                                      _p(t.codes) if t else None, _p(t.scales) if t else None,
-                                                     _stream()), "fp8_block_quantise_weight")
+                                                     _stream(W)), "fp8_block_quantise_weight")
     return (w, t) if transposed else w
 
 
@@ -178,7 +186,7 @@ def matmul(a: BlockFp8, w: BlockFp8, bias: Optional[torch.Tensor] = None, activa
     check(L.nflow_fp8_block_matmul_workspace(M, N, a.k, dt, C.byref(n)), "fp8_block_matmul")
     ws = _workspace(n.value, out.device)
     check(L.nflow_fp8_block_matmul(_p(a.codes), _p(a.scales), _p(w.codes), _p(w.scales), int(blocks), M, N, a.k,
-                                   _p(bias), _act(activation), _p(out), dt, N, _p(ws), n.value, _stream()),
+                                   _p(bias), _act(activation), _p(out), dt, N, _p(ws), n.value, _stream(out)),
           "fp8_block_matmul")
     return out
 
@@ -197,7 +205,7 @@ def linear(x: torch.Tensor, w: BlockFp8, bias: Optional[torch.Tensor] = None, ac
     check(L.nflow_fp8_block_linear_workspace(M, N, K, dt, C.byref(n)), "fp8_block_linear")
     ws = _workspace(n.value, x.device)
     check(L.nflow_fp8_block_linear(_p(x), dt, M, K, ldx, _p(w.codes), _p(w.scales), N, _p(bias), _act(activation),
-                                   _p(y), N, _p(ws), n.value, _stream()), "fp8_block_linear")
+                                   _p(y), N, _p(ws), n.value, _stream(x)), "fp8_block_linear")
     return y
 
 
@@ -221,5 +229,5 @@ def linear_backward(dy: torch.Tensor, x_columns: BlockFp8, w_transposed: BlockFp
     ws = _workspace(n.value, dy.device)
     check(L.nflow_fp8_block_linear_backward(_p(dy), dt, M, N, lddy, _p(x_columns.codes), _p(x_columns.scales),
                                             _p(w_transposed.codes), _p(w_transposed.scales), K, _p(dx), K, _p(dW),
-                                            _p(db), _p(ws), n.value, _stream()), "fp8_block_linear_backward")
+                                            _p(db), _p(ws), n.value, _stream(dy)), "fp8_block_linear_backward")
     return dx, dW, db

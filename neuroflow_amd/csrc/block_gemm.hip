@@ -196,6 +196,31 @@ struct BlockSpace {
     size_t bytes() const { return codes + scales; }
 };
 
+size_t matmul_space(int64_t M, int64_t N, int64_t K, int out) {
+    return M > 0 && N > 0 ? gemm_plan(M, N, K, out).bytes : 0;
+}
+size_t linear_space(int64_t M, int64_t N, int64_t K, int dtype) {
+    if (M == 0 || N == 0 || linear_direct(M, N, K, dtype)) return 0;
+    return BlockSpace(M, K).bytes() + matmul_space(M, N, K, dtype);
+}
+struct BackwardSpace {
+    BlockSpace rows, cols;
+    size_t sums, part_w, part_x;
+    BackwardSpace(int64_t M, int64_t N, int64_t K, int dtype)
+        : rows(M, N), cols(N, M), sums(round16(static_cast<size_t>(blk_count(M) * N) * sizeof(float))),
+          part_w(round16(matmul_space(N, K, M, NFLOW_DTYPE_F32))), part_x(round16(matmul_space(M, K, N, dtype))) {}
+    size_t bytes() const { return rows.bytes() + cols.bytes() + sums + part_w + part_x; }
+};
+
+// Sizes and type ahead of anything that is worked out from them; *bytes = 0.
+int check_sizes(const char* what, int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
+    if (!bytes) return bad_arg(what, "null output");
+    *bytes = 0;
+    if (M < 0 || N < 0 || K < 0) return bad_arg(what, "bad dims");
+    if (!dtype_ok(dtype)) return bad_arg(what, "unknown dtype");
+    return NFLOW_OK;
+}
+
 }  // namespace
 }  // namespace nfq
 
@@ -205,11 +230,8 @@ extern "C" {
 
 int nflow_fp8_block_matmul_workspace(int64_t M, int64_t N, int64_t K, int c_dtype, size_t* bytes) {
     clear_error();
-    if (!bytes) return bad_arg("fp8_block_matmul_workspace", "null output");
-    *bytes = 0;
-    if (M < 0 || N < 0 || K < 0) return bad_arg("fp8_block_matmul_workspace", "bad dims");
-    if (!dtype_ok(c_dtype)) return bad_arg("fp8_block_matmul_workspace", "unknown dtype");
-    if (M > 0 && N > 0) *bytes = gemm_plan(M, N, K, c_dtype).bytes;
+    if (int rc = check_sizes("fp8_block_matmul_workspace", M, N, K, c_dtype, bytes)) return rc;
+    *bytes = matmul_space(M, N, K, c_dtype);
     return NFLOW_OK;
 }
 
@@ -221,18 +243,14 @@ int nflow_fp8_block_matmul(const uint8_t* A, const float* scale_A, const uint8_t
     const char* what = "fp8_block_matmul";
     const BlockGemmArgs a{A, scale_A, W, scale_W, w_blocks != 0, M, N, K, bias, activation, C, c_dtype, ldc};
     if (int rc = check_gemm(what, a)) return rc;
-    size_t need = 0;
-    if (int rc = nflow_fp8_block_matmul_workspace(M, N, K, c_dtype, &need)) return rc;
-    if (int rc = check_workspace(what, workspace, workspace_bytes, need)) return rc;
+    if (int rc = check_workspace(what, workspace, workspace_bytes, matmul_space(M, N, K, c_dtype))) return rc;
     return block_gemm(what, a, workspace, as_stream(stream));
 }
 
 int nflow_fp8_block_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
     clear_error();
-    if (!bytes) return bad_arg("fp8_block_linear_workspace", "null output");
-    *bytes = 0;
-    if (int rc = nflow_fp8_block_matmul_workspace(M, N, K, dtype, bytes)) return rc;
-    if (!linear_direct(M, N, K, dtype)) *bytes = round16(*bytes) + BlockSpace(M, K).bytes();
+    if (int rc = check_sizes("fp8_block_linear_workspace", M, N, K, dtype, bytes)) return rc;
+    *bytes = linear_space(M, N, K, dtype);
     return NFLOW_OK;
 }
 
@@ -242,8 +260,8 @@ int nflow_fp8_block_linear(const void* x, int dtype, int64_t M, int64_t K, int64
     clear_error();
     const char* what = "fp8_block_linear";
     size_t need = 0;
-    if (int rc = nflow_fp8_block_linear_workspace(M, N, K, dtype, &need)) return rc;
-    if (int rc = check_workspace(what, workspace, workspace_bytes, need)) return rc;
+    if (int rc = check_sizes(what, M, N, K, dtype, &need)) return rc;
+    if (int rc = check_workspace(what, workspace, workspace_bytes, linear_space(M, N, K, dtype))) return rc;
     if (ldx < K) return bad_arg(what, "row stride smaller than a row");
     // The codes the product reads: none where it quantises by itself.
     const bool direct = linear_direct(M, N, K, dtype);
@@ -270,13 +288,8 @@ int nflow_fp8_block_linear(const void* x, int dtype, int64_t M, int64_t K, int64
 
 int nflow_fp8_block_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
     clear_error();
-    if (!bytes) return bad_arg("fp8_block_linear_backward_workspace", "null output");
-    *bytes = 0;
-    size_t dx = 0, dw = 0;
-    if (int rc = nflow_fp8_block_matmul_workspace(M, K, N, dtype, &dx)) return rc;
-    if (int rc = nflow_fp8_block_matmul_workspace(N, K, M, NFLOW_DTYPE_F32, &dw)) return rc;
-    *bytes = round16(dw) + round16(dx) + BlockSpace(M, N).bytes() + BlockSpace(N, M).bytes() +
-             round16(static_cast<size_t>(blk_count(M)) * static_cast<size_t>(N) * sizeof(float));
+    if (int rc = check_sizes("fp8_block_linear_backward_workspace", M, N, K, dtype, bytes)) return rc;
+    *bytes = BackwardSpace(M, N, K, dtype).bytes();
     return NFLOW_OK;
 }
 
@@ -287,35 +300,36 @@ int nflow_fp8_block_linear_backward(const void* dy, int dtype, int64_t M, int64_
     clear_error();
     const char* what = "fp8_block_linear_backward";
     size_t need = 0;
-    if (int rc = nflow_fp8_block_linear_backward_workspace(M, N, K, dtype, &need)) return rc;
-    if (int rc = check_workspace(what, workspace, workspace_bytes, need)) return rc;
+    if (int rc = check_sizes(what, M, N, K, dtype, &need)) return rc;
+    const BackwardSpace sp(M, N, K, dtype);
+    if (int rc = check_workspace(what, workspace, workspace_bytes, sp.bytes())) return rc;
     if (lddy < N) return bad_arg(what, "row stride smaller than a row");
     if (M > 0 && N > 0 && !dy) return bad_arg(what, "null dy");
     hipStream_t st = as_stream(stream);
+    // dy's codes and scales along its rows and its columns, the sums of 128 of
+    // its rows, the partial results of dW and of dx.
     uint8_t* q = static_cast<uint8_t*>(workspace);
-    const BlockSpace rows(M, N), cols(N, M);
-    float* sq = reinterpret_cast<float*>(q + rows.codes);
-    uint8_t* t = q + rows.bytes();
-    float* stt = reinterpret_cast<float*>(t + cols.codes);
+    float* sq = reinterpret_cast<float*>(q + sp.rows.codes);
+    uint8_t* t = q + sp.rows.bytes();
+    float* stt = reinterpret_cast<float*>(t + sp.cols.codes);
+    float* sums = reinterpret_cast<float*>(t + sp.cols.bytes());
+    uint8_t* part_w = t + sp.cols.bytes() + sp.sums;
+    uint8_t* part_x = part_w + sp.part_w;
     const BlockGemmArgs ax{q, sq, W_t, scale_W_t, true, M, K, N, nullptr, NFLOW_ACT_NONE, dx, dtype, lddx};
     const BlockGemmArgs aw{t, stt, x_t, scale_x_t, false, N, K, M, nullptr, NFLOW_ACT_NONE, dW, NFLOW_DTYPE_F32, K};
     if (dx)
         if (int rc = check_gemm(what, ax)) return rc;
     if (dW)
         if (int rc = check_gemm(what, aw)) return rc;
-    float* sums = reinterpret_cast<float*>(t + cols.bytes());
-    const size_t sum_bytes = round16(static_cast<size_t>(blk_count(M)) * N * sizeof(float));
-    uint8_t* parts = t + cols.bytes() + sum_bytes;      // dW's partial results, then dx's
-    const size_t part_dw = round16(gemm_plan(N, K, M, NFLOW_DTYPE_F32).bytes);
     if (M > 0 && N > 0 && (dx || dW || dbias))
         if (int rc = block_quantise(what, dy, dtype, M, N, lddy, dx ? q : nullptr, dx ? sq : nullptr,
                                     dW ? t : nullptr, dW ? stt : nullptr, dbias ? sums : nullptr, st))
             return rc;
     if (dbias && N > 0)
         if (int rc = sum_parts(what, sums, blk_count(M), N, dbias, st)) return rc;
-    if (dx && dW) return block_gemm_both(what, aw, ax, parts, parts + part_dw, st);
-    if (dx) return block_gemm(what, ax, parts + part_dw, st);
-    return dW ? block_gemm(what, aw, parts, st) : NFLOW_OK;
+    if (dx && dW) return block_gemm_both(what, aw, ax, part_w, part_x, st);
+    if (dx) return block_gemm(what, ax, part_x, st);
+    return dW ? block_gemm(what, aw, part_w, st) : NFLOW_OK;
 }
 
 }  // extern "C"

@@ -432,6 +432,10 @@ constexpr int64_t kNormRegMax = 16384;
 // Workgroups (and partial rows) of the backward pass.
 int64_t grad_blocks(int64_t M) { return std::min<int64_t>(M, num_cus()); }
 
+size_t grad_space(int64_t M, int64_t D) {
+    return static_cast<size_t>(grad_blocks(M)) * 2 * static_cast<size_t>(D) * sizeof(float);
+}
+
 unsigned row_grid(int64_t M) { return static_cast<unsigned>(std::min<int64_t>(M, 8 * num_cus())); }
 
 // Workgroups of `threads` that run at once, from the kernel's registers and LDS.
@@ -546,7 +550,7 @@ int nflow_layer_norm_backward_workspace(int64_t M, int64_t D, size_t* bytes) {
     if (!bytes) return bad_arg("layer_norm_backward_workspace", "null output");
     *bytes = 0;
     if (M < 0 || D <= 0) return bad_arg("layer_norm_backward_workspace", "bad dims");
-    *bytes = static_cast<size_t>(grad_blocks(M)) * 2 * static_cast<size_t>(D) * sizeof(float);
+    *bytes = grad_space(M, D);
     return NFLOW_OK;
 }
 
@@ -559,12 +563,11 @@ int nflow_layer_norm_backward(const void* dy, const void* x, int dtype, int64_t 
     if (int rc = check_norm(what, x, dtype, M, D, ldx, 0.0f)) return rc;
     if (lddy < D || lddx < D) return bad_arg(what, "row stride smaller than a row");
     if (M > 0 && (!dy || !mean || !rstd || !dx)) return bad_arg(what, "null dy, mean, rstd or dx");
-    size_t need = 0;
-    if (int rc = nflow_layer_norm_backward_workspace(M, D, &need)) return rc;
-    if (int rc = check_workspace(what, workspace, workspace_bytes, need)) return rc;
+    if (int rc = check_workspace(what, workspace, workspace_bytes, grad_space(M, D))) return rc;
     hipStream_t st = as_stream(stream);
     const int64_t nb = grad_blocks(M);
     const bool params = dweight || dbias;
+    if (M == 0 && !params) return NFLOW_OK;
     const NormGradArgs a{dy, x, M, D, lddy, ldx, weight, mean, rstd, dx, lddx,
                          params ? static_cast<float*>(workspace) : nullptr, nb ? (M + nb - 1) / nb : 0};
     if (M > 0) {

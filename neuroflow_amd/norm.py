@@ -15,8 +15,8 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .block_fp8 import BlockFp8, _activation, _dtype, _empty_block, _matrix, _param, _workspace
-from .quant import _p, _stream
+from .block_fp8 import _activation, _dtype, _empty_block, _matrix, _param, _stream, _workspace
+from .quant import _p
 
 
 def _params(D: int, weight, bias) -> None:
@@ -44,7 +44,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         y, ldy = out, _matrix(_activation(out, "out", like=x), "out")[2]
     mean, rstd = _stats(M, x, return_stats)
     check(_lib.lib().nflow_layer_norm_forward(_p(x), _dtype(x), M, D, ldx, _p(weight), _p(bias), float(eps), _p(y),
-                                              ldy, _p(mean), _p(rstd), _stream()), "layer_norm")
+                                              ldy, _p(mean), _p(rstd), _stream(x)), "layer_norm")
     return (y, mean, rstd) if return_stats else y
 
 
@@ -57,7 +57,7 @@ def layer_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
     q = _empty_block(M, D, x.device)
     mean, rstd = _stats(M, x, return_stats)
     check(_lib.lib().nflow_layer_norm_fp8_block(_p(x), _dtype(x), M, D, ldx, _p(weight), _p(bias), float(eps),
-                                                _p(q.codes), _p(q.scales), _p(mean), _p(rstd), _stream()),
+                                                _p(q.codes), _p(q.scales), _p(mean), _p(rstd), _stream(x)),
           "layer_norm_fp8")
     return (q, mean, rstd) if return_stats else q
 
@@ -80,6 +80,6 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     check(L.nflow_layer_norm_backward_workspace(M, D, C.byref(n)), "layer_norm_backward")
     ws = _workspace(n.value, x.device)
     check(L.nflow_layer_norm_backward(_p(dy), _p(x), _dtype(x), M, D, lddy, ldx, _p(weight), _p(mean), _p(rstd),
-                                      _p(dx), D, _p(dw), dw.data_ptr() + 4 * D, _p(ws), n.value, _stream()),
+                                      _p(dx), D, _p(dw), dw.data_ptr() + 4 * D, _p(ws), n.value, _stream(x)),
           "layer_norm_backward")
     return dx, dw[0], dw[1]

@@ -165,6 +165,18 @@ def test_matmul(gpu, M, N, K, out):
 
 
 @pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 256), (4001, 4099, 300), (512, 1024, 8192), (65, 1000, 8200), (64, 2000, 8192),
+                                   (1, 8192, 2048), (20000, 768, 256)])
+def test_matmul_cuts(gpu, M, N, K, out):
+    """Enough rows and columns for each tile, and few enough for splits over K."""
+    bias = WL.uniform(305, (N,), -1, 1).astype(np.float32)
+    for wide in (False, True):
+        a, w = _operands(306 + M + N + K, M, N, K, wide)
+        y = B.matmul(_block(a, K), _block(w, K), torch.from_numpy(bias).cuda(), "relu", out)
+        _check(y, a, w, bias, "relu", K)
+
+
+@pytest.mark.parametrize("out", [F32, BF16])
 @pytest.mark.parametrize("M", [1, 5, 40, 300])
 def test_matmul_all_codes(gpu, M, out):
     """Every finite code in both operands, scales over many magnitudes."""
@@ -238,7 +250,8 @@ def test_linear_nonfinite_rows(gpu, M, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 300, 200), (5, 128, 128), (64, 768, 256), (129, 130, 131), (1000, 200, 77),
-                                   (515, 385, 1000), (4099, 256, 300), (20000, 64, 96)])
+                                   (515, 385, 1000), (4099, 256, 300), (20000, 64, 96),
+                                   (5003, 1544, 1000)])
 def test_linear_backward(gpu, M, N, K, dtype):
     t, x = _x(340 + M + N + K, M, K, dtype)
     dyt, dy = _x(350 + M + N + K, M, N, dtype)
