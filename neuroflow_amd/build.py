@@ -1,12 +1,12 @@
 """Build libnflow_quant.so (the gfx950 kernels + C-ABI) in-tree, and the
-pybind11 module neuroflow_cpp on top of it.
+pybind11 modules neuroflow_cpp and block_ops on top of it.
 
     python -m neuroflow_amd.build
 
 Compiles neuroflow_amd/csrc/*.hip and *.cpp with hipcc for gfx950 and links
 neuroflow_amd/lib/libnflow_quant.so; then compiles
-neuroflow_amd/bindings/neuroflow_cpp.cpp (host code only) into
-neuroflow_amd/lib/neuroflow_cpp<ext>, which loads the library from its own
+neuroflow_amd/bindings/*.cpp (host code only) into
+neuroflow_amd/lib/<name><ext>, which load the library from their own
 directory.  Flags:
   -ffp-contract=off   float expressions round in the written order (the
                       dequantise step must match the reference bit for bit);
@@ -49,21 +49,18 @@ def _compile(src: Path, obj: Path) -> None:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
 
 
-def build_bindings(verbose: bool = True) -> Path:
-    """neuroflow_cpp: g++ against pybind11 and the Python headers, linked to
+def _build_binding(name: str, flags: list[str], verbose: bool) -> Path:
+    """bindings/<name>.cpp with g++ against the Python headers, linked to
     libnflow_quant.so with an $ORIGIN rpath."""
     import sysconfig
 
-    import pybind11
-
-    out = LIB_DIR / ("neuroflow_cpp" + sysconfig.get_config_var("EXT_SUFFIX"))
+    out = LIB_DIR / (name + sysconfig.get_config_var("EXT_SUFFIX"))
     rocm = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
     tmp = out.with_name(out.name + ".tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__",
-           "-I", str(PKG.parent / "include"), "-I", pybind11.get_include(), "-I", sysconfig.get_paths()["include"],
-           "-I", str(rocm / "include"), str(PKG / "bindings" / "neuroflow_cpp.cpp"), "-o", str(tmp),
-           "-L", str(LIB_DIR), "-lnflow_quant", "-Wl,-rpath,$ORIGIN", "-L", str(rocm / "lib"), "-lamdhip64",
-           "-Wl,-rpath," + str(rocm / "lib")]
+           "-I", str(PKG.parent / "include"), "-I", sysconfig.get_paths()["include"], "-I", str(rocm / "include"),
+           str(PKG / "bindings" / f"{name}.cpp"), "-o", str(tmp), "-L", str(LIB_DIR), "-lnflow_quant",
+           "-Wl,-rpath,$ORIGIN", "-L", str(rocm / "lib"), "-lamdhip64", "-Wl,-rpath," + str(rocm / "lib"), *flags]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"bindings build failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
@@ -71,6 +68,21 @@ def build_bindings(verbose: bool = True) -> Path:
     if verbose:
         print(f"built {out}")
     return out
+
+
+def build_bindings(verbose: bool = True) -> Path:
+    """neuroflow_cpp, against pybind11; and block_ops, against torch's headers
+    and its pybind11 (torch's libraries are in the process by the time it is
+    imported)."""
+    import pybind11
+    import torch
+
+    t = Path(torch.__file__).resolve().parent
+    _build_binding("block_ops", ["-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                                 "-I", str(t / "include"), "-I", str(t / "include" / "torch" / "csrc" / "api" / "include"),
+                                 "-L", str(t / "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip"],
+                   verbose)
+    return _build_binding("neuroflow_cpp", ["-I", pybind11.get_include()], verbose)
 
 
 def build(verbose: bool = True, lib: Path = LIB) -> Path:

@@ -203,7 +203,9 @@ def test_matmul_nonfinite_stays_in_its_row_and_column(gpu, M, out):
 
 
 def test_matmul_empty(gpu):
-    e = lambda R_, K: B._empty_block(R_, K, "cuda")  # noqa: E731
+    def e(rows, K):
+        return B.BlockFp8(torch.empty(rows, 128 * R.blocks(K), dtype=torch.uint8, device="cuda"),
+                          torch.empty(R.blocks(K), rows, device="cuda"), K)
     assert B.matmul(e(0, 128), e(4, 128)).shape == (0, 4)
     assert B.matmul(e(4, 128), e(0, 128)).shape == (4, 0)
     b = torch.tensor([1.0, -2.0, 3.0], device="cuda")

@@ -225,7 +225,7 @@ def test_backward_strides_and_in_place(gpu, D, dtype):
     for over_x in (False, True):
         p, q = dy.clone(), x.clone()
         out = q if over_x else p
-        rc = lib.nflow_layer_norm_backward(p.data_ptr(), q.data_ptr(), B._dtype(x), M, D, D, D, wt.data_ptr(),
+        rc = lib.nflow_layer_norm_backward(p.data_ptr(), q.data_ptr(), B._DTYPES[x.dtype], M, D, D, D, wt.data_ptr(),
                                            mean.data_ptr(), rstd.data_ptr(), out.data_ptr(), D, None, None,
                                            ws.data_ptr(), n.value, torch.cuda.current_stream().cuda_stream)
         assert rc == 0 and torch.equal(out, dx)
