@@ -78,7 +78,16 @@ __device__ __forceinline__ void store8(T* p, int64_t left, const float (&v)[8]) 
 // overflows: such a block is all zero codes under scale 1.
 constexpr float kBlkTiny = 448.0f * 0x1p-126f;
 
-__device__ __forceinline__ float blk_scale(float amax) { return amax < kBlkTiny ? 1.0f : amax / 448.0f; }
+// The correctly rounded amax / 448 without a division: q is within an ulp of it,
+// the remainder a - 448 q is exact (a multiple of 2^-143 for amax >= kBlkTiny),
+// and a quotient within an ulp plus its remainder times the correctly rounded
+// inverse of the divisor rounds correctly (Markstein's theorem).
+__device__ __forceinline__ float blk_scale(float amax) {
+    constexpr float kInv = 1.0f / 448.0f;
+    const float q = amax * kInv;
+    const float s = __builtin_fmaf(__builtin_fmaf(-448.0f, q, amax), kInv, q);
+    return amax < kBlkTiny ? 1.0f : (amax == HUGE_VALF ? amax : s);
+}
 
 // The four bytes fp8_quant(x[e], inv) under a block's own scale.  There
 // |x inv| <= 448 (1 + 2^-22), which the conversion rounds to 448, so no clamp
