@@ -104,6 +104,46 @@ __device__ __forceinline__ uint32_t blk_pack4(float x0, float x1, float x2, floa
     return u & ~(((u & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u);
 }
 
+// The codes of 4 W values.  Neither the cap nor the NaN matters but where the
+// plain conversion gave +-2^-6 (0x08, the only code the cap changes) or a NaN
+// (0x7F); per byte c of u without signs, (c ^ 8) - 1 and c + 1 have their top
+// bit set there (a borrow from a flagged byte may flag its neighbour too).  A
+// wave that holds one such code, one in a hundred thousand on normal data, goes
+// through blk_pack4; the rest pays 5 instructions a word for the test where the
+// cap and the NaN take 15.
+template <int W>
+__device__ __forceinline__ void blk_codes(const float (&x)[4 * W], float inv, uint32_t (&w)[W]) {
+    uint32_t rare = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inv, x[4 * i + 1] * inv, 0, false);
+        c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inv, x[4 * i + 3] * inv, c, true);
+        w[i] = static_cast<uint32_t>(c);
+        const uint32_t u = w[i] & 0x7F7F7F7Fu;
+        rare |= ((u ^ 0x08080808u) - 0x01010101u) | (u + 0x01010101u);
+    }
+    if (__builtin_amdgcn_ballot_w64((rare & 0x80808080u) != 0)) [[unlikely]] {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = blk_pack4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], inv);
+    }
+}
+
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ v2u blk_codes8(const float (&x)[8], float inv) {
+    uint32_t w[2];
+    blk_codes<2>(x, inv, w);
+    return v2u{w[0], w[1]};
+}
+
+// The correctly rounded 1 / s of a block's scale: the hardware's estimate is
+// within an ulp, its remainder 1 - s r is exact, and one step from there rounds
+// correctly (compared with the division at every mantissa of nine exponents
+// over the scales' range: the same bits).  The fix-up makes 1 / inf 0.
+__device__ __forceinline__ float blk_inverse(float s) {
+    const float r = __builtin_amdgcn_rcpf(s);
+    return __builtin_amdgcn_div_fixupf(__builtin_fmaf(__builtin_fmaf(-s, r, 1.0f), r, r), s, 1.0f);
+}
+
 // Scale and inverse of C blocks whose largest magnitudes every one of 16 lanes
 // holds: lane l divides for block l % C (C a power of two), and a lane's value
 // goes to the 16 by DPP, instead of 2 C divisions (a dozen instructions each) in
@@ -133,7 +173,7 @@ __device__ __forceinline__ void spread(float v, float (&out)[C]) {
 template <int C>
 __device__ __forceinline__ void blk_scales(const float (&amax)[C], float& own_scale, float (&inv)[C]) {
     own_scale = blk_scale(pick<C>(amax, threadIdx.x));
-    spread<C>(1.0f / own_scale, inv);
+    spread<C>(blk_inverse(own_scale), inv);
 }
 
 // max that ignores a NaN in v (amax itself is never one).

@@ -72,10 +72,8 @@ __global__ __launch_bounds__(64 * W) void k_block_few(BlockGemmArgs a, const X* 
             load8(x + m * ldx + c, a.K - c, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) amax = amax_of(amax, v[e]);
-            const float sc = blk_scale(max16(amax)), inv = 1.0f / sc;
-            typedef uint32_t v2u __attribute__((ext_vector_type(2)));
-            *reinterpret_cast<v2u*>(lds + m * ldl + c) = v2u{blk_pack4(v[0], v[1], v[2], v[3], inv),
-                                                             blk_pack4(v[4], v[5], v[6], v[7], inv)};
+            const float sc = blk_scale(max16(amax));
+            *reinterpret_cast<v2u*>(lds + m * ldl + c) = blk_codes8(v, blk_inverse(sc));
             if (cl == 0) lds_scale[i] = sc;
         }
         __syncthreads();

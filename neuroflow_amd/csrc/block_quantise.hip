@@ -7,8 +7,6 @@
 namespace nfq {
 namespace {
 
-typedef uint32_t v2u __attribute__((ext_vector_type(2)));
-
 // ---- rows ------------------------------------------------------------------
 // 16 lanes take a block of 128 values, 8 adjacent ones a lane: the largest
 // magnitude is a DPP reduction within the 16, the codes are 8 bytes a lane.
@@ -47,8 +45,7 @@ __global__ __launch_bounds__(256) void k_quantise_rows_blk(const T* __restrict__
         const int64_t b = b0 + u;
         if (b >= kb) break;
         *reinterpret_cast<v2u*>(codes + m * kb * kBlk + b * kBlk + 8 * cl) =
-            v2u{blk_pack4(v[u][0], v[u][1], v[u][2], v[u][3], inv[u]),
-                blk_pack4(v[u][4], v[u][5], v[u][6], v[u][7], inv[u])};
+            blk_codes8(v[u], inv[u]);
     }
 }
 
@@ -124,7 +121,7 @@ __global__ __launch_bounds__(256) void k_quantise_tile(const T* __restrict__ x, 
         float w = 0.0f;
 #pragma unroll
         for (int q = 0; q < 8; ++q) w = fmaxf(w, cmax[q >> 1][64 * (q & 1) + lane]);
-        const float sblk = blk_scale(wave_max(w)), inv = 1.0f / sblk;
+        const float sblk = blk_scale(wave_max(w)), inv = blk_inverse(sblk);
 #pragma unroll
         for (int e = 0; e < 8; ++e) cinv[e] = inv;
         if (tid == 0) {
@@ -137,7 +134,7 @@ __global__ __launch_bounds__(256) void k_quantise_tile(const T* __restrict__ x, 
             const float m4 = fmaxf(fmaxf(cmax[0][tid], cmax[1][tid]), fmaxf(cmax[2][tid], cmax[3][tid]));
             const float sc = blk_scale(m4);
             if (o.codes_t) {
-                colinv[tid] = 1.0f / sc;
+                colinv[tid] = blk_inverse(sc);
                 if (tk * kBlk + tid < K) o.scales_t[tm * K + tk * kBlk + tid] = sc;
             }
             if (o.col_sums && tk * kBlk + tid < K)
@@ -165,11 +162,13 @@ __global__ __launch_bounds__(256) void k_quantise_tile(const T* __restrict__ x, 
             if (cl < 8 && m0 + cl < M) o.scales[tk * M + m0 + cl] = sc;
         }
 #pragma unroll
-        for (int p = 0; p < 8; ++p)
-            if (m0 + p < M)
-                *reinterpret_cast<v2u*>(o.codes + (m0 + p) * kb * kBlk + c0) =
-                    v2u{blk_pack4(v[p][0], v[p][1], v[p][2], v[p][3], rinv[p]),
-                        blk_pack4(v[p][4], v[p][5], v[p][6], v[p][7], rinv[p])};
+        for (int p = 0; p < 8; ++p) {
+            float r[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[e] = v[p][e];
+            const v2u q8 = blk_codes8(r, rinv[p]);
+            if (m0 + p < M) *reinterpret_cast<v2u*>(o.codes + (m0 + p) * kb * kBlk + c0) = q8;
+        }
     }
     keep();
     if (!WEIGHT && o.codes_t) {
@@ -179,10 +178,12 @@ __global__ __launch_bounds__(256) void k_quantise_tile(const T* __restrict__ x, 
     }
     if (o.codes_t) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<v2u*>(lt + (8 * cl + e) * kBlk + 8 * (rg ^ cl)) =
-                v2u{blk_pack4(v[0][e], v[1][e], v[2][e], v[3][e], cinv[e]),
-                    blk_pack4(v[4][e], v[5][e], v[6][e], v[7][e], cinv[e])};
+        for (int e = 0; e < 8; ++e) {
+            float r[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p) r[p] = v[p][e];
+            *reinterpret_cast<v2u*>(lt + (8 * cl + e) * kBlk + 8 * (rg ^ cl)) = blk_codes8(r, cinv[e]);
+        }
         __syncthreads();
 #pragma unroll
         for (int it = 0; it < 4; ++it) {

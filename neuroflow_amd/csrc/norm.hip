@@ -8,7 +8,6 @@ namespace nfq {
 namespace {
 
 constexpr int kNormThreads = 256;
-typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 // Sum over the block; every thread gets it.  `part` holds a value per wave.
 __device__ __forceinline__ float block_sum(float v, float* part) {
@@ -22,9 +21,10 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
     return s;
 }
 
-// 1 / sqrt(v): the hardware's estimate (an ulp) and a Newton step, which an
-// FP8 norm, bound by its VALU work, is 8% faster for; the division at the
-// ends of the range, where the estimate or the step would leave it.
+// 1 / sqrt(v): the hardware's estimate (an ulp) and a Newton step (50.2 us
+// against 51.8 with a square root and a division, FP8 norm of 16384 x 4096
+// bf16); the division at the ends of the range, where the estimate or the step
+// would leave it.
 __device__ __forceinline__ float norm_rstd(float v) {
     const float r = __builtin_amdgcn_rsqf(v);
     const float s = __builtin_fmaf(0.5f * r, __builtin_fmaf(-v * r, r, 1.0f), r);
@@ -159,10 +159,11 @@ __global__ __launch_bounds__(row_threads<L>()) void k_norm(NormArgs a, int64_t p
                 store8(static_cast<T*>(a.y) + m * a.ldy + c, on ? D - c : 0, y[j]);
             }
         } else {
-            // 16 threads hold a block of 128; columns past D count as 0.  (Sharing
-            // the blocks' divisions among the lanes, as the quantise does, is
-            // slower here, 54.0 against 51.5 us at 16384 x 4096 bf16: a row is a
-            // chain of reductions, and this lengthens it.)
+            // 16 threads hold a block of 128; columns past D count as 0.  Every
+            // lane inverts its own block's scale: shared among the lanes, as the
+            // quantise has it, the inverses lengthen a row's chain of reductions.
+            // At 16384 x 4096 bf16: 47.4 us, 4.3 TB/s, the VALU's issue as busy as
+            // HBM (50.2 us with divisions and the cap at every value).
             const int kb = static_cast<int>(blk_count(D));
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
@@ -174,11 +175,10 @@ __global__ __launch_bounds__(row_threads<L>()) void k_norm(NormArgs a, int64_t p
                 float amax = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) amax = amax_of(amax, y[j][e]);
-                const float sc = blk_scale(max16(amax)), inv = 1.0f / sc;
+                const float sc = blk_scale(max16(amax));
+                const v2u q8 = blk_codes8(y[j], blk_inverse(sc));
                 if (on && c / kBlk < kb) {
-                    *reinterpret_cast<v2u*>(a.codes + m * kb * kBlk + c) =
-                        v2u{blk_pack4(y[j][0], y[j][1], y[j][2], y[j][3], inv),
-                            blk_pack4(y[j][4], y[j][5], y[j][6], y[j][7], inv)};
+                    *reinterpret_cast<v2u*>(a.codes + m * kb * kBlk + c) = q8;
                     if (t % 16 == 0) a.scales[c / kBlk * a.M + m] = sc;
                 }
             }
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(kNormThreads) void k_norm_rows(NormArgs a) {
                 const int64_t c = b * kBlk + 2 * lane;
                 const float v0 = c < a.D ? value(c) : 0.0f, v1 = c + 1 < a.D ? value(c + 1) : 0.0f;
                 const float sc = blk_scale(wave_max(amax_of(amax_of(0.0f, v0), v1)));
-                const float inv = 1.0f / sc;
+                const float inv = blk_inverse(sc);
                 const uint32_t w = fp8_quant(v0, inv) | fp8_quant(v1, inv) << 8;
                 *reinterpret_cast<uint16_t*>(a.codes + m * kb * kBlk + c) =
                     static_cast<uint16_t>(c + 1 < a.D ? w : (c < a.D ? w & 0xFFu : 0u));
