@@ -28,9 +28,6 @@ struct BlockGemmArgs {
 int block_quantise(const char* what, const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* codes,
                    float* scales, uint8_t* codes_t, float* scales_t, float* col_sums, hipStream_t st);
 
-// out[n] = sum over p of part[p][n], in an order that depends on P alone.
-int sum_parts(const char* what, const float* part, int64_t P, int64_t N, float* out, hipStream_t st);
-
 // The product for few rows (block_few.hip): from codes, and from the values of
 // x (of C's type, row stride ldx) quantised on the way, W in 128 x 128 blocks.
 void launch_block_few(const BlockGemmArgs& a, hipStream_t st);

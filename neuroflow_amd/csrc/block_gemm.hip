@@ -7,14 +7,51 @@
 namespace nfq {
 namespace {
 
-// Sum of the splits' partial results, in their order, and the epilogue.
+// out[n] = the sum of part (P, N) over P, in an order that depends on P alone:
+// 16 columns a workgroup, every sixteenth part a thread, the threads' sums in turn.
+struct PartSums {
+    const float* part;
+    int64_t P, N;
+    float* out;
+    __host__ __device__ int blocks() const { return out ? static_cast<int>((N + 15) / 16) : 0; }
+};
+__device__ __forceinline__ void sum_parts(const PartSums& a, int blk) {
+    __shared__ float s[16][17];
+    const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const int64_t n = static_cast<int64_t>(blk) * 16 + c;
+    float v = 0.0f;
+    if (n < a.N) {
+#pragma unroll 8
+        for (int64_t p = g; p < a.P; p += 16) v += a.part[p * a.N + n];
+    }
+    s[g][c] = v;
+    __syncthreads();
+    if (g == 0 && n < a.N) {
+        float z = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) z += s[k][c];
+        a.out[n] = z;
+    }
+}
+__global__ __launch_bounds__(256) void k_sum_parts(PartSums a) { sum_parts(a, blockIdx.x); }
+
+// Sum of the splits' partial results, in their order, and the epilogue.  The
+// first workgroups take `sums`, which are a few latencies long and would cost a
+// launch of their own (4 to 5 us).  Bound by the partial results' bytes, most of
+// them from L2 and the Infinity Cache.
 template <typename TO>
-__global__ __launch_bounds__(256) void k_block_gemm_join(BlockGemmArgs a, const float* __restrict__ part, int splits) {
+__global__ __launch_bounds__(256) void k_block_gemm_join(BlockGemmArgs a, const float* __restrict__ part, int splits,
+                                                         PartSums sums) {
+    const int first = sums.blocks();
+    if (static_cast<int>(blockIdx.x) < first) {
+        sum_parts(sums, blockIdx.x);
+        return;
+    }
     const int64_t n4 = (a.N + 3) / 4, total = a.M * n4;
     const bool vec = a.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(a.C) & (4 * sizeof(TO) - 1)) == 0;
     const bool vin = a.N % 4 == 0;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.x) * 256) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x - first) * 256 + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x - first) * 256) {
         const int64_t m = i / n4, n = (i - m * n4) * 4;
         v4f z{0.0f, 0.0f, 0.0f, 0.0f};
         for (int s = 0; s < splits; ++s) {
@@ -60,10 +97,12 @@ void launch_tiles(const BlockGemmArgs& a, int splits, float* part, hipStream_t s
 }
 
 template <typename TO>
-void launch_join(const BlockGemmArgs& a, int splits, const float* part, hipStream_t st) {
+void launch_join(const BlockGemmArgs& a, int splits, const float* part, const PartSums& sums, hipStream_t st) {
     if (splits > 1)
-        hipLaunchKernelGGL((k_block_gemm_join<TO>), dim3(grid_for(a.M * ((a.N + 3) / 4), 256, 8)), dim3(256), 0, st, a,
-                           part, splits);
+        hipLaunchKernelGGL((k_block_gemm_join<TO>), dim3(sums.blocks() + grid_for(a.M * ((a.N + 3) / 4), 256, 8)),
+                           dim3(256), 0, st, a, part, splits, sums);
+    else if (sums.out)
+        hipLaunchKernelGGL(k_sum_parts, dim3(sums.blocks()), dim3(256), 0, st, sums);
 }
 
 // How a product is cut: the kernel or tile, and the number of runs of K blocks
@@ -121,29 +160,35 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int out) {
 }
 
 template <typename TO, bool BLOCKS>
-void launch_gemm(const BlockGemmArgs& a, const GemmPlan& p, float* part, hipStream_t st) {
+void launch_gemm(const BlockGemmArgs& a, const GemmPlan& p, float* part, const PartSums& sums, hipStream_t st) {
     if constexpr (std::is_same_v<TO, bf16>) {
         if (p.kind == GEMM_BIG) launch_tiles<TO, BLOCKS, TileBig>(a, p.splits, part, st);
     }
     if (p.kind == GEMM_MID) launch_tiles<TO, BLOCKS, TileMid>(a, p.splits, part, st);
     if (p.kind == GEMM_SMALL) launch_tiles<TO, BLOCKS, TileSmall>(a, p.splits, part, st);
-    launch_join<TO>(a, p.splits, part, st);
+    launch_join<TO>(a, p.splits, part, sums, st);
 }
 
-int block_gemm(const char* what, const BlockGemmArgs& a, void* ws, hipStream_t st) {
-    if (a.M == 0 || a.N == 0) return NFLOW_OK;
+// a's product, and on its way `sums`, which its caller has asked for.
+int block_gemm(const char* what, const BlockGemmArgs& a, void* ws, hipStream_t st, const PartSums& sums = {}) {
+    if (a.M == 0 || a.N == 0) {
+        if (!sums.out) return NFLOW_OK;
+        launch_join<float>(a, 1, nullptr, sums, st);
+        return launch_status(what);
+    }
     const GemmPlan p = gemm_plan(a.M, a.N, a.K, a.out);
     if (p.kind == GEMM_FEW) {
         launch_block_few(a, st);
+        launch_join<float>(a, 1, nullptr, sums, st);
         return launch_status(what);
     }
     float* part = static_cast<float*>(ws);
     if (a.out == NFLOW_DTYPE_BF16) {
-        if (a.w_blocks) launch_gemm<bf16, true>(a, p, part, st);
-        else launch_gemm<bf16, false>(a, p, part, st);
+        if (a.w_blocks) launch_gemm<bf16, true>(a, p, part, sums, st);
+        else launch_gemm<bf16, false>(a, p, part, sums, st);
     } else {
-        if (a.w_blocks) launch_gemm<float, true>(a, p, part, st);
-        else launch_gemm<float, false>(a, p, part, st);
+        if (a.w_blocks) launch_gemm<float, true>(a, p, part, sums, st);
+        else launch_gemm<float, false>(a, p, part, sums, st);
     }
     return launch_status(what);
 }
@@ -151,19 +196,19 @@ int block_gemm(const char* what, const BlockGemmArgs& a, void* ws, hipStream_t s
 // The two products of the fp32 backward pass, a (row scales) and b (block
 // scales), in one launch where both take 128 x 128 tiles.
 int block_gemm_both(const char* what, const BlockGemmArgs& a, const BlockGemmArgs& b, void* ws_a, void* ws_b,
-                    hipStream_t st) {
+                    hipStream_t st, const PartSums& sums) {
     if (a.M > 0 && a.N > 0 && b.M > 0 && b.N > 0 && a.out == NFLOW_DTYPE_F32 && b.out == NFLOW_DTYPE_F32) {
         const GemmPlan pa = gemm_plan(a.M, a.N, a.K, a.out), pb = gemm_plan(b.M, b.N, b.K, b.out);
         if (pa.kind == GEMM_MID && pb.kind == GEMM_MID) {
             float *fa = static_cast<float*>(ws_a), *fb = static_cast<float*>(ws_b);
             const GemmShare sa = gemm_share<TileMid>(a, pa.splits, fa), sb = gemm_share<TileMid>(b, pb.splits, fb);
             launch_staged<TileMid, &k_block_gemm_pair<TileMid>>(sa.blocks + sb.blocks, st, a, sa, b, sb);
-            launch_join<float>(a, pa.splits, fa, st);
-            launch_join<float>(b, pb.splits, fb, st);
+            launch_join<float>(a, pa.splits, fa, sums, st);
+            launch_join<float>(b, pb.splits, fb, PartSums{}, st);
             return launch_status(what);
         }
     }
-    if (int rc = block_gemm(what, a, ws_a, st)) return rc;
+    if (int rc = block_gemm(what, a, ws_a, st, sums)) return rc;
     return block_gemm(what, b, ws_b, st);
 }
 
@@ -325,11 +370,10 @@ int nflow_fp8_block_linear_backward(const void* dy, int dtype, int64_t M, int64_
         if (int rc = block_quantise(what, dy, dtype, M, N, lddy, dx ? q : nullptr, dx ? sq : nullptr,
                                     dW ? t : nullptr, dW ? stt : nullptr, dbias ? sums : nullptr, st))
             return rc;
-    if (dbias && N > 0)
-        if (int rc = sum_parts(what, sums, blk_count(M), N, dbias, st)) return rc;
-    if (dx && dW) return block_gemm_both(what, aw, ax, part_w, part_x, st);
-    if (dx) return block_gemm(what, ax, part_x, st);
-    return dW ? block_gemm(what, aw, part_w, st) : NFLOW_OK;
+    const PartSums bias{sums, blk_count(M), N, N > 0 ? dbias : nullptr};
+    if (dx && dW) return block_gemm_both(what, aw, ax, part_w, part_x, st, bias);
+    return dx ? block_gemm(what, ax, part_x, st, bias)
+              : dW ? block_gemm(what, aw, part_w, st, bias) : block_gemm(what, BlockGemmArgs{}, nullptr, st, bias);
 }
 
 }  // extern "C"

@@ -197,28 +197,6 @@ __global__ __launch_bounds__(256) void k_quantise_tile(const T* __restrict__ x, 
     }
 }
 
-// out[n] = the sum of parts (P, N) over P: 64 columns a workgroup, a sixteenth
-// of the parts a wave.
-__global__ __launch_bounds__(1024) void k_sum_parts(const float* __restrict__ part, int64_t P, int64_t N,
-                                                    float* __restrict__ out) {
-    __shared__ float s[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * 64 + lane;
-    float v = 0.0f;
-    if (n < N) {
-#pragma unroll 8
-        for (int64_t p = wave; p < P; p += 16) v += part[p * N + n];
-    }
-    s[wave][lane] = v;
-    __syncthreads();
-    if (wave == 0 && n < N) {
-        float z = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) z += s[k][lane];
-        out[n] = z;
-    }
-}
-
 int check_matrix(const char* what, const void* x, int dtype, int64_t M, int64_t K, int64_t ldx) {
     if (!dtype_ok(dtype)) return bad_arg(what, "unknown dtype");
     if (M < 0 || K < 0) return bad_arg(what, "bad dims");
@@ -246,11 +224,6 @@ int block_quantise(const char* what, const void* x, int dtype, int64_t M, int64_
     };
     if (dtype == NFLOW_DTYPE_BF16) run(static_cast<const bf16*>(x));
     else run(static_cast<const float*>(x));
-    return launch_status(what);
-}
-
-int sum_parts(const char* what, const float* part, int64_t P, int64_t N, float* out, hipStream_t st) {
-    hipLaunchKernelGGL(k_sum_parts, dim3(static_cast<unsigned>((N + 63) / 64)), dim3(1024), 0, st, part, P, N, out);
     return launch_status(what);
 }
 

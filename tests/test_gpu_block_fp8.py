@@ -293,6 +293,30 @@ def test_linear_backward_against_differences(gpu):
         assert abs(got - want) <= 300 * R.U * mag
 
 
+@pytest.mark.parametrize("M,N,K", [(40, 24, 32), (700, 48, 130), (3000, 150, 200), (65, 257, 300)])
+def test_linear_backward_of_some_results(gpu, M, N, K):
+    """Each result has the same bits whichever others the call is asked for."""
+    import ctypes
+    lib = _lib.lib()
+    dy, _ = _x(640 + M, M, N)
+    xc = B.quantise_columns(_x(641 + M, M, K)[0])
+    _, wt = B.quantise_weight(_x(642 + M, N, K)[0], transposed=True)
+    want = B.linear_backward(dy, xc, wt)
+    need = ctypes.c_size_t()
+    assert lib.nflow_fp8_block_linear_backward_workspace(M, N, K, _lib.DTYPE_F32, ctypes.byref(need)) == 0
+    ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    for ask in range(1, 8):
+        got = [torch.full_like(t, 7.0) for t in want]
+        p = [t.data_ptr() if ask >> i & 1 else None for i, t in enumerate(got)]
+        rc = lib.nflow_fp8_block_linear_backward(
+            dy.data_ptr(), _lib.DTYPE_F32, M, N, N, xc.codes.data_ptr(), xc.scales.data_ptr(), wt.codes.data_ptr(),
+            wt.scales.data_ptr(), K, p[0], K, p[1], p[2], ws.data_ptr(), need.value,
+            torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        for i in range(3):
+            assert torch.equal(got[i], want[i] if ask >> i & 1 else torch.full_like(want[i], 7.0)), (ask, i)
+
+
 def test_linear_backward_empty(gpu):
     w, wt = B.quantise_weight(torch.ones(30, 20, device="cuda"), transposed=True)
     xc = B.quantise_columns(torch.empty(0, 20, device="cuda"))
