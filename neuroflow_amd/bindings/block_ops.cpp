@@ -219,7 +219,9 @@ Tensor matmul(const Tensor& ac, const Tensor& as, int64_t ak, const Tensor& wc, 
     if (ak != wk)
         throw py::value_error("a has " + std::to_string(ak) + " columns, w has " + std::to_string(wk));
     const int64_t M = block_rows(ac, as, ak, false, "a");
-    const bool weight = wc.defined() && wsc.defined() && wc.dim() == 2 && wsc.dim() == 2 && wsc.size(1) != wc.size(0);
+    // One row has one scale a block in either form: taken as a weight's, as linear has it.
+    const bool weight = wc.defined() && wsc.defined() && wc.dim() == 2 && wsc.dim() == 2 &&
+                        (wsc.size(1) != wc.size(0) || wc.size(0) == 1);
     const int64_t N = block_rows(wc, wsc, wk, weight, "w");
     const float* b = param(bias, N, "bias");
     const Tensor y = empty({M, N}, ac, dt == NFLOW_DTYPE_BF16 ? at::kBFloat16 : at::kFloat);

@@ -293,6 +293,32 @@ def test_linear_backward_against_differences(gpu):
         assert abs(got - want) <= 300 * R.U * mag
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,N,K", [(17, 1, 1), (17, 129, 128), (64, 7, 100), (65, 33, 129), (100, 500, 200), (129, 4097, 90),
+                                   (700, 130, 256), (2049, 1000, 300), (2100, 70, 512), (8200, 256, 500),
+                                   (16384, 768, 256), (33000, 640, 120)])
+def test_linear_is_the_product_of_the_codes(gpu, M, N, K, dtype):
+    """Whichever kernel a size takes, linear gives the bits of quantise and
+    matmul: rows of zeros, infinities and NaN, odd row strides, every activation."""
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    wide = (torch.randn(M, K + 5, device="cuda", generator=g) * torch.randn(M, 1, device="cuda", generator=g).exp()).to(dtype)
+    w = B.quantise_weight(torch.randn(N, K, device="cuda", generator=g))
+    bias = torch.randn(N, device="cuda", generator=g)
+    for off in (0, 3):
+        x = wide[:, off:off + K]
+        x[M // 2] = 0
+        x[M // 3, K // 2] = float("inf")
+        x[M // 4, K - 1] = float("nan")
+        x[M - 1, 0] = -1e30
+        for b, act in ((None, "none"), (bias, "relu"), (bias, "gelu")):
+            got, want = B.linear(x, w, b, act), B.matmul(B.quantise(x), w, b, act, out_dtype=dtype)
+            assert torch.equal(got.isnan(), want.isnan())
+            assert torch.equal(got.nan_to_num(nan=0.5), want.nan_to_num(nan=0.5))
+    strided = wide.t().contiguous().t()[:, :K].contiguous().unsqueeze(0)
+    assert torch.equal(B.linear(strided, w).nan_to_num(nan=0.5)[0],
+                       B.matmul(B.quantise(strided[0]), w, out_dtype=dtype).nan_to_num(nan=0.5))
+
+
 @pytest.mark.parametrize("M,N,K", [(40, 24, 32), (700, 48, 130), (3000, 150, 200), (65, 257, 300)])
 def test_linear_backward_of_some_results(gpu, M, N, K):
     """Each result has the same bits whichever others the call is asked for."""
