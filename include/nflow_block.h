@@ -112,7 +112,9 @@ int nflow_fp8_block_matmul(const uint8_t* A, const float* scale_A, const uint8_t
 int nflow_fp8_block_matmul_workspace(int64_t M, int64_t N, int64_t K, int c_dtype, size_t* bytes);
 
 /* y = act(q(x) W^T + bias), q the quantise above: x (M, K) and y (M, N) of
- * one type, W a weight in 128 x 128 blocks.  A few rows are one launch. */
+ * one type, W a weight in 128 x 128 blocks.  A few rows, and many rows of up to
+ * 512 columns where that is faster, are one launch; the workspace has room for
+ * x's codes past a few rows either way. */
 int nflow_fp8_block_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* W,
                            const float* scale_W, int64_t N, const float* bias, int activation, void* y,
                            int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);

@@ -212,9 +212,12 @@ int block_gemm_both(const char* what, const BlockGemmArgs& a, const BlockGemmArg
     return block_gemm(what, b, ws_b, st);
 }
 
-// Whether linear is one launch of the few-row kernel on x's values.
-bool linear_direct(int64_t M, int64_t N, int64_t K, int dtype) {
-    return few_values(M, K) && gemm_plan(M, N, K, dtype).kind == GEMM_FEW;
+// What linear runs: a kernel that takes x's values, for few rows or for many
+// rows of few K blocks, or the quantise and the product.
+enum LinearKind { LINEAR_FEW, LINEAR_ROWS, LINEAR_CODES };
+LinearKind linear_kind(int64_t M, int64_t N, int64_t K, int dtype) {
+    if (few_values(M, K) && gemm_plan(M, N, K, dtype).kind == GEMM_FEW) return LINEAR_FEW;
+    return many_rows_values(M, N, K, dtype) ? LINEAR_ROWS : LINEAR_CODES;
 }
 
 int check_gemm(const char* what, const BlockGemmArgs& a) {
@@ -244,8 +247,10 @@ struct BlockSpace {
 size_t matmul_space(int64_t M, int64_t N, int64_t K, int out) {
     return M > 0 && N > 0 ? gemm_plan(M, N, K, out).bytes : 0;
 }
+// Room for x's codes past a few rows, also at the sizes whose kernel does
+// without: which kernel serves a size is then no part of the interface.
 size_t linear_space(int64_t M, int64_t N, int64_t K, int dtype) {
-    if (M == 0 || N == 0 || linear_direct(M, N, K, dtype)) return 0;
+    if (M == 0 || N == 0 || linear_kind(M, N, K, dtype) == LINEAR_FEW) return 0;
     return BlockSpace(M, K).bytes() + matmul_space(M, N, K, dtype);
 }
 struct BackwardSpace {
@@ -309,20 +314,21 @@ int nflow_fp8_block_linear(const void* x, int dtype, int64_t M, int64_t K, int64
     if (int rc = check_workspace(what, workspace, workspace_bytes, linear_space(M, N, K, dtype))) return rc;
     if (ldx < K) return bad_arg(what, "row stride smaller than a row");
     // The codes the product reads: none where it quantises by itself.
-    const bool direct = linear_direct(M, N, K, dtype);
+    const LinearKind kind = linear_kind(M, N, K, dtype);
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     const BlockSpace xs(M, K);
     float* scales = reinterpret_cast<float*>(codes + xs.codes);
     BlockGemmArgs a{codes, scales, W, scale_W, true, M, N, K, bias, activation, y, dtype, ldy};
-    if (direct) {
+    if (kind != LINEAR_CODES) {
         a.A = W;            // not read; check_gemm wants the operands' pointers
         a.sA = scale_W;
     }
     if (int rc = check_gemm(what, a)) return rc;
     if (M == 0 || N == 0) return NFLOW_OK;
     if (K > 0 && !x) return bad_arg(what, "null x");
-    if (direct) {
-        launch_block_few_values(a, x, ldx, as_stream(stream));
+    if (kind != LINEAR_CODES) {
+        if (kind == LINEAR_FEW) launch_block_few_values(a, x, ldx, as_stream(stream));
+        else launch_block_rows(a, x, ldx, as_stream(stream));
         return launch_status(what);
     }
     if (K > 0)
