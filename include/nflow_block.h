@@ -135,6 +135,15 @@ int nflow_fp8_block_linear_backward(const void* dy, int dtype, int64_t M, int64_
                                     float* dbias, void* workspace, size_t workspace_bytes, void* stream);
 int nflow_fp8_block_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes);
 
+/* ---- for tests: which kernel a size takes (no GPU needed: 256 CUs without one) ---- */
+
+/* The tile edge of matmul's kernel at this size, 64, 128 or 256, or 0 for the
+ * few-row kernel; and the runs that the K blocks are split into. */
+int nflow_debug_fp8_block_cut(int64_t M, int64_t N, int64_t K, int c_dtype, int* edge, int* splits);
+/* What linear runs: 0 the few-row kernel on x's values, 1 the kernel of many
+ * rows on x's values, with its workgroups, 2 the quantise and matmul's kernel. */
+int nflow_debug_fp8_block_linear_kernel(int64_t M, int64_t N, int64_t K, int dtype, int* kernel, int* workgroups);
+
 #ifdef __cplusplus
 }
 #endif

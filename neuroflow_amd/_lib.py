@@ -154,6 +154,8 @@ SIGNATURES = {
     "nflow_fp8_block_linear_backward": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp,
                                         _vp, C.c_size_t, _vp],
     "nflow_fp8_block_linear_backward_workspace": [_i64, _i64, _i64, _i32, C.POINTER(C.c_size_t)],
+    "nflow_debug_fp8_block_cut": [_i64, _i64, _i64, _i32, C.POINTER(_i32), C.POINTER(_i32)],
+    "nflow_debug_fp8_block_linear_kernel": [_i64, _i64, _i64, _i32, C.POINTER(_i32), C.POINTER(_i32)],
     # include/nflow_runtime.h
     "nflow_runtime_create": [C.c_char_p, C.POINTER(_vp)],
     "nflow_runtime_create_memory": [_vp, C.c_size_t, C.POINTER(_vp)],

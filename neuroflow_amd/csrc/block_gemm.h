@@ -37,5 +37,6 @@ void launch_block_few_values(const BlockGemmArgs& a, const void* x, int64_t ldx,
 // And for many rows of few K blocks, from the values (block_rows.hip).
 bool many_rows_values(int64_t M, int64_t N, int64_t K, int dtype);
 void launch_block_rows(const BlockGemmArgs& a, const void* x, int64_t ldx, hipStream_t st);
+unsigned block_rows_grid(int64_t M, int64_t N);      // its workgroups
 
 }  // namespace nfq

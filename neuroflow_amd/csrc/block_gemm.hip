@@ -382,4 +382,28 @@ int nflow_fp8_block_linear_backward(const void* dy, int dtype, int64_t M, int64_
               : dW ? block_gemm(what, aw, part_w, st, bias) : block_gemm(what, BlockGemmArgs{}, nullptr, st, bias);
 }
 
+int nflow_debug_fp8_block_cut(int64_t M, int64_t N, int64_t K, int c_dtype, int* edge, int* splits) {
+    clear_error();
+    const char* what = "debug_fp8_block_cut";
+    if (!edge || !splits) return bad_arg(what, "null output");
+    size_t bytes = 0;
+    if (int rc = check_sizes(what, M, N, K, c_dtype, &bytes)) return rc;
+    const GemmPlan p = gemm_plan(M, N, K, c_dtype);
+    *edge = p.kind == GEMM_FEW ? 0 : p.kind == GEMM_SMALL ? TileSmall::BM : p.kind == GEMM_MID ? TileMid::BM : TileBig::BM;
+    *splits = p.splits;
+    return NFLOW_OK;
+}
+
+int nflow_debug_fp8_block_linear_kernel(int64_t M, int64_t N, int64_t K, int dtype, int* kernel, int* workgroups) {
+    clear_error();
+    const char* what = "debug_fp8_block_linear_kernel";
+    if (!kernel || !workgroups) return bad_arg(what, "null output");
+    size_t bytes = 0;
+    if (int rc = check_sizes(what, M, N, K, dtype, &bytes)) return rc;
+    const LinearKind kind = linear_kind(M, N, K, dtype);
+    *kernel = static_cast<int>(kind);
+    *workgroups = kind == LINEAR_ROWS ? static_cast<int>(block_rows_grid(M, N)) : 0;
+    return NFLOW_OK;
+}
+
 }  // extern "C"

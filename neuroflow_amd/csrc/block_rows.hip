@@ -161,15 +161,19 @@ RowsCut rows_cut(int64_t M, int64_t N) {
     return best;
 }
 
+unsigned rows_grid(int64_t M, int64_t N, int per) {
+    return static_cast<unsigned>((M + RowsTile::BM - 1) / RowsTile::BM * ((blk_count(N) + per - 1) / per));
+}
+
 template <typename T, int KB>
 void launch_rows(const BlockGemmArgs& a, const void* x, int64_t ldx, hipStream_t st) {
     static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_block_rows<T, KB>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, RowsTile::BYTES);
     (void)once;
     const int groups = static_cast<int>((a.M + RowsTile::BM - 1) / RowsTile::BM);
-    const int per = rows_cut(a.M, a.N).per, tiles = static_cast<int>(blk_count(a.N));
-    hipLaunchKernelGGL((k_block_rows<T, KB>), dim3(static_cast<unsigned>(groups) * ((tiles + per - 1) / per)),
-                       dim3(64 * RowsTile::WAVES), RowsTile::BYTES, st, a, static_cast<const T*>(x), ldx, groups, per);
+    const int per = rows_cut(a.M, a.N).per;
+    hipLaunchKernelGGL((k_block_rows<T, KB>), dim3(rows_grid(a.M, a.N, per)), dim3(64 * RowsTile::WAVES), RowsTile::BYTES,
+                       st, a, static_cast<const T*>(x), ldx, groups, per);
 }
 
 template <typename T>
@@ -208,6 +212,8 @@ bool many_rows_values(int64_t M, int64_t N, int64_t K, int dtype) {
     const RowsCut c = rows_cut(M, N);
     return c.n == 1 || c.filled >= 0.9;
 }
+
+unsigned block_rows_grid(int64_t M, int64_t N) { return rows_grid(M, N, rows_cut(M, N).per); }
 
 void launch_block_rows(const BlockGemmArgs& a, const void* x, int64_t ldx, hipStream_t st) {
     if (a.out == NFLOW_DTYPE_BF16) launch_rows_kb<bf16>(a, x, ldx, st);
