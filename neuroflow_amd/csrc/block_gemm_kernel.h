@@ -13,7 +13,11 @@
 // bf16 outputs take the FP8 instruction.  It drops low bits of the products
 // it sums: measured against the exact sum on normal and uniform codes, 1.3e-5
 // and 6e-6 of the result in the 2-norm, at worst 2^-12.6 of the block's sum
-// of magnitudes over all finite codes, whatever K; a bf16 result keeps 2^-9.
+// of magnitudes over all finite codes, whatever K.  Rounding to bf16 costs
+// 1.7e-3 in the 2-norm, so as a whole a result is no less exact; one whose
+// products cancel to under an eighth of their magnitudes may lose more here than
+// in its rounding.  That is the price of twice the bf16 instruction's rate
+// (8192 x 8192 x 8192: 473 us against 876), and the type of the result chooses.
 // fp32 outputs take the bf16 instruction on the codes' values, which are exact
 // in bf16 (1e-8 to 1e-7 of the result), at half the rate.
 //
