@@ -6,6 +6,8 @@
 // 1.5 (layer_norm of one token with its statistics: 9.0 -> 6.0 us a call).
 // neuroflow_amd/norm.py and block_fp8.py are the public face; the errors raised
 // here are theirs (TypeError, ValueError, NflowError).
+#include <dlfcn.h>
+
 #include <ATen/ATen.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -14,6 +16,7 @@
 
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "nflow_block.h"
 
@@ -22,6 +25,48 @@ using at::Tensor;
 using Maybe = std::optional<Tensor>;
 
 namespace {
+
+// The library's entry points.  bind() takes their addresses from the library that
+// Python has loaded, which may be another build than the one beside this module:
+// linked, the module would bring a second copy into the process.
+#define NFLOW_BLOCK_OPS(X) \
+    X(nflow_last_error) \
+    X(nflow_fp8_block_linear) \
+    X(nflow_fp8_block_linear_backward) \
+    X(nflow_fp8_block_linear_backward_workspace) \
+    X(nflow_fp8_block_linear_workspace) \
+    X(nflow_fp8_block_matmul) \
+    X(nflow_fp8_block_matmul_workspace) \
+    X(nflow_fp8_block_quantise) \
+    X(nflow_fp8_block_quantise_weight) \
+    X(nflow_layer_norm_backward) \
+    X(nflow_layer_norm_backward_workspace) \
+    X(nflow_layer_norm_forward) \
+    X(nflow_layer_norm_fp8_block)
+
+struct Api {
+#define X(f) decltype(&::f) f = nullptr;
+    NFLOW_BLOCK_OPS(X)
+#undef X
+} api;
+
+std::vector<std::string> entry_points() {
+#define X(f) #f,
+    return {NFLOW_BLOCK_OPS(X)};
+#undef X
+}
+
+void bind(const py::function& address) {
+#define X(f) api.f = reinterpret_cast<decltype(api.f)>(address(#f).cast<uintptr_t>());
+    NFLOW_BLOCK_OPS(X)
+#undef X
+}
+
+// The file that the bound entry points are in.
+std::string library() {
+    Dl_info info{};
+    return dladdr(reinterpret_cast<void*>(api.nflow_last_error), &info) && info.dli_fname ? info.dli_fname : "";
+}
 
 struct Matrix {
     int64_t rows, cols, ld;
@@ -106,7 +151,7 @@ void* stream_of(const Tensor& t) {
 void ok(int rc, const char* what) {
     if (rc == NFLOW_OK) return;
     const py::object type = py::module_::import("neuroflow_amd._lib").attr("NflowError");
-    const py::object e = type(rc, what, nflow_last_error());
+    const py::object e = type(rc, what, api.nflow_last_error());
     PyErr_SetObject(type.ptr(), e.ptr());
     throw py::error_already_set();
 }
@@ -139,7 +184,7 @@ py::object layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, d
         mean = empty({m.rows}, x, at::kFloat);
         rstd = empty({m.rows}, x, at::kFloat);
     }
-    ok(nflow_layer_norm_forward(data(x), dt, m.rows, m.cols, m.ld, w, b, static_cast<float>(eps), data(y), ldy,
+    ok(api.nflow_layer_norm_forward(data(x), dt, m.rows, m.cols, m.ld, w, b, static_cast<float>(eps), data(y), ldy,
                                 data<float>(mean), data<float>(rstd), stream_of(x)), "layer_norm");
     if (!stats) return py::cast(y);
     return py::make_tuple(y, mean, rstd);
@@ -156,7 +201,7 @@ py::tuple layer_norm_fp8(const Tensor& x, const Maybe& weight, const Maybe& bias
         mean = empty({m.rows}, x, at::kFloat);
         rstd = empty({m.rows}, x, at::kFloat);
     }
-    ok(nflow_layer_norm_fp8_block(data(x), dt, m.rows, m.cols, m.ld, w, b, static_cast<float>(eps), data<uint8_t>(codes),
+    ok(api.nflow_layer_norm_fp8_block(data(x), dt, m.rows, m.cols, m.ld, w, b, static_cast<float>(eps), data<uint8_t>(codes),
                                   data<float>(scales), data<float>(mean), data<float>(rstd), stream_of(x)),
        "layer_norm_fp8");
     return py::make_tuple(codes, scales, m.cols, mean, rstd);
@@ -173,9 +218,9 @@ py::tuple layer_norm_backward(const Tensor& dy, const Tensor& x, const Maybe& we
     const Tensor dx = empty(x.sizes(), x, x.scalar_type());
     const Tensor dw = empty({m.cols}, x, at::kFloat), db = empty({m.cols}, x, at::kFloat);
     size_t n = 0;
-    ok(nflow_layer_norm_backward_workspace(m.rows, m.cols, &n), "layer_norm_backward");
+    ok(api.nflow_layer_norm_backward_workspace(m.rows, m.cols, &n), "layer_norm_backward");
     const Tensor ws = scratch(n, x);
-    ok(nflow_layer_norm_backward(data(dy), data(x), dt, m.rows, m.cols, g.ld, m.ld, w, mu, rs, data(dx), m.cols,
+    ok(api.nflow_layer_norm_backward(data(dy), data(x), dt, m.rows, m.cols, g.ld, m.ld, w, mu, rs, data(dx), m.cols,
                                  data<float>(dw), data<float>(db), data(ws), n, stream_of(x)), "layer_norm_backward");
     return py::make_tuple(dx, dw, db);
 }
@@ -194,7 +239,7 @@ py::tuple quantise(const Tensor& x, bool rows, bool columns) {
         ct = empty({m.cols, 128 * blocks(m.rows)}, x, at::kByte);
         st = empty({blocks(m.rows), m.cols}, x, at::kFloat);
     }
-    ok(nflow_fp8_block_quantise(data(x), dt, m.rows, m.cols, m.ld, data<uint8_t>(c), data<float>(s), data<uint8_t>(ct),
+    ok(api.nflow_fp8_block_quantise(data(x), dt, m.rows, m.cols, m.ld, data<uint8_t>(c), data<float>(s), data<uint8_t>(ct),
                                 data<float>(st), stream_of(x)), "fp8_block_quantise");
     return py::make_tuple(c, s, m.cols, ct, st, m.rows);
 }
@@ -209,7 +254,7 @@ py::tuple quantise_weight(const Tensor& W, bool transposed) {
         ct = empty({m.cols, 128 * nb}, W, at::kByte);
         st = empty({nb, kb}, W, at::kFloat);
     }
-    ok(nflow_fp8_block_quantise_weight(data(W), dt, m.rows, m.cols, m.ld, data<uint8_t>(c), data<float>(s),
+    ok(api.nflow_fp8_block_quantise_weight(data(W), dt, m.rows, m.cols, m.ld, data<uint8_t>(c), data<float>(s),
                                        data<uint8_t>(ct), data<float>(st), stream_of(W)), "fp8_block_quantise_weight");
     return py::make_tuple(c, s, m.cols, ct, st, m.rows);
 }
@@ -226,9 +271,9 @@ Tensor matmul(const Tensor& ac, const Tensor& as, int64_t ak, const Tensor& wc, 
     const float* b = param(bias, N, "bias");
     const Tensor y = empty({M, N}, ac, dt == NFLOW_DTYPE_BF16 ? at::kBFloat16 : at::kFloat);
     size_t n = 0;
-    ok(nflow_fp8_block_matmul_workspace(M, N, ak, dt, &n), "fp8_block_matmul");
+    ok(api.nflow_fp8_block_matmul_workspace(M, N, ak, dt, &n), "fp8_block_matmul");
     const Tensor ws = scratch(n, ac);
-    ok(nflow_fp8_block_matmul(data<uint8_t>(ac), data<float>(as), data<uint8_t>(wc), data<float>(wsc), weight, M, N, ak,
+    ok(api.nflow_fp8_block_matmul(data<uint8_t>(ac), data<float>(as), data<uint8_t>(wc), data<float>(wsc), weight, M, N, ak,
                               b, act, data(y), dt, N, data(ws), n, stream_of(ac)), "fp8_block_matmul");
     return y;
 }
@@ -244,9 +289,9 @@ Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& wsc, int64_t wk, 
     size.back() = N;
     const Tensor y = empty(size, x, x.scalar_type());
     size_t n = 0;
-    ok(nflow_fp8_block_linear_workspace(m.rows, N, wk, dt, &n), "fp8_block_linear");
+    ok(api.nflow_fp8_block_linear_workspace(m.rows, N, wk, dt, &n), "fp8_block_linear");
     const Tensor ws = scratch(n, x);
-    ok(nflow_fp8_block_linear(data(x), dt, m.rows, m.cols, m.ld, data<uint8_t>(wc), data<float>(wsc), N, b, act, data(y),
+    ok(api.nflow_fp8_block_linear(data(x), dt, m.rows, m.cols, m.ld, data<uint8_t>(wc), data<float>(wsc), N, b, act, data(y),
                               N, data(ws), n, stream_of(x)), "fp8_block_linear");
     return y;
 }
@@ -265,9 +310,9 @@ py::tuple linear_backward(const Tensor& dy, const Tensor& xc, const Tensor& xs, 
     const Tensor dx = empty(size, dy, dy.scalar_type());
     const Tensor dW = empty({m.cols, K}, dy, at::kFloat), db = empty({m.cols}, dy, at::kFloat);
     size_t n = 0;
-    ok(nflow_fp8_block_linear_backward_workspace(m.rows, m.cols, K, dt, &n), "fp8_block_linear_backward");
+    ok(api.nflow_fp8_block_linear_backward_workspace(m.rows, m.cols, K, dt, &n), "fp8_block_linear_backward");
     const Tensor ws = scratch(n, dy);
-    ok(nflow_fp8_block_linear_backward(data(dy), dt, m.rows, m.cols, m.ld, data<uint8_t>(xc), data<float>(xs),
+    ok(api.nflow_fp8_block_linear_backward(data(dy), dt, m.rows, m.cols, m.ld, data<uint8_t>(xc), data<float>(xs),
                                        data<uint8_t>(wc), data<float>(wsc), K, data(dx), K, data<float>(dW),
                                        data<float>(db), data(ws), n, stream_of(dy)), "fp8_block_linear_backward");
     return py::make_tuple(dx, dW, db);
@@ -277,6 +322,9 @@ py::tuple linear_backward(const Tensor& dy, const Tensor& xc, const Tensor& xs, 
 
 PYBIND11_MODULE(block_ops, m) {
     m.doc() = "torch calls of include/nflow_block.h (neuroflow_amd.norm, neuroflow_amd.block_fp8)";
+    m.def("bind", &bind);
+    m.def("entry_points", &entry_points);
+    m.def("library", &library);
     m.def("layer_norm", &layer_norm);
     m.def("layer_norm_fp8", &layer_norm_fp8);
     m.def("layer_norm_backward", &layer_norm_backward);

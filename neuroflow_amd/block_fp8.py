@@ -13,8 +13,10 @@ wrong shape ValueError, a status of the library NflowError.
 """
 from __future__ import annotations
 
+import ctypes
 import importlib.util
 import sysconfig
+from pathlib import Path
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -23,20 +25,24 @@ from . import _lib
 from .quant import _act
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+_LIB_DIR = Path(__file__).resolve().parent / "lib"
 _module = None
 
 
 def _ops():
-    """The built module block_ops (neuroflow_amd/bindings/block_ops.cpp)."""
+    """The built module block_ops (neuroflow_amd/bindings/block_ops.cpp), its
+    calls bound to the library that is loaded."""
     global _module
     if _module is None:
-        _lib.lib()
-        path = _lib.LIB_PATH.parent / ("block_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
+        lib = _lib.lib()
+        path = _LIB_DIR / ("block_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
         if not path.exists():
             raise ImportError(f"{path} is not built; run `python -m neuroflow_amd.build` (there is no CPU fallback)")
         spec = importlib.util.spec_from_file_location("block_ops", path)
-        _module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(_module)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(lambda name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value)
+        _module = module
     return _module
 
 

@@ -6,8 +6,8 @@ pybind11 modules neuroflow_cpp and block_ops on top of it.
 Compiles neuroflow_amd/csrc/*.hip and *.cpp with hipcc for gfx950 and links
 neuroflow_amd/lib/libnflow_quant.so; then compiles
 neuroflow_amd/bindings/*.cpp (host code only) into
-neuroflow_amd/lib/<name><ext>, which load the library from their own
-directory.  Flags:
+neuroflow_amd/lib/<name><ext>: neuroflow_cpp loads the library from its own
+directory, block_ops is given the one in use.  Flags:
   -ffp-contract=off   float expressions round in the written order (the
                       dequantise step must match the reference bit for bit);
   -target-feature -packed-fp32-ops   no packed fp32 VALU instructions.
@@ -50,8 +50,8 @@ def _compile(src: Path, obj: Path) -> None:
 
 
 def _build_binding(name: str, flags: list[str], verbose: bool) -> Path:
-    """bindings/<name>.cpp with g++ against the Python headers, linked to
-    libnflow_quant.so with an $ORIGIN rpath."""
+    """bindings/<name>.cpp with g++ against the Python headers, with the HIP
+    runtime."""
     import sysconfig
 
     out = LIB_DIR / (name + sysconfig.get_config_var("EXT_SUFFIX"))
@@ -71,9 +71,10 @@ def _build_binding(name: str, flags: list[str], verbose: bool) -> Path:
 
 
 def build_bindings(verbose: bool = True) -> Path:
-    """neuroflow_cpp, against pybind11; and block_ops, against torch's headers
-    and its pybind11 (torch's libraries are in the process by the time it is
-    imported)."""
+    """neuroflow_cpp, against pybind11, linked to libnflow_quant.so with an
+    $ORIGIN rpath; and block_ops, against torch's headers and its pybind11
+    (torch's libraries are in the process by the time it is imported, and so is
+    libnflow_quant, whose entry points it is told)."""
     import pybind11
     import torch
 
@@ -82,7 +83,8 @@ def build_bindings(verbose: bool = True) -> Path:
                                  "-I", str(t / "include"), "-I", str(t / "include" / "torch" / "csrc" / "api" / "include"),
                                  "-L", str(t / "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip"],
                    verbose)
-    return _build_binding("neuroflow_cpp", ["-I", pybind11.get_include()], verbose)
+    return _build_binding("neuroflow_cpp", ["-I", pybind11.get_include(), "-L", str(LIB_DIR), "-lnflow_quant",
+                                            "-Wl,-rpath,$ORIGIN"], verbose)
 
 
 def build(verbose: bool = True, lib: Path = LIB) -> Path:
