@@ -102,7 +102,14 @@ void same(const Tensor& t, const char* name, const Tensor& like) {
         throw py::value_error(str(name, " must have the shape, type and device of x"));
 }
 
-float* param(const Maybe& p, int64_t n, const char* name, bool required = false) {
+// An operand's memory has to be on the GPU that the call runs on.
+void on_device(const Tensor& t, const char* name, const Tensor& like) {
+    if (t.device() != like.device())
+        throw py::value_error(str(name, " is on ") + t.device().str() + ", the call's other tensors on " +
+                              like.device().str());
+}
+
+float* param(const Maybe& p, int64_t n, const char* name, const Tensor& like, bool required = false) {
     if (!p) {
         if (required) throw py::type_error(str(name, " is required"));
         return nullptr;
@@ -112,13 +119,15 @@ float* param(const Maybe& p, int64_t n, const char* name, bool required = false)
     if (t.scalar_type() != at::kFloat) throw py::type_error(str(name, " must be float32"));
     if (t.numel() != n || !t.is_contiguous())
         throw py::value_error(str(name, " must be ") + std::to_string(n) + " contiguous values");
+    on_device(t, name, like);
     return static_cast<float*>(t.data_ptr());
 }
 
 int64_t blocks(int64_t n) { return (n + 127) / 128; }
 
-// Rows of a block-FP8 matrix, its tensors checked against k.
-int64_t block_rows(const Tensor& codes, const Tensor& scales, int64_t k, bool weight, const char* name) {
+// Rows of a block-FP8 matrix, its tensors checked against k and the device of `like`.
+int64_t block_rows(const Tensor& codes, const Tensor& scales, int64_t k, bool weight, const char* name,
+                   const Tensor& like) {
     if (!codes.defined() || !scales.defined() || !codes.is_cuda() || !scales.is_cuda())
         throw py::type_error(str(name, " must hold CUDA tensors"));
     if (codes.scalar_type() != at::kByte || scales.scalar_type() != at::kFloat)
@@ -131,6 +140,8 @@ int64_t block_rows(const Tensor& codes, const Tensor& scales, int64_t k, bool we
     if (scales.dim() != 2 || scales.size(0) != kb || scales.size(1) != cols || !scales.is_contiguous())
         throw py::value_error(str(name, ".scales must be a contiguous (") + std::to_string(kb) + ", " +
                               std::to_string(cols) + ")");
+    on_device(codes, name, like);
+    on_device(scales, name, like);
     return R;
 }
 
@@ -169,7 +180,7 @@ py::object layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, d
                       bool stats) {
     const int dt = dtype_of(x, "x");
     const Matrix m = matrix(x, "x");
-    const float *w = param(weight, m.cols, "weight"), *b = param(bias, m.cols, "bias");
+    const float *w = param(weight, m.cols, "weight", x), *b = param(bias, m.cols, "bias", x);
     Tensor y;
     int64_t ldy = m.cols;
     if (out) {
@@ -193,7 +204,7 @@ py::object layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, d
 py::tuple layer_norm_fp8(const Tensor& x, const Maybe& weight, const Maybe& bias, double eps, bool stats) {
     const int dt = dtype_of(x, "x");
     const Matrix m = matrix(x, "x");
-    const float *w = param(weight, m.cols, "weight"), *b = param(bias, m.cols, "bias");
+    const float *w = param(weight, m.cols, "weight", x), *b = param(bias, m.cols, "bias", x);
     const Tensor codes = empty({m.rows, 128 * blocks(m.cols)}, x, at::kByte);
     const Tensor scales = empty({blocks(m.cols), m.rows}, x, at::kFloat);
     Tensor mean, rstd;
@@ -213,8 +224,8 @@ py::tuple layer_norm_backward(const Tensor& dy, const Tensor& x, const Maybe& we
     const Matrix m = matrix(x, "x");
     same(dy, "dy", x);
     const Matrix g = matrix(dy, "dy");
-    const float* w = param(weight, m.cols, "weight");
-    const float *mu = param(mean, m.rows, "mean", true), *rs = param(rstd, m.rows, "rstd", true);
+    const float* w = param(weight, m.cols, "weight", x);
+    const float *mu = param(mean, m.rows, "mean", x, true), *rs = param(rstd, m.rows, "rstd", x, true);
     const Tensor dx = empty(x.sizes(), x, x.scalar_type());
     const Tensor dw = empty({m.cols}, x, at::kFloat), db = empty({m.cols}, x, at::kFloat);
     size_t n = 0;
@@ -263,12 +274,12 @@ Tensor matmul(const Tensor& ac, const Tensor& as, int64_t ak, const Tensor& wc, 
               const Maybe& bias, int act, int dt) {
     if (ak != wk)
         throw py::value_error("a has " + std::to_string(ak) + " columns, w has " + std::to_string(wk));
-    const int64_t M = block_rows(ac, as, ak, false, "a");
+    const int64_t M = block_rows(ac, as, ak, false, "a", ac);
     // One row has one scale a block in either form: taken as a weight's, as linear has it.
     const bool weight = wc.defined() && wsc.defined() && wc.dim() == 2 && wsc.dim() == 2 &&
                         (wsc.size(1) != wc.size(0) || wc.size(0) == 1);
-    const int64_t N = block_rows(wc, wsc, wk, weight, "w");
-    const float* b = param(bias, N, "bias");
+    const int64_t N = block_rows(wc, wsc, wk, weight, "w", ac);
+    const float* b = param(bias, N, "bias", ac);
     const Tensor y = empty({M, N}, ac, dt == NFLOW_DTYPE_BF16 ? at::kBFloat16 : at::kFloat);
     size_t n = 0;
     ok(api.nflow_fp8_block_matmul_workspace(M, N, ak, dt, &n), "fp8_block_matmul");
@@ -283,8 +294,8 @@ Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& wsc, int64_t wk, 
     const Matrix m = matrix(x, "x");
     if (wk != m.cols)
         throw py::value_error("x has " + std::to_string(m.cols) + " columns, w has " + std::to_string(wk));
-    const int64_t N = block_rows(wc, wsc, wk, true, "w");
-    const float* b = param(bias, N, "bias");
+    const int64_t N = block_rows(wc, wsc, wk, true, "w", x);
+    const float* b = param(bias, N, "bias", x);
     c10::SmallVector<int64_t, 6> size(x.sizes().begin(), x.sizes().end());
     size.back() = N;
     const Tensor y = empty(size, x, x.scalar_type());
@@ -300,10 +311,10 @@ py::tuple linear_backward(const Tensor& dy, const Tensor& xc, const Tensor& xs, 
                           const Tensor& wsc, int64_t wk) {
     const int dt = dtype_of(dy, "dy");
     const Matrix m = matrix(dy, "dy");
-    const int64_t K = block_rows(wc, wsc, wk, true, "w_transposed");
+    const int64_t K = block_rows(wc, wsc, wk, true, "w_transposed", dy);
     if (wk != m.cols)
         throw py::value_error("dy has " + std::to_string(m.cols) + " columns, w_transposed has " + std::to_string(wk));
-    if (xk != m.rows || block_rows(xc, xs, xk, false, "x_columns") != K)
+    if (xk != m.rows || block_rows(xc, xs, xk, false, "x_columns", dy) != K)
         throw py::value_error("x_columns must be (" + std::to_string(K) + " rows, k = " + std::to_string(m.rows) + ")");
     c10::SmallVector<int64_t, 6> size(dy.sizes().begin(), dy.sizes().end());
     size.back() = K;

@@ -7,9 +7,10 @@ are rows) or 2-D with a contiguous last axis and any row stride.  Results in
 float32 come from bf16 matrix instructions on the codes' exact values, to fp32
 accuracy; results in bfloat16 from FP8 ones, whose sums of 128 products are off
 by up to 2^-12 of the products' magnitudes (1.3e-5 of the result on normal data;
-more than its rounding only where products cancel).  Calls run on the current stream of the tensors'
-device; scratch comes from torch's allocator.  A wrong type raises TypeError, a
-wrong shape ValueError, a status of the library NflowError.
+more than its rounding only where products cancel).  A call runs on the current
+stream of the current device, on which all of its tensors have to be; scratch
+comes from torch's allocator.  A wrong type raises TypeError, a wrong shape or
+device ValueError, a status of the library NflowError.
 """
 from __future__ import annotations
 

@@ -4,9 +4,10 @@ straight into 128-block FP8 (include/nflow_block.h).
 The norm is the one ahead of a token mixer's projections
 (cpp/src/fno.cpp:1418-1438).  Activations are float32 or bfloat16 CUDA
 tensors, contiguous or 2-D with a contiguous last axis and any row stride;
-parameters and their gradients are float32.  Calls run on the current stream
-of the tensors' device.  A wrong type raises TypeError, a wrong shape
-ValueError, a status of the library NflowError.
+parameters and their gradients are float32.  A call runs on the current stream
+of the current device, on which all of its tensors have to be.  A wrong type
+raises TypeError, a wrong shape or device ValueError, a status of the library
+NflowError.
 """
 from __future__ import annotations
 
