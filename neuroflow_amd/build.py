@@ -72,19 +72,25 @@ def _build_binding(name: str, flags: list[str], verbose: bool) -> Path:
 
 def build_bindings(verbose: bool = True) -> Path:
     """neuroflow_cpp, against pybind11, linked to libnflow_quant.so with an
-    $ORIGIN rpath; and block_ops, against torch's headers and its pybind11
-    (torch's libraries are in the process by the time it is imported, and so is
-    libnflow_quant, whose entry points it is told)."""
+    $ORIGIN rpath; then, where torch is installed, block_ops, against torch's
+    headers and its pybind11 (torch's libraries are in the process by the time
+    it is imported, and so is libnflow_quant, whose entry points it is told).
+    The path of neuroflow_cpp."""
     import pybind11
-    import torch
 
+    out = _build_binding("neuroflow_cpp", ["-I", pybind11.get_include(), "-L", str(LIB_DIR), "-lnflow_quant",
+                                           "-Wl,-rpath,$ORIGIN"], verbose)
+    try:
+        import torch
+    except ImportError:
+        print("block_ops (neuroflow_amd.norm and block_fp8) is not built: it needs torch")
+        return out
     t = Path(torch.__file__).resolve().parent
     _build_binding("block_ops", ["-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                                  "-I", str(t / "include"), "-I", str(t / "include" / "torch" / "csrc" / "api" / "include"),
                                  "-L", str(t / "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip"],
                    verbose)
-    return _build_binding("neuroflow_cpp", ["-I", pybind11.get_include(), "-L", str(LIB_DIR), "-lnflow_quant",
-                                            "-Wl,-rpath,$ORIGIN"], verbose)
+    return out
 
 
 def build(verbose: bool = True, lib: Path = LIB) -> Path:
