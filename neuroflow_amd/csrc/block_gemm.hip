@@ -402,7 +402,7 @@ int nflow_debug_fp8_block_linear_kernel(int64_t M, int64_t N, int64_t K, int dty
     if (int rc = check_sizes(what, M, N, K, dtype, &bytes)) return rc;
     const LinearKind kind = linear_kind(M, N, K, dtype);
     *kernel = static_cast<int>(kind);
-    *workgroups = kind == LINEAR_ROWS ? static_cast<int>(block_rows_grid(M, N)) : 0;
+    *workgroups = kind == LINEAR_ROWS && N > 0 ? static_cast<int>(block_rows_grid(M, N)) : 0;
     return NFLOW_OK;
 }
 

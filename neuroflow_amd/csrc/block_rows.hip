@@ -149,8 +149,10 @@ RowsCut rows_cut(int64_t M, int64_t N) {
     const int64_t groups = (M + RowsTile::BM - 1) / RowsTile::BM, tiles = blk_count(N), cus = num_cus();
     RowsCut best{};
     double least = HUGE_VAL;
-    for (int64_t shares = 1; shares <= std::min<int64_t>(tiles, 64); ++shares) {
-        const int64_t per = (tiles + shares - 1) / shares, n = (groups * ((tiles + per - 1) / per) + cus - 1) / cus;
+    // From a workgroup for every CU (fewer shares than that are no faster) to a tile each.
+    const int64_t shares = std::max<int64_t>(1, cus / groups);
+    for (int64_t per = (tiles + shares - 1) / shares; per > 0; --per) {
+        const int64_t n = (groups * ((tiles + per - 1) / per) + cus - 1) / cus;
         const double t = (static_cast<double>(per) + 1.5) * std::max(1.0, 0.8 * static_cast<double>(n));
         if (t < least) {
             least = t;
@@ -190,7 +192,9 @@ void launch_rows_kb(const BlockGemmArgs& a, const void* x, int64_t ldx, hipStrea
 
 // Where this is the faster of the two.  Of 600 sizes (17 to 32768 rows, 64 to 4096
 // columns, K of 100 to 512) it holds at 301, which take 0.77 of the time of the
-// quantise and the product (geometric mean; 0.52 to 1.035).  Here / there in us:
+// quantise and the product (geometric mean; 0.52 to 1.035).  At 17 to 2000 rows of
+// 2048 to 200000 columns it takes 0.67 to 1.08 of it (fp32 results of two K blocks
+// are the ones over 1: 96 x 256 -> 32768 11.6 / 10.8).  Here / there in us:
 // fp32 100 x 256 -> 256 7.6 / 8.8, 32768 x 128 -> 768 24.3 / 31.2, 32768 x 256 ->
 // 768 33.0 / 35.1; bf16 4096 x 256 -> 768 9.0 / 11.2, 32768 x 256 -> 256 11.6 / 21.3.
 // - A wave converts or reads the whole weight for 16 rows, which the tiled
@@ -200,12 +204,16 @@ void launch_rows_kb(const BlockGemmArgs& a, const void* x, int64_t ldx, hipStrea
 // - A large result has to leave in whole 128-byte lines (bf16 20000 x 256 -> 1000
 //   41 / 31), from CUs with equal work (313 groups of rows, bf16 20000 x 512 ->
 //   768 35 / 28); in a small one the launch saved is more than either.
+// - Past 32768 columns a second group of rows makes a CU pass three tiles and more
+//   of the weight one after the other (65 x 256 -> 64000 bf16 15.6 / 11.6, fp32
+//   18.8 / 13.3); one group does not (17 x 128 -> 200000 bf16 15.7 / 21.9).
 // - Up to 64 rows the product of the codes is the few-row kernel, which sums
 //   several K blocks in another order; elsewhere both give the same bits.
 bool many_rows_values(int64_t M, int64_t N, int64_t K, int dtype) {
     const int64_t kb = blk_count(K);
     if (kb == 0 || kb > kRowsMaxBlocks || M <= (kb == 1 ? 16 : 64)) return false;
     const bool bf = dtype == NFLOW_DTYPE_BF16, small = M * N <= (1 << 22);
+    if (M > 64 && N > 32768) return false;
     if (kb > 2 && (bf ? M < 2048 || N > 1024 : M < 8192 || N > 256)) return false;
     if (small || N <= 256) return true;
     if (N > (bf ? 2048 : 1024) || N * (bf ? 2 : 4) % 128 != 0) return false;
