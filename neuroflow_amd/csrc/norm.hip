@@ -21,13 +21,16 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
     return s;
 }
 
-// 1 / sqrt(v): the hardware's estimate (an ulp) and a Newton step (50.2 us
-// against 51.8 with a square root and a division, FP8 norm of 16384 x 4096
-// bf16); the division at the ends of the range, where the estimate or the step
-// would leave it.
+// 1 / sqrt(v), correctly rounded but for a hundredth of an ulp: the hardware's
+// estimate r (an ulp) and a Newton step from its remainder 1 - v r r, taken
+// exactly (v r as a rounded product and what that leaves; without the latter the
+// result is up to 1.9 ulp off, with a square root and a division 1.5).  The
+// division at the ends of the range, where the estimate or the step would leave it.
 __device__ __forceinline__ float norm_rstd(float v) {
     const float r = __builtin_amdgcn_rsqf(v);
-    const float s = __builtin_fmaf(0.5f * r, __builtin_fmaf(-v * r, r, 1.0f), r);
+    const float p = v * r, left = __builtin_fmaf(v, r, -p);
+    const float e = __builtin_fmaf(-left, r, __builtin_fmaf(-p, r, 1.0f));
+    const float s = __builtin_fmaf(0.5f * r, e, r);
     return v > 0x1p-100f && v < 0x1p100f ? s : 1.0f / sqrtf(v);
 }
 
@@ -77,6 +80,15 @@ __device__ __forceinline__ float row_sum(float v, float (*part)[L <= 64 ? 1 : L 
     }
 }
 
+// The sum of n values, n a power of two, by halves: as many additions as in a
+// row, and the mean's error is that of log2 D of them (7.6e-8 of it at 256
+// columns where sixteen in a row gave 9.7e-8).
+template <int n>
+__device__ __forceinline__ float pair_sum(const float* v) {
+    if constexpr (n == 1) return v[0];
+    else return pair_sum<n / 2>(v) + pair_sum<n / 2>(v + n / 2);
+}
+
 // Eight values of a parameter from column c on; `none` where there is no parameter.
 __device__ __forceinline__ void load_param(const float* p, int c, int D, float none, float (&v)[8]) {
     if (p) {
@@ -120,14 +132,14 @@ __global__ __launch_bounds__(row_threads<L>()) void k_norm(NormArgs a, int64_t p
         // Beyond a partial last round the lanes of absent rows work on zeros and
         // store nothing: the workgroup's barriers and the DPP reductions stay whole.
         const bool on = m < end;
-        float v[NV][8], s = 0.0f;
+        float v[NV][8], vs[NV];
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[j][e] = next[j][e];
-                s += v[j][e];
-            }
+            for (int e = 0; e < 8; ++e) v[j][e] = next[j][e];
+            vs[j] = pair_sum<8>(v[j]);
+        }
+        const float s = pair_sum<NV>(vs);
         fetch(i + G < per && m + G < end ? m + G : a.M);
         const float mean = row_sum<L>(s, part, 0) * inv_d;
         float q = 0.0f;
