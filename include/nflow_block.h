@@ -58,7 +58,8 @@ enum nflow_dtype {
 /* y = (x - mean) * rstd * weight + bias over the D columns of each of M rows,
  * mean and rstd = 1 / sqrt(var + eps) in fp32 (var the mean of squares about
  * the mean).  weight, bias (D) may be NULL (ones, zeros); mean, rstd (M) may
- * be NULL (not wanted).  y may be x. */
+ * be NULL (not wanted).  y may be x, at the same row stride; rows that overlap
+ * x's in any other way are refused. */
 int nflow_layer_norm_forward(const void* x, int dtype, int64_t M, int64_t D, int64_t ldx, const float* weight,
                              const float* bias, float eps, void* y, int64_t ldy, float* mean, float* rstd,
                              void* stream);
@@ -73,7 +74,8 @@ int nflow_layer_norm_fp8_block(const void* x, int dtype, int64_t M, int64_t D, i
  *   dx = rstd * (g - mean_D(g) - h * mean_D(g * h)),
  *   dweight = sum_M(dy * h), dbias = sum_M(dy)
  * from the mean and rstd of the forward pass.  weight may be NULL (ones);
- * dweight and dbias (D) may each be NULL (not wanted).  dx may be dy or x.
+ * dweight and dbias (D) may each be NULL (not wanted).  dx may be dy or x,
+ * as y may be x above.
  * M = 0 gives zero dweight and dbias. */
 int nflow_layer_norm_backward(const void* dy, const void* x, int dtype, int64_t M, int64_t D, int64_t lddy,
                               int64_t ldx, const float* weight, const float* mean, const float* rstd, void* dx,

@@ -239,6 +239,19 @@ inline int check_workspace(const char* what, const void* ws, size_t have, size_t
     return NFLOW_OK;
 }
 
+// Whether M rows of D elements (of `size` bytes) from a on, `lda` elements apart,
+// and such rows from b on share memory in another way than row for row.  Rows at
+// one stride are compared exactly, others by the memory they span.
+inline bool rows_clash(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t D, size_t size) {
+    if (M <= 0 || (a == b && (lda == ldb || M == 1))) return false;
+    const auto pa = reinterpret_cast<intptr_t>(a), pb = reinterpret_cast<intptr_t>(b);
+    const int64_t e = static_cast<int64_t>(size), row = D * e;
+    if (pb >= pa + (M - 1) * lda * e + row || pa >= pb + (M - 1) * ldb * e + row) return false;
+    if (lda != ldb || M == 1) return true;
+    const int64_t step = lda * e, off = ((pb - pa) % step + step) % step;
+    return off < row || off + row > step;
+}
+
 inline size_t round16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
 
 }  // namespace nfq

@@ -520,6 +520,8 @@ void launch_norm_grad(const NormGradArgs& a, unsigned nb, hipStream_t st) {
     }
 }
 
+constexpr const char* kOverlap = "the result overlaps an input, and not row for row";
+
 int check_norm(const char* what, const void* x, int dtype, int64_t M, int64_t D, int64_t ldx, float eps) {
     if (!dtype_ok(dtype)) return bad_arg(what, "unknown dtype");
     if (M < 0 || D <= 0) return bad_arg(what, "bad dims");
@@ -553,6 +555,7 @@ int nflow_layer_norm_forward(const void* x, int dtype, int64_t M, int64_t D, int
     if (ldy < D) return bad_arg(what, "row stride smaller than a row");
     if (M == 0) return NFLOW_OK;
     if (!y) return bad_arg(what, "null y");
+    if (rows_clash(x, ldx, y, ldy, M, D, dtype_size(dtype))) return bad_arg(what, kOverlap);
     return norm_forward<false>(what, NormArgs{x, M, D, ldx, weight, bias, eps, y, ldy, nullptr, nullptr, mean, rstd},
                                dtype, stream);
 }
@@ -588,6 +591,8 @@ int nflow_layer_norm_backward(const void* dy, const void* x, int dtype, int64_t 
     if (int rc = check_norm(what, x, dtype, M, D, ldx, 0.0f)) return rc;
     if (lddy < D || lddx < D) return bad_arg(what, "row stride smaller than a row");
     if (M > 0 && (!dy || !mean || !rstd || !dx)) return bad_arg(what, "null dy, mean, rstd or dx");
+    if (rows_clash(dy, lddy, dx, lddx, M, D, dtype_size(dtype)) || rows_clash(x, ldx, dx, lddx, M, D, dtype_size(dtype)))
+        return bad_arg(what, kOverlap);
     if (int rc = check_workspace(what, workspace, workspace_bytes, grad_space(M, D))) return rc;
     hipStream_t st = as_stream(stream);
     const int64_t nb = grad_blocks(M);

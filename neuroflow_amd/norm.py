@@ -22,7 +22,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5, out: Optional[torch.Tensor] = None, return_stats: bool = False):
     """(x - mean) * rstd * weight + bias over the last axis; with
     return_stats also the fp32 mean and rstd of every row, which the backward
-    pass takes.  out may be x."""
+    pass takes.  out may be x, but not overlap it otherwise."""
     return _ops().layer_norm(x, weight, bias, eps, out, return_stats)
 
 
