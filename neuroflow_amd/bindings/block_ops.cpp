@@ -9,6 +9,7 @@
 #include <dlfcn.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/stl.h>
@@ -187,6 +188,8 @@ py::object layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, d
         y = *out;
         same(y, "out", x);
         ldy = matrix(y, "out").ld;
+        if (y.requires_grad() && at::GradMode::is_enabled())
+            throw py::value_error("out requires grad: these functions record no autograd graph");
     } else {
         y = empty(x.sizes(), x, x.scalar_type());
     }
@@ -197,6 +200,7 @@ py::object layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, d
     }
     ok(api.nflow_layer_norm_forward(data(x), dt, m.rows, m.cols, m.ld, w, b, static_cast<float>(eps), data(y), ldy,
                                 data<float>(mean), data<float>(rstd), stream_of(x)), "layer_norm");
+    if (out && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();   // a graph that saved it has to notice
     if (!stats) return py::cast(y);
     return py::make_tuple(y, mean, rstd);
 }

@@ -10,7 +10,9 @@ by up to 2^-12 of the products' magnitudes (1.3e-5 of the result on normal data;
 more than its rounding only where products cancel).  A call runs on the current
 stream of the current device, on which all of its tensors have to be; scratch
 comes from torch's allocator.  A wrong type raises TypeError, a wrong shape or
-device ValueError, a status of the library NflowError.
+device ValueError, a status of the library NflowError.  Nothing records an
+autograd graph: results require no gradient whatever the inputs do, and
+linear_backward is the caller's to call.
 """
 from __future__ import annotations
 

@@ -7,7 +7,8 @@ tensors, contiguous or 2-D with a contiguous last axis and any row stride;
 parameters and their gradients are float32.  A call runs on the current stream
 of the current device, on which all of its tensors have to be.  A wrong type
 raises TypeError, a wrong shape or device ValueError, a status of the library
-NflowError.
+NflowError.  Nothing records an autograd graph: results require no gradient
+whatever the inputs do, and layer_norm_backward is the caller's to call.
 """
 from __future__ import annotations
 
