@@ -108,9 +108,10 @@ __device__ __forceinline__ uint32_t blk_pack4(float x0, float x1, float x2, floa
 // plain conversion gave +-2^-6 (0x08, the only code the cap changes) or a NaN
 // (0x7F); per byte c of u without signs, (c ^ 8) - 1 and c + 1 have their top
 // bit set there (a borrow from a flagged byte may flag its neighbour too).  A
-// wave that holds one such code, one in a hundred thousand on normal data, goes
-// through blk_pack4; the rest pays 5 instructions a word for the test where the
-// cap and the NaN take 15.
+// wave that holds one such code goes through blk_pack4: on normal data one value
+// in a hundred thousand is one, so one wave of 512 values in two hundred, and more
+// where a few large values in a block leave many small ones; the rest pays 5
+// instructions a word for the test where the cap and the NaN take 15.
 template <int W>
 __device__ __forceinline__ void blk_codes(const float (&x)[4 * W], float inv, uint32_t (&w)[W]) {
     uint32_t rare = 0;

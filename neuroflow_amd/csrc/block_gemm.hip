@@ -125,7 +125,10 @@ struct GemmPlan {
 // against 52 us, which win from one for every CU on (8192 x 8192 x 8192 460
 // against 560 us).  A split pays a launch and its partial results' way through
 // the caches; the few-row kernel a CU's rate of reading fragments from L2
-// (36 GB/s), or the weight's from HBM.
+// (36 GB/s), or the weight's from HBM.  Outside those sizes the estimate orders
+// the cuts but is no time: it has no term for a tile's fill and stores (65536 x
+// 1024 x 1024 bf16 estimated 56 us, measured 82), and 16 splits are its most,
+// however many CUs a small result leaves idle.
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int out) {
     const bool f32 = out == NFLOW_DTYPE_F32;
     const double cus = num_cus(), kb = static_cast<double>(blk_count(K)), m = static_cast<double>(M),

@@ -193,10 +193,11 @@ void launch_rows_kb(const BlockGemmArgs& a, const void* x, int64_t ldx, hipStrea
 // Where this is the faster of the two.  Of 600 sizes (17 to 32768 rows, 64 to 4096
 // columns, K of 100 to 512) it holds at 301, which take 0.77 of the time of the
 // quantise and the product (geometric mean; 0.52 to 1.035).  At 17 to 2000 rows of
-// 2048 to 200000 columns it takes 0.67 to 1.08 of it (fp32 results of two K blocks
-// are the ones over 1: 96 x 256 -> 32768 11.6 / 10.8).  Here / there in us:
-// fp32 100 x 256 -> 256 7.6 / 8.8, 32768 x 128 -> 768 24.3 / 31.2, 32768 x 256 ->
-// 768 33.0 / 35.1; bf16 4096 x 256 -> 768 9.0 / 11.2, 32768 x 256 -> 256 11.6 / 21.3.
+// 2048 to 200000 columns, in replayed graphs, where a launch costs least, it takes
+// 0.67 to 1.08 of it (fp32 results of two K blocks are the ones over 1: 96 x 256 ->
+// 32768 11.6 / 10.8, 100 x 256 -> 256 7.7 / 7.2).  Here / there in us, call by call:
+// fp32 100 x 256 -> 256 7.4 / 8.7, 32768 x 128 -> 768 24.6 / 30.3, 32768 x 256 ->
+// 768 32.1 / 34.7; bf16 4096 x 256 -> 768 8.6 / 10.7, 32768 x 256 -> 256 10.4 / 18.7.
 // - A wave converts or reads the whole weight for 16 rows, which the tiled
 //   product does for 64: past two K blocks, and past a width, that costs more
 //   than the rows' codes save, for fp32 results (whose codes are converted)
