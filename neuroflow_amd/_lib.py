@@ -1,5 +1,5 @@
 """ctypes binding of libnflow_quant.so (include/nflow_quant.h, include/nflow_block.h,
-include/nflow_runtime.h).
+include/nflow_residual.h, include/nflow_runtime.h).
 
 The library is loaded from neuroflow_amd/lib/ (built in-tree by
 `python -m neuroflow_amd.build`).  There is no fallback: if the library is
@@ -66,6 +66,16 @@ class X2QuantC(C.Structure):
         ("n_positions", C.c_int64),
         ("width", C.c_int32),
         ("points", C.c_int32),
+    ]
+
+
+class GradTensorC(C.Structure):
+    """nflow_grad_tensor (include/nflow_residual.h)."""
+    _fields_ = [
+        ("grad", C.c_void_p),
+        ("out", C.c_void_p),
+        ("count", C.c_int64),
+        ("dtype", C.c_int),
     ]
 
 
@@ -156,6 +166,22 @@ SIGNATURES = {
     "nflow_fp8_block_linear_backward_workspace": [_i64, _i64, _i64, _i32, C.POINTER(C.c_size_t)],
     "nflow_debug_fp8_block_cut": [_i64, _i64, _i64, _i32, C.POINTER(_i32), C.POINTER(_i32)],
     "nflow_debug_fp8_block_linear_kernel": [_i64, _i64, _i64, _i32, C.POINTER(_i32), C.POINTER(_i32)],
+    # include/nflow_residual.h
+    "nflow_rms_norm_forward": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _f32, _vp, _i64, _vp, _i64, _vp, _vp],
+    "nflow_rms_norm_fp8": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _f32, _vp, _vp, _vp, _i64, _vp, _vp],
+    "nflow_rms_norm_backward": [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp,
+                                C.c_size_t, _vp],
+    "nflow_rms_norm_backward_workspace": [_i64, _i64, C.POINTER(C.c_size_t)],
+    "nflow_dense_linear": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp,
+                           C.c_size_t, _vp],
+    "nflow_dense_linear_workspace": [_i64, _i64, _i64, _i32, C.POINTER(C.c_size_t)],
+    "nflow_dense_linear_backward": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _i64,
+                                    _vp, _i64, _vp, _i64, _vp, _vp, C.c_size_t, _vp],
+    "nflow_dense_linear_backward_workspace": [_i64, _i64, _i64, _i32, C.POINTER(C.c_size_t)],
+    "nflow_grad_norm": [C.POINTER(GradTensorC), _i32, _vp, _vp, C.c_size_t, _vp],
+    "nflow_grad_clip": [C.POINTER(GradTensorC), _i32, _f32, _vp, _vp, C.c_size_t, _vp],
+    "nflow_grad_workspace": [C.POINTER(GradTensorC), _i32, C.POINTER(C.c_size_t)],
+    "nflow_debug_dense_cut": [_i32, _i64, _i64, _i64, _i32, C.POINTER(_i32), C.POINTER(_i32)],
     # include/nflow_runtime.h
     "nflow_runtime_create": [C.c_char_p, C.POINTER(_vp)],
     "nflow_runtime_create_memory": [_vp, C.c_size_t, C.POINTER(_vp)],

@@ -1,0 +1,294 @@
+// dense.hip -- the linear layer in bf16 or fp32, forward and backward
+// (include/nflow_residual.h): the cut of its products, the gradient ahead of the
+// activation, and the entry points.
+#include <type_traits>
+
+#include "dense.h"
+
+namespace nfq {
+namespace {
+
+// ---- dz and dbias ------------------------------------------------------------------
+
+// act'(z) times dy.  For GELU with p = 1 / (1 + 2^(z (k1 + k3 z^2))), z p is the
+// activation (gelu_tanh) and its slope p + z p (1 - p) 2 c (1 + 3 * 0.044715 z^2);
+// 1 - p from whichever side has no cancellation.  Past |z| = 64 the slope is 0 or
+// 1 to all bits, and z is held there, so that no infinity meets a 0.
+__device__ __forceinline__ float act_grad(float dy, float z, int act) {
+    if (act == NFLOW_ACT_RELU) return z > 0.0f ? dy : (z != z ? z : 0.0f);
+    const float k1 = -0x1.26aec2p+1f;       // -2 sqrt(2 / pi) log2(e)
+    const float k3 = -0x1.a5a7cep-4f;       // 0.044715 k1
+    const float c2 = 0x1.988454p+0f;        // 2 sqrt(2 / pi)
+    const float c6 = 0x1.b6676cp-3f;        // 3 * 0.044715 c2
+    z = z > 64.0f ? 64.0f : (z < -64.0f ? -64.0f : z);
+    const float zz = z * z;
+    const float e = __builtin_amdgcn_exp2f(z * __builtin_fmaf(k3, zz, k1));
+    const float p = __builtin_amdgcn_rcpf(1.0f + e);
+    const float q = z > 0.0f ? e * p : 1.0f - p;
+    return dy * __builtin_fmaf(z * p * q, __builtin_fmaf(c6, zz, c2), p);
+}
+
+// dz = dy act'(pre), and the sums of dz's columns over this workgroup's rows:
+// a thread has eight columns and every eighth row, and the eight threads of a
+// column join in LDS.  With no activation only the sums.
+constexpr int kDzCols = 256, kDzRows = 8;            // of a workgroup at a time
+struct DzArgs {
+    const void* dy;
+    const void* pre;
+    void* dz;
+    int64_t M, N, lddy, ldpre, lddz;
+    int act;
+    float* part;        // (row runs, N), or null
+    int64_t rows_per;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void k_dense_dz(DzArgs a) {
+    __shared__ __attribute__((aligned(16))) float join[kDzRows][kDzCols];
+    const int c = 8 * (threadIdx.x & 31), g = threadIdx.x >> 5;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * kDzCols + c, left = a.N - n;
+    const int64_t m0 = blockIdx.y * a.rows_per, m1 = m0 + a.rows_per < a.M ? m0 + a.rows_per : a.M;
+    float s[8] = {};
+    if (left > 0) {
+#pragma unroll 4
+        for (int64_t m = m0 + g; m < m1; m += kDzRows) {
+            float d[8];
+            load8(static_cast<const T*>(a.dy) + m * a.lddy + n, left, d);
+            if (a.act != NFLOW_ACT_NONE) {
+                float z[8];
+                load8(static_cast<const T*>(a.pre) + m * a.ldpre + n, left, z);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[e] = act_grad(d[e], z[e], a.act);
+                store8(static_cast<T*>(a.dz) + m * a.lddz + n, left, d);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] += d[e];
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) *reinterpret_cast<v4f*>(&join[g][c + e]) = v4f{s[e], s[e + 1], s[e + 2], s[e + 3]};
+    __syncthreads();
+    const int64_t col = static_cast<int64_t>(blockIdx.x) * kDzCols + threadIdx.x;
+    if (col >= a.N) return;
+    float z = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kDzRows; ++k) z += join[k][threadIdx.x];
+    a.part[blockIdx.y * a.N + col] = z;
+}
+
+// dbias = the sum of part (P, N) over P.
+__global__ __launch_bounds__(256) void k_dense_dbias(const float* __restrict__ part, int64_t P, int64_t N,
+                                                     float* __restrict__ dbias) {
+    __shared__ float s[16][17];
+    const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * 16 + c;
+    float v = 0.0f;
+    if (n < N) {
+#pragma unroll 8
+        for (int64_t p = g; p < P; p += 16) v += part[p * N + n];
+    }
+    s[g][c] = v;
+    __syncthreads();
+    if (g == 0 && n < N) {
+        float z = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) z += s[k][c];
+        dbias[n] = z;
+    }
+}
+
+// Runs of rows of the sums: four workgroups a CU, of 32 rows at least.
+int64_t dz_runs(int64_t M, int64_t N) {
+    const int64_t cols = (N + kDzCols - 1) / kDzCols;
+    return std::max<int64_t>(1, std::min<int64_t>((M + 31) / 32, 4 * num_cus() / std::max<int64_t>(cols, 1)));
+}
+
+// ---- the cut -----------------------------------------------------------------------------
+
+DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype) {
+    if (form == DENSE_FORWARD && M <= kDenseFewRows) return DensePlan{DENSE_FEW, 1, 0};
+    auto tiles = [&](int64_t e) { return ((M + e - 1) / e) * ((N + e - 1) / e); };
+    const DenseKind kind = tiles(128) >= num_cus() ? DENSE_MID : DENSE_SMALL;
+    const int64_t t = tiles(kind == DENSE_MID ? 128 : 64), steps = (K + 63) / 64;
+    int s = 1;
+    while (s < 16 && 2 * s * t <= 2 * num_cus() && 4 * s <= steps) s *= 2;
+    return DensePlan{kind, s, s > 1 ? round16(static_cast<size_t>(s) * M * N * sizeof(float)) : 0};
+}
+
+size_t product_space(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype) {
+    return M > 0 && N > 0 && K > 0 ? dense_plan(form, M, N, K, dtype).bytes : 0;
+}
+
+int product(const char* what, DenseForm form, const DenseArgs& a, int dtype, void* ws, hipStream_t st) {
+    if (a.M == 0 || a.N == 0) return NFLOW_OK;
+    const DensePlan p = dense_plan(form, a.M, a.N, a.K, dtype);
+    if (p.kind == DENSE_FEW) {
+        if (dtype == NFLOW_DTYPE_BF16) launch_dense_few<bf16>(a, st);
+        else launch_dense_few<float>(a, st);
+    } else {
+        if (dtype == NFLOW_DTYPE_BF16) launch_dense<bf16>(a, form, p, static_cast<float*>(ws), st);
+        else launch_dense<float>(a, form, p, static_cast<float*>(ws), st);
+    }
+    return launch_status(what);
+}
+
+int check_sizes(const char* what, int64_t M, int64_t N, int64_t K, int dtype) {
+    if (M < 0 || N < 0 || K < 0) return bad_arg(what, "bad dims");
+    if (!dtype_ok(dtype)) return bad_arg(what, "unknown dtype");
+    const int64_t top = std::max(std::max(M, N), K);
+    if (K > NFLOW_DENSE_MAX_K || N > NFLOW_DENSE_MAX_K || top > INT64_C(1) << 40)
+        return bad_arg(what, "more than NFLOW_DENSE_MAX_K columns, or too many rows");
+    auto many = [](int64_t m, int64_t n) { return ((m + 63) / 64) * ((n + 63) / 64) > INT32_MAX / 16; };
+    if (many(M, N) || many(M, K) || many(N, K)) return bad_arg(what, "too many results for one launch");
+    return NFLOW_OK;
+}
+
+int check_act(const char* what, int act) {
+    if (act != NFLOW_ACT_NONE && act != NFLOW_ACT_RELU && act != NFLOW_ACT_GELU_TANH)
+        return bad_arg(what, "unknown activation");
+    return NFLOW_OK;
+}
+
+// Whether the memory that two matrices span meets.
+struct Span {
+    const void* p;
+    int64_t rows, cols, ld;
+};
+bool meet(const Span& a, const Span& b, size_t e) {
+    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.cols <= 0 || b.cols <= 0) return false;
+    auto end = [e](const Span& s) {
+        return reinterpret_cast<uintptr_t>(s.p) + (static_cast<uintptr_t>(s.rows - 1) * s.ld + s.cols) * e;
+    };
+    return reinterpret_cast<uintptr_t>(a.p) < end(b) && reinterpret_cast<uintptr_t>(b.p) < end(a);
+}
+// The same, where lying in the same rows is allowed.
+bool clash(const Span& a, const Span& b, size_t e) {
+    return a.p && b.p && a.cols > 0 && rows_clash(a.p, a.ld, b.p, b.ld, a.rows, a.cols, e);
+}
+
+struct BackwardSpace {
+    size_t sums, x, w;
+    BackwardSpace(int64_t M, int64_t N, int64_t K, int dtype)
+        : sums(round16(static_cast<size_t>(M > 0 ? dz_runs(M, N) * N : 0) * sizeof(float))),
+          x(product_space(DENSE_DX, M, K, N, dtype)), w(product_space(DENSE_DW, N, K, M, dtype)) {}
+    size_t bytes() const { return sums + x + w; }
+};
+
+constexpr const char* kShared = "a result shares memory with an input or another result";
+
+}  // namespace
+}  // namespace nfq
+
+using namespace nfq;
+
+extern "C" {
+
+int nflow_dense_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
+    clear_error();
+    const char* what = "dense_linear_workspace";
+    if (!bytes) return bad_arg(what, "null output");
+    *bytes = 0;
+    if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
+    *bytes = product_space(DENSE_FORWARD, M, N, K, dtype);
+    return NFLOW_OK;
+}
+
+int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* W, int64_t ldw,
+                       int64_t N, const float* bias, const void* residual, int64_t ldr, int activation, void* y,
+                       int64_t ldy, void* pre, int64_t ldpre, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+    clear_error();
+    const char* what = "dense_linear";
+    if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
+    if (int rc = check_act(what, activation)) return rc;
+    if (ldx < K || ldw < K || ldy < N || (residual && ldr < N) || (pre && ldpre < N))
+        return bad_arg(what, "row stride smaller than a row");
+    if (int rc = check_workspace(what, workspace, workspace_bytes, product_space(DENSE_FORWARD, M, N, K, dtype))) return rc;
+    if (M == 0 || N == 0) return NFLOW_OK;
+    if (!y) return bad_arg(what, "null y");
+    if (K > 0 && (!x || !W)) return bad_arg(what, "null x or W");
+    const size_t e = dtype_size(dtype);
+    const Span sx{x, M, K, ldx}, sw{W, N, K, ldw}, sr{residual, M, N, ldr}, sy{y, M, N, ldy}, sp{pre, M, N, ldpre};
+    if (meet(sx, sy, e) || meet(sw, sy, e) || meet(sx, sp, e) || meet(sw, sp, e) || meet(sy, sp, e) || meet(sr, sp, e) ||
+        clash(sr, sy, e))
+        return bad_arg(what, kShared);
+    const DenseArgs a{x, W, ldx, ldw, M, N, K, bias, residual, ldr, activation, y, ldy, pre, ldpre};
+    return product(what, DENSE_FORWARD, a, dtype, workspace, as_stream(stream));
+}
+
+int nflow_dense_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
+    clear_error();
+    const char* what = "dense_linear_backward_workspace";
+    if (!bytes) return bad_arg(what, "null output");
+    *bytes = 0;
+    if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
+    *bytes = BackwardSpace(M, N, K, dtype).bytes();
+    return NFLOW_OK;
+}
+
+int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N, int64_t lddy, const void* x,
+                                int64_t ldx, const void* W, int64_t ldw, int64_t K, int activation, const void* pre,
+                                int64_t ldpre, void* dz, int64_t lddz, void* dx, int64_t lddx, void* dW,
+                                int64_t lddw, float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    const char* what = "dense_linear_backward";
+    if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
+    if (int rc = check_act(what, activation)) return rc;
+    const bool act = activation != NFLOW_ACT_NONE;
+    if (!act && (pre || dz)) return bad_arg(what, "pre and dz are of an activation, and there is none");
+    if (lddy < N || (dW && ldx < K) || (dx && ldw < K) || (act && (ldpre < N || lddz < N)) || (dx && lddx < K) ||
+        (dW && lddw < K))
+        return bad_arg(what, "row stride smaller than a row");
+    const BackwardSpace sp(M, N, K, dtype);
+    if (int rc = check_workspace(what, workspace, workspace_bytes, sp.bytes())) return rc;
+    if (M > 0 && N > 0) {
+        if (!dy || (act && (!pre || !dz))) return bad_arg(what, "null dy, pre or dz");
+        if (K > 0 && ((dx && !W) || (dW && !x))) return bad_arg(what, "null x or W");
+    }
+    const size_t e = dtype_size(dtype);
+    const Span sdy{dy, M, N, lddy}, spr{pre, M, N, ldpre}, sdz{dz, M, N, lddz}, sx{dW ? x : nullptr, M, K, ldx},
+        sw{dx ? W : nullptr, N, K, ldw}, sdx{dx, M, K, lddx}, sdw{dW, N, K, lddw};
+    for (const Span* in : {&sdy, &spr, &sdz, &sx, &sw})
+        if (meet(*in, sdx, e) || meet(*in, sdw, e)) return bad_arg(what, kShared);
+    if (meet(sdx, sdw, e) || meet(sx, sdz, e) || meet(sw, sdz, e) || clash(sdy, sdz, e) || clash(spr, sdz, e))
+        return bad_arg(what, kShared);
+    hipStream_t st = as_stream(stream);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    float* sums = reinterpret_cast<float*>(ws);
+    const int64_t runs = dz_runs(M, N);
+    if (M > 0 && N > 0 && (act || dbias)) {
+        const DzArgs a{dy, pre, dz, M, N, lddy, ldpre, lddz, activation, dbias ? sums : nullptr, (M + runs - 1) / runs};
+        const dim3 grid(static_cast<unsigned>((N + kDzCols - 1) / kDzCols), static_cast<unsigned>(runs));
+        if (dtype == NFLOW_DTYPE_BF16) hipLaunchKernelGGL((k_dense_dz<bf16>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_dense_dz<float>), grid, dim3(256), 0, st, a);
+    }
+    if (dbias && N > 0)
+        hipLaunchKernelGGL(k_dense_dbias, dim3(static_cast<unsigned>((N + 15) / 16)), dim3(256), 0, st, sums,
+                           M > 0 ? runs : 0, N, dbias);
+    if (int rc = launch_status(what)) return rc;
+    const void* g = act ? dz : dy;
+    const int64_t ldg = act ? lddz : lddy;
+    if (dx && K > 0) {
+        const DenseArgs a{g, W, ldg, ldw, M, K, N, nullptr, nullptr, 0, NFLOW_ACT_NONE, dx, lddx, nullptr, 0};
+        if (int rc = product(what, DENSE_DX, a, dtype, ws + sp.sums, st)) return rc;
+    }
+    if (dW && K > 0) {
+        const DenseArgs a{g, x, ldg, ldx, N, K, M, nullptr, nullptr, 0, NFLOW_ACT_NONE, dW, lddw, nullptr, 0};
+        if (int rc = product(what, DENSE_DW, a, dtype, ws + sp.sums + sp.x, st)) return rc;
+    }
+    return NFLOW_OK;
+}
+
+int nflow_debug_dense_cut(int form, int64_t M, int64_t N, int64_t K, int dtype, int* edge, int* splits) {
+    clear_error();
+    const char* what = "debug_dense_cut";
+    if (!edge || !splits) return bad_arg(what, "null output");
+    if (form < 0 || form > 2) return bad_arg(what, "unknown form");
+    if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
+    const DensePlan p = dense_plan(static_cast<DenseForm>(form), M, N, K, dtype);
+    *edge = p.kind == DENSE_FEW ? 0 : p.kind == DENSE_SMALL ? 64 : p.kind == DENSE_MID ? 128 : 256;
+    *splits = p.splits;
+    return NFLOW_OK;
+}
+
+}  // extern "C"
