@@ -108,9 +108,15 @@ int64_t dz_runs(int64_t M, int64_t N) {
 DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype) {
     if (form == DENSE_FORWARD && M <= kDenseFewRows) return DensePlan{DENSE_FEW, 1, 0};
     auto tiles = [&](int64_t e) { return ((M + e - 1) / e) * ((N + e - 1) / e); };
-    const DenseKind kind = tiles(128) >= num_cus() ? DENSE_MID : DENSE_SMALL;
-    const int64_t t = tiles(kind == DENSE_MID ? 128 : 64), steps = (K + 63) / 64;
+    DenseKind kind = tiles(128) >= num_cus() ? DENSE_MID : DENSE_SMALL;
+    if (dtype == NFLOW_DTYPE_BF16 && tiles(256) >= num_cus()) kind = DENSE_BIG;
+    static const char* force = getenv("DENSE_KIND");
+    if (force) kind = force[0] == 's' ? DENSE_SMALL : force[0] == 'm' ? DENSE_MID : DENSE_BIG;
+    const int64_t t = tiles(kind == DENSE_BIG ? 256 : kind == DENSE_MID ? 128 : 64), steps = (K + 63) / 64;
     int s = 1;
+    static const char* fs = getenv("DENSE_SPLITS");
+    if (fs) s = atoi(fs);
+    else
     while (s < 16 && 2 * s * t <= 2 * num_cus() && 4 * s <= steps) s *= 2;
     return DensePlan{kind, s, s > 1 ? round16(static_cast<size_t>(s) * M * N * sizeof(float)) : 0};
 }

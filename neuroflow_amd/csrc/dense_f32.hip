@@ -9,8 +9,8 @@ using Mid = DenseTile<float, 2, 2, 4, 4, 1>;       // 128 x 128, four waves
 
 template <bool AX, bool BX>
 void launch(const DenseArgs& a, const DensePlan& p, float* part, hipStream_t st) {
-    if (p.kind == DENSE_SMALL) launch_dense_tile<float, AX, BX, Small>(a, p.splits, part, st);
-    else launch_dense_tile<float, AX, BX, Mid>(a, p.splits, part, st);
+    if (p.kind == DENSE_SMALL) launch_dense_tile<float, Small, &k_dense<float, AX, BX, Small>>(a, p.splits, part, st);
+    else launch_dense_tile<float, Mid, &k_dense<float, AX, BX, Mid>>(a, p.splits, part, st);
 }
 
 }  // namespace

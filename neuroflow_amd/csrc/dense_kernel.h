@@ -46,9 +46,9 @@ __device__ __forceinline__ void dense_split(const float (&v)[8], v8bf (&p)[3]) {
 
 // Tiles of BM x BN, WM x WN waves of TI x TJ 16 x 16 tiles each; a stage is KB
 // values of k of every row, NS stages.
-template <typename T, int WM_, int WN_, int TI_, int TJ_, int NS_>
+template <typename T, int WM_, int WN_, int TI_, int TJ_, int NS_, int OCC_ = 2>
 struct DenseTile {
-    static constexpr int WM = WM_, WN = WN_, TI = TI_, TJ = TJ_, NS = NS_;
+    static constexpr int WM = WM_, WN = WN_, TI = TI_, TJ = TJ_, NS = NS_, OCC = OCC_;
     static constexpr int P = dense_planes<T>();
     static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int BM = 16 * TI * WM, BN = 16 * TJ * WN;
@@ -74,13 +74,13 @@ __device__ __forceinline__ int dense_place(int i, int c) {
     }
 }
 
-// A 16-row fragment of 32 k's (step hh of the stage): lane (r, g) has row row0 +
-// r, k's 32 hh + 8 g .. + 7.
+// A 16-row fragment of 32 k's: lane (r, g) = (l % 16, l / 16) has row row0 + r, k's
+// k0 + 8 g .. + 7.
 template <bool ACROSS, int R, int KB>
-__device__ __forceinline__ v8bf dense_fragment(const uint8_t* plane, int row0, int hh) {
+__device__ __forceinline__ v8bf dense_fragment(const uint8_t* plane, int row0, int k0) {
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     if constexpr (!ACROSS) {
-        return *reinterpret_cast<const v8bf*>(plane + dense_place<false, R, KB>(row0 + r, 4 * hh + g));
+        return *reinterpret_cast<const v8bf*>(plane + dense_place<false, R, KB>(row0 + r, k0 / 8 + g));
     } else {
         // Lane i of a group of 16 addresses row i / 4 and columns 4 (i % 4) .. + 3.
         union {
@@ -89,7 +89,7 @@ __device__ __forceinline__ v8bf dense_fragment(const uint8_t* plane, int row0, i
         } u;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            const int k = 32 * hh + 8 * g + 4 * q + (r >> 2), c = row0 + 4 * (r & 3);
+            const int k = k0 + 8 * g + 4 * q + (r >> 2), c = row0 + 4 * (r & 3);
             const uint8_t* p = plane + dense_place<true, R, KB>(k, c >> 3) + 2 * (c & 7);
             u.half[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)p);
         }
@@ -243,18 +243,18 @@ __device__ __forceinline__ void dense_step(const uint8_t* st, v4f (&acc)[Tile::T
     constexpr int P = Tile::P, TI = Tile::TI, TJ = Tile::TJ, KB = Tile::KB;
     const uint8_t* sb = st + P * Tile::PLANE_A;
 #pragma unroll
-    for (int hh = 0; hh < KB / 32; ++hh) {
+    for (int k = 0; k < KB; k += 32) {
         v8bf bf[P][TJ];
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll
             for (int j = 0; j < TJ; ++j)
-                bf[p][j] = dense_fragment<BX, Tile::BN, KB>(sb + p * Tile::PLANE_B, brow + 16 * j, hh);
+                bf[p][j] = dense_fragment<BX, Tile::BN, KB>(sb + p * Tile::PLANE_B, brow + 16 * j, k);
 #pragma unroll
         for (int i = 0; i < TI; ++i) {
             v8bf af[P];
 #pragma unroll
-            for (int p = 0; p < P; ++p) af[p] = dense_fragment<AX, Tile::BM, KB>(st + p * Tile::PLANE_A, arow + 16 * i, hh);
+            for (int p = 0; p < P; ++p) af[p] = dense_fragment<AX, Tile::BM, KB>(st + p * Tile::PLANE_A, arow + 16 * i, k);
             if constexpr (P == 1) {
 #pragma unroll
                 for (int j = 0; j < TJ; ++j)
@@ -272,7 +272,7 @@ __device__ __forceinline__ void dense_step(const uint8_t* st, v4f (&acc)[Tile::T
 }
 
 template <typename T, bool AX, bool BX, typename Tile>
-__global__ __launch_bounds__(Tile::THREADS, 2) void k_dense(DenseArgs a, DenseShare sh) {
+__global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense(DenseArgs a, DenseShare sh) {
     constexpr int TI = Tile::TI, TJ = Tile::TJ, KB = Tile::KB;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -334,16 +334,16 @@ __global__ __launch_bounds__(256) void k_dense_join(DenseArgs a, const float* __
     }
 }
 
-template <typename T, bool AX, bool BX, typename Tile>
+// `kernel` over the tiles of the product and its splits, and their join.
+template <typename T, typename Tile, auto kernel>
 void launch_dense_tile(const DenseArgs& a, int splits, float* part, hipStream_t st) {
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_dense<T, AX, BX, Tile>),
+    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, Tile::LDS);
     (void)once;
     const int64_t tm = (a.M + Tile::BM - 1) / Tile::BM, tn = (a.N + Tile::BN - 1) / Tile::BN;
     const int ks = static_cast<int>((a.K + Tile::KB - 1) / Tile::KB);
     const DenseShare sh{tm, tn, splits, (ks + splits - 1) / splits, part, static_cast<int>(tm * tn * splits)};
-    hipLaunchKernelGGL((k_dense<T, AX, BX, Tile>), dim3(static_cast<unsigned>(sh.blocks)), dim3(Tile::THREADS), Tile::LDS,
-                       st, a, sh);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(sh.blocks)), dim3(Tile::THREADS), Tile::LDS, st, a, sh);
     if (splits > 1)
         hipLaunchKernelGGL((k_dense_join<T>), dim3(grid_for(a.M * ((a.N + 3) / 4), 256, 8)), dim3(256), 0, st, a, part,
                            splits);
