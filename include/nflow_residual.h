@@ -72,12 +72,14 @@ int nflow_rms_norm_backward_workspace(int64_t M, int64_t D, size_t* bytes);
  * bf16 parts of each operand, which hold it exactly, without the three smallest
  * of nine (2^-26 of a product); an infinite operand gives NaN there, as a NaN
  * does.  y may be residual at the same row stride; y and pre may share no other
- * memory with an input or one another. */
+ * memory with an input or one another.  A bf16 operand x or W whose address, row
+ * stride and row are not whole 16-byte groups is copied into the workspace first
+ * (but for a few rows, M <= 32): `copies` asks for the room, if any may be such. */
 int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* W, int64_t ldw,
                        int64_t N, const float* bias, const void* residual, int64_t ldr, int activation, void* y,
                        int64_t ldy, void* pre, int64_t ldpre, void* workspace, size_t workspace_bytes,
                        void* stream);
-int nflow_dense_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes);
+int nflow_dense_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, int copies, size_t* bytes);
 
 /* The gradients of nflow_dense_linear from dy (M, N):
  *   dz = dy * act'(pre) (M, N), the gradient of residual too,
@@ -87,12 +89,12 @@ int nflow_dense_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, siz
  * dz and pre are NULL; with one both are required (for ReLU pre may be y).  dx,
  * dW and dbias may each be NULL (not wanted).  M = 0 gives zero dW and dbias.
  * dz may be dy or pre at the same row stride; results share no other memory
- * with an input or one another. */
+ * with an input or one another.  `copies` as above, for dz (or dy), x and W. */
 int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N, int64_t lddy, const void* x,
                                 int64_t ldx, const void* W, int64_t ldw, int64_t K, int activation, const void* pre,
                                 int64_t ldpre, void* dz, int64_t lddz, void* dx, int64_t lddx, void* dW,
                                 int64_t lddw, float* dbias, void* workspace, size_t workspace_bytes, void* stream);
-int nflow_dense_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes);
+int nflow_dense_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, int copies, size_t* bytes);
 
 /* ---- gradient clipping ---- */
 
@@ -119,14 +121,15 @@ int nflow_grad_norm(const nflow_grad_tensor* tensors, int count, float* norm, vo
 int nflow_grad_clip(const nflow_grad_tensor* tensors, int count, float max_norm, float* norm, void* workspace,
                     size_t workspace_bytes, void* stream);
 
-/* For both; depends on the tensors' counts alone. */
-int nflow_grad_workspace(const nflow_grad_tensor* tensors, int count, size_t* bytes);
+/* For both, of `count` tensors. */
+int nflow_grad_workspace(int count, size_t* bytes);
 
 /* ---- for tests: which kernel a size takes (no GPU needed: 256 CUs without one) ---- */
 
 /* The tile edge of the linear layer's product at this size, or 0 for the few-row
- * kernel, and the runs that K is split into.  form: 0 forward, 1 dx, 2 dW. */
-int nflow_debug_dense_cut(int form, int64_t M, int64_t N, int64_t K, int dtype, int* edge, int* splits);
+ * kernel, and the workgroups that share tiles, or 0 where none does.  form: 0
+ * forward, 1 dx, 2 dW. */
+int nflow_debug_dense_cut(int form, int64_t M, int64_t N, int64_t K, int dtype, int* edge, int* groups);
 
 #ifdef __cplusplus
 }

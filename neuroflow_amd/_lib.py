@@ -174,13 +174,13 @@ SIGNATURES = {
     "nflow_rms_norm_backward_workspace": [_i64, _i64, C.POINTER(C.c_size_t)],
     "nflow_dense_linear": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp,
                            C.c_size_t, _vp],
-    "nflow_dense_linear_workspace": [_i64, _i64, _i64, _i32, C.POINTER(C.c_size_t)],
+    "nflow_dense_linear_workspace": [_i64, _i64, _i64, _i32, _i32, C.POINTER(C.c_size_t)],
     "nflow_dense_linear_backward": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _i64,
                                     _vp, _i64, _vp, _i64, _vp, _vp, C.c_size_t, _vp],
-    "nflow_dense_linear_backward_workspace": [_i64, _i64, _i64, _i32, C.POINTER(C.c_size_t)],
+    "nflow_dense_linear_backward_workspace": [_i64, _i64, _i64, _i32, _i32, C.POINTER(C.c_size_t)],
     "nflow_grad_norm": [C.POINTER(GradTensorC), _i32, _vp, _vp, C.c_size_t, _vp],
     "nflow_grad_clip": [C.POINTER(GradTensorC), _i32, _f32, _vp, _vp, C.c_size_t, _vp],
-    "nflow_grad_workspace": [C.POINTER(GradTensorC), _i32, C.POINTER(C.c_size_t)],
+    "nflow_grad_workspace": [_i32, C.POINTER(C.c_size_t)],
     "nflow_debug_dense_cut": [_i32, _i64, _i64, _i64, _i32, C.POINTER(_i32), C.POINTER(_i32)],
     # include/nflow_runtime.h
     "nflow_runtime_create": [C.c_char_p, C.POINTER(_vp)],

@@ -88,6 +88,11 @@ inline py::tuple rms_norm_backward(const Tensor& dy, const Tensor& x, const Mayb
 
 // ---- the linear layer in bf16 or fp32 ----
 
+// Whether a bf16 operand may have to be copied (nflow_dense_linear).
+inline bool odd(const Tensor& t, const Matrix& m) {
+    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) != 0 || m.ld % 8 != 0 || m.cols % 8 != 0;
+}
+
 // A weight (N, K) of x's type.
 inline Matrix weight_of(const Tensor& W, const Tensor& x, int64_t cols, const char* of) {
     dtype_of(W, "W");
@@ -125,7 +130,7 @@ inline py::tuple dense_linear(const Tensor& x, const Tensor& W, const Maybe& bia
     }
     if (return_pre) pre = empty(size, x, x.scalar_type());
     size_t n = 0;
-    ok(api.nflow_dense_linear_workspace(m.rows, N, m.cols, dt, &n), "dense_linear");
+    ok(api.nflow_dense_linear_workspace(m.rows, N, m.cols, dt, odd(x, m) || odd(W, w), &n), "dense_linear");
     const Tensor ws = scratch(n, x);
     ok(api.nflow_dense_linear(data(x), dt, m.rows, m.cols, m.ld, data(W), w.ld, N, b, residual ? data(*residual) : nullptr,
                               r.ld, act, data(y), yl.ld, data(pre), N, data(ws), n, stream_of(x)), "dense_linear");
@@ -158,7 +163,7 @@ inline py::tuple dense_linear_backward(const Tensor& dy, const Tensor& x, const 
     const Tensor dx = empty(size, dy, dy.scalar_type()), dW = empty({m.cols, K}, dy, dy.scalar_type());
     const Tensor db = empty({m.cols}, dy, at::kFloat);
     size_t n = 0;
-    ok(api.nflow_dense_linear_backward_workspace(m.rows, m.cols, K, dt, &n), "dense_linear_backward");
+    ok(api.nflow_dense_linear_backward_workspace(m.rows, m.cols, K, dt, odd(dy, m) || odd(x, xm) || odd(W, w), &n), "dense_linear_backward");
     const Tensor ws = scratch(n, dy);
     ok(api.nflow_dense_linear_backward(data(dy), dt, m.rows, m.cols, m.ld, data(x), xm.ld, data(W), w.ld, K, act,
                                        pre ? data(*pre) : nullptr, p.ld, data(dz), m.cols, data(dx), K, data(dW), K,
@@ -200,7 +205,7 @@ inline Tensor global_norm(const std::vector<Tensor>& grads) {
     const int count = static_cast<int>(l.t.size());
     const Tensor norm = empty({}, *l.like, at::kFloat);
     size_t n = 0;
-    ok(api.nflow_grad_workspace(l.t.data(), count, &n), "grad_norm");
+    ok(api.nflow_grad_workspace(count, &n), "grad_norm");
     const Tensor ws = scratch(n, *l.like);
     ok(api.nflow_grad_norm(l.t.data(), count, data<float>(norm), data(ws), n, stream_of(*l.like)), "grad_norm");
     return norm;
@@ -216,7 +221,7 @@ inline Tensor clip_by_global_norm(const std::vector<Tensor>& grads, double max_n
     const int count = static_cast<int>(l.t.size());
     const Tensor norm = empty({}, *l.like, at::kFloat);
     size_t n = 0;
-    ok(api.nflow_grad_workspace(l.t.data(), count, &n), "grad_clip");
+    ok(api.nflow_grad_workspace(count, &n), "grad_clip");
     const Tensor ws = scratch(n, *l.like);
     ok(api.nflow_grad_clip(l.t.data(), count, static_cast<float>(max_norm), data<float>(norm), data(ws), n,
                            stream_of(*l.like)), "grad_clip");

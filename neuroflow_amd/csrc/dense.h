@@ -27,21 +27,35 @@ struct DenseArgs {
 // Which operands lie across k: the layer's three products.
 enum DenseForm { DENSE_FORWARD = 0, DENSE_DX = 1, DENSE_DW = 2 };
 
-// How a product is cut: the kernel or tile, and the runs that K is split into
-// (joined by a second launch).
-enum DenseKind { DENSE_FEW, DENSE_SMALL, DENSE_MID, DENSE_BIG };
+// How a product is cut: the kernel or tile, and, unless 0, the workgroups that
+// the tiles and the K steps of what is left of them are dealt out to.
+enum DenseKind { DENSE_FEW, DENSE_SMALL, DENSE_MID, DENSE_DEEP, DENSE_BIG };
 struct DensePlan {
     DenseKind kind;
-    int splits;
-    size_t bytes;       // of the partial results
+    int groups;
+    size_t bytes;       // of the shared tiles' partial results
 };
 
 // The tiled product, one translation unit per type.
-template <typename T>
-void launch_dense(const DenseArgs& a, DenseForm form, const DensePlan& p, float* part, hipStream_t st);
+void launch_dense_bf16(const DenseArgs& a, DenseForm form, const DensePlan& p, float* part, hipStream_t st);
+void launch_dense_f32(const DenseArgs& a, DenseForm form, const DensePlan& p, float* part, hipStream_t st);
+
+// A bf16 operand as the tiled product can fetch it: whole 16-byte groups at
+// 16-byte places, and a tile's rows within a buffer's range.
+inline bool dense_fetchable(const void* p, int64_t ld, int64_t cols) {
+    return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0 && ld < (INT64_C(1) << 21);
+}
+// Others are copied into rows of this many values.
+__host__ __device__ inline int64_t dense_pitch(int64_t cols) { return (cols + 7) / 8 * 8; }
+struct DensePack {
+    const void* from;
+    void* to;
+    int64_t rows, cols, ld;
+};
+void launch_dense_pack(const DensePack (&m)[3], hipStream_t st);
 
 // The product for few rows, operands along k (dense_few.hip).
-constexpr int64_t kDenseFewRows = 64;
+constexpr int64_t kDenseFewRows = 32;
 template <typename T>
 void launch_dense_few(const DenseArgs& a, hipStream_t st);
 

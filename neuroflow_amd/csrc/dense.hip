@@ -105,20 +105,58 @@ int64_t dz_runs(int64_t M, int64_t N) {
 
 // ---- the cut -----------------------------------------------------------------------------
 
+// The cut with the least estimated time, in us: `steps` of 64 k's, of which a
+// workgroup alone on its CU takes `alone` each and n together `each` apiece, and
+// `tile` for what a tile does outside its K loop.  Dealt out whole, the busiest
+// CU has ceil(tiles / CUs) of them.  Dealt out to `groups` workgroups, with the K
+// steps of what is left shared evenly, every CU is as busy as the next, for the
+// shared parts' way through the caches and a second launch.  Fitted to MI355X
+// times at 256 to 1024 tiles of 16 and 64 steps.
 DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype) {
-    if (form == DENSE_FORWARD && M <= kDenseFewRows) return DensePlan{DENSE_FEW, 1, 0};
-    auto tiles = [&](int64_t e) { return ((M + e - 1) / e) * ((N + e - 1) / e); };
-    DenseKind kind = tiles(128) >= num_cus() ? DENSE_MID : DENSE_SMALL;
-    if (dtype == NFLOW_DTYPE_BF16 && tiles(256) >= num_cus()) kind = DENSE_BIG;
-    static const char* force = getenv("DENSE_KIND");
-    if (force) kind = force[0] == 's' ? DENSE_SMALL : force[0] == 'm' ? DENSE_MID : DENSE_BIG;
-    const int64_t t = tiles(kind == DENSE_BIG ? 256 : kind == DENSE_MID ? 128 : 64), steps = (K + 63) / 64;
-    int s = 1;
-    static const char* fs = getenv("DENSE_SPLITS");
-    if (fs) s = atoi(fs);
-    else
-    while (s < 16 && 2 * s * t <= 2 * num_cus() && 4 * s <= steps) s *= 2;
-    return DensePlan{kind, s, s > 1 ? round16(static_cast<size_t>(s) * M * N * sizeof(float)) : 0};
+    const bool f32 = dtype == NFLOW_DTYPE_F32;
+    const double cus = num_cus(), m = static_cast<double>(M), n = static_cast<double>(N),
+                 steps = std::ceil(static_cast<double>(K) / 64);
+    struct Cut {
+        DenseKind kind;
+        int bm, bn, per_cu;
+        double alone, each, tile;
+    };
+    static const Cut of_bf16[] = {{DENSE_SMALL, 64, 64, 3, 0.233, 0.182, 0.7},
+                                  {DENSE_MID, 128, 128, 2, 0.613, 0.435, 2.4},
+                                  {DENSE_DEEP, 128, 128, 1, 0.481, 0.476, 2.6},
+                                  {DENSE_BIG, 256, 256, 1, 1.43, 1.50, 5.3}};
+    static const Cut of_f32[] = {{DENSE_SMALL, 64, 64, 3, 0.98, 0.99, 0.7},
+                                 {DENSE_MID, 128, 128, 1, 2.66, 2.66, 2.5},
+                                 {DENSE_BIG, 256, 128, 1, 4.77, 4.77, 5.0}};
+    DensePlan best{DENSE_MID, 0, 0};
+    double least = HUGE_VAL;
+    static const char* fk = getenv("DENSE_KIND");
+    static const char* fs = getenv("DENSE_GROUPS");
+    if (form == DENSE_FORWARD && M <= kDenseFewRows && (!fk || fk[0] == 'f')) return DensePlan{DENSE_FEW, 0, 0};
+    for (int i = 0; i < (f32 ? 3 : 4); ++i) {
+        const Cut& c = f32 ? of_f32[i] : of_bf16[i];
+        if (fk && fk[0] != (c.kind == DENSE_BIG ? 'b' : c.kind == DENSE_MID ? 'm' : c.kind == DENSE_DEEP ? 'd' : 's')) continue;
+        const double tiles = std::ceil(m / c.bm) * std::ceil(n / c.bn), per = std::ceil(tiles / cus);
+        const double plain = steps * std::max(c.alone, per * c.each) + per * c.tile;
+        if (plain < least && (!fs || atoi(fs) == 0)) {
+            least = plain;
+            best = DensePlan{c.kind, 0, 0};
+        }
+        for (int occ = 1; occ <= c.per_cu; ++occ) {
+            const int groups = occ * static_cast<int>(cus);
+            if (fs && atoi(fs) != occ) continue;
+            const int64_t t = static_cast<int64_t>(tiles), rest = t % groups;
+            if (rest == 0 || rest * steps < groups) continue;
+            const double share = (t / groups) * steps + rest * steps / groups + 0.5;
+            const double moved = 2.0 * (groups + rest) * c.bm * c.bn * 4;
+            const double time = share * std::max(c.alone, occ * c.each) + (t / groups + 2) * occ * c.tile + 3.0 + moved / 5e6;
+            if (time < least) {
+                least = time;
+                best = DensePlan{c.kind, groups, static_cast<size_t>(2) * groups * c.bm * c.bn * sizeof(float)};
+            }
+        }
+    }
+    return best;
 }
 
 size_t product_space(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype) {
@@ -128,15 +166,36 @@ size_t product_space(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype)
 int product(const char* what, DenseForm form, const DenseArgs& a, int dtype, void* ws, hipStream_t st) {
     if (a.M == 0 || a.N == 0) return NFLOW_OK;
     const DensePlan p = dense_plan(form, a.M, a.N, a.K, dtype);
+    const bool b16 = dtype == NFLOW_DTYPE_BF16;
     if (p.kind == DENSE_FEW) {
-        if (dtype == NFLOW_DTYPE_BF16) launch_dense_few<bf16>(a, st);
+        if (b16) launch_dense_few<bf16>(a, st);
         else launch_dense_few<float>(a, st);
     } else {
-        if (dtype == NFLOW_DTYPE_BF16) launch_dense<bf16>(a, form, p, static_cast<float*>(ws), st);
-        else launch_dense<float>(a, form, p, static_cast<float*>(ws), st);
+        if (b16) launch_dense_bf16(a, form, p, static_cast<float*>(ws), st);
+        else launch_dense_f32(a, form, p, static_cast<float*>(ws), st);
     }
     return launch_status(what);
 }
+
+// ---- operands that the tiled product of bf16 cannot fetch where they lie ---------------------
+
+size_t copy_space(int64_t rows, int64_t cols) { return round16(static_cast<size_t>(rows * dense_pitch(cols)) * 2); }
+
+// Operands on their way into a product; those that need it are copied to `to`, all by one launch.
+struct Copies {
+    DensePack m[3] = {};
+    int n = 0;
+    size_t bytes = 0;
+    // p and its row stride, as the product takes them.
+    void take(const void*& p, int64_t& ld, int64_t rows, int64_t cols, void* to) {
+        if (dense_fetchable(p, ld, cols)) return;
+        uint8_t* at = static_cast<uint8_t*>(to) + bytes;
+        m[n++] = DensePack{p, at, rows, cols, ld};
+        bytes += copy_space(rows, cols);
+        p = at;
+        ld = dense_pitch(cols);
+    }
+};
 
 int check_sizes(const char* what, int64_t M, int64_t N, int64_t K, int dtype) {
     if (M < 0 || N < 0 || K < 0) return bad_arg(what, "bad dims");
@@ -180,6 +239,11 @@ struct BackwardSpace {
     size_t bytes() const { return sums + x + w; }
 };
 
+// Whether the forward product of these sizes is a tiled one of bf16.
+bool forward_copies(int64_t M, int64_t N, int64_t K, int dtype) {
+    return dtype == NFLOW_DTYPE_BF16 && M > 0 && N > 0 && K > 0 && dense_plan(DENSE_FORWARD, M, N, K, dtype).kind != DENSE_FEW;
+}
+
 constexpr const char* kShared = "a result shares memory with an input or another result";
 
 }  // namespace
@@ -189,13 +253,14 @@ using namespace nfq;
 
 extern "C" {
 
-int nflow_dense_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
+int nflow_dense_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, int copies, size_t* bytes) {
     clear_error();
     const char* what = "dense_linear_workspace";
     if (!bytes) return bad_arg(what, "null output");
     *bytes = 0;
     if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
     *bytes = product_space(DENSE_FORWARD, M, N, K, dtype);
+    if (copies && forward_copies(M, N, K, dtype)) *bytes += copy_space(M, K) + copy_space(N, K);
     return NFLOW_OK;
 }
 
@@ -209,7 +274,15 @@ int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     if (int rc = check_act(what, activation)) return rc;
     if (ldx < K || ldw < K || ldy < N || (residual && ldr < N) || (pre && ldpre < N))
         return bad_arg(what, "row stride smaller than a row");
-    if (int rc = check_workspace(what, workspace, workspace_bytes, product_space(DENSE_FORWARD, M, N, K, dtype))) return rc;
+    const size_t parts = product_space(DENSE_FORWARD, M, N, K, dtype);
+    Copies copies;
+    const void *px = x, *pw = W;
+    int64_t lx = ldx, lw = ldw;
+    if (forward_copies(M, N, K, dtype)) {
+        copies.take(px, lx, M, K, static_cast<uint8_t*>(workspace) + parts);
+        copies.take(pw, lw, N, K, static_cast<uint8_t*>(workspace) + parts);
+    }
+    if (int rc = check_workspace(what, workspace, workspace_bytes, parts + copies.bytes)) return rc;
     if (M == 0 || N == 0) return NFLOW_OK;
     if (!y) return bad_arg(what, "null y");
     if (K > 0 && (!x || !W)) return bad_arg(what, "null x or W");
@@ -218,17 +291,20 @@ int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     if (meet(sx, sy, e) || meet(sw, sy, e) || meet(sx, sp, e) || meet(sw, sp, e) || meet(sy, sp, e) || meet(sr, sp, e) ||
         clash(sr, sy, e))
         return bad_arg(what, kShared);
-    const DenseArgs a{x, W, ldx, ldw, M, N, K, bias, residual, ldr, activation, y, ldy, pre, ldpre};
-    return product(what, DENSE_FORWARD, a, dtype, workspace, as_stream(stream));
+    hipStream_t st = as_stream(stream);
+    if (copies.n) launch_dense_pack(copies.m, st);
+    const DenseArgs a{px, pw, lx, lw, M, N, K, bias, residual, ldr, activation, y, ldy, pre, ldpre};
+    return product(what, DENSE_FORWARD, a, dtype, workspace, st);
 }
 
-int nflow_dense_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
+int nflow_dense_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, int copies, size_t* bytes) {
     clear_error();
     const char* what = "dense_linear_backward_workspace";
     if (!bytes) return bad_arg(what, "null output");
     *bytes = 0;
     if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
     *bytes = BackwardSpace(M, N, K, dtype).bytes();
+    if (copies && dtype == NFLOW_DTYPE_BF16) *bytes += copy_space(M, N) + copy_space(N, K) + copy_space(M, K);
     return NFLOW_OK;
 }
 
@@ -246,7 +322,16 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
         (dW && lddw < K))
         return bad_arg(what, "row stride smaller than a row");
     const BackwardSpace sp(M, N, K, dtype);
-    if (int rc = check_workspace(what, workspace, workspace_bytes, sp.bytes())) return rc;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    Copies copies;
+    const void *g = act ? dz : dy, *px = x, *pw = W;
+    int64_t lg = act ? lddz : lddy, lx = ldx, lw = ldw;
+    if (dtype == NFLOW_DTYPE_BF16 && M > 0 && N > 0 && K > 0) {
+        if (dx || dW) copies.take(g, lg, M, N, ws + sp.bytes());
+        if (dx) copies.take(pw, lw, N, K, ws + sp.bytes());
+        if (dW) copies.take(px, lx, M, K, ws + sp.bytes());
+    }
+    if (int rc = check_workspace(what, workspace, workspace_bytes, sp.bytes() + copies.bytes)) return rc;
     if (M > 0 && N > 0) {
         if (!dy || (act && (!pre || !dz))) return bad_arg(what, "null dy, pre or dz");
         if (K > 0 && ((dx && !W) || (dW && !x))) return bad_arg(what, "null x or W");
@@ -259,7 +344,6 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
     if (meet(sdx, sdw, e) || meet(sx, sdz, e) || meet(sw, sdz, e) || clash(sdy, sdz, e) || clash(spr, sdz, e))
         return bad_arg(what, kShared);
     hipStream_t st = as_stream(stream);
-    uint8_t* ws = static_cast<uint8_t*>(workspace);
     float* sums = reinterpret_cast<float*>(ws);
     const int64_t runs = dz_runs(M, N);
     if (M > 0 && N > 0 && (act || dbias)) {
@@ -271,29 +355,28 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
     if (dbias && N > 0)
         hipLaunchKernelGGL(k_dense_dbias, dim3(static_cast<unsigned>((N + 15) / 16)), dim3(256), 0, st, sums,
                            M > 0 ? runs : 0, N, dbias);
+    if (copies.n) launch_dense_pack(copies.m, st);
     if (int rc = launch_status(what)) return rc;
-    const void* g = act ? dz : dy;
-    const int64_t ldg = act ? lddz : lddy;
     if (dx && K > 0) {
-        const DenseArgs a{g, W, ldg, ldw, M, K, N, nullptr, nullptr, 0, NFLOW_ACT_NONE, dx, lddx, nullptr, 0};
+        const DenseArgs a{g, pw, lg, lw, M, K, N, nullptr, nullptr, 0, NFLOW_ACT_NONE, dx, lddx, nullptr, 0};
         if (int rc = product(what, DENSE_DX, a, dtype, ws + sp.sums, st)) return rc;
     }
     if (dW && K > 0) {
-        const DenseArgs a{g, x, ldg, ldx, N, K, M, nullptr, nullptr, 0, NFLOW_ACT_NONE, dW, lddw, nullptr, 0};
+        const DenseArgs a{g, px, lg, lx, N, K, M, nullptr, nullptr, 0, NFLOW_ACT_NONE, dW, lddw, nullptr, 0};
         if (int rc = product(what, DENSE_DW, a, dtype, ws + sp.sums + sp.x, st)) return rc;
     }
     return NFLOW_OK;
 }
 
-int nflow_debug_dense_cut(int form, int64_t M, int64_t N, int64_t K, int dtype, int* edge, int* splits) {
+int nflow_debug_dense_cut(int form, int64_t M, int64_t N, int64_t K, int dtype, int* edge, int* groups) {
     clear_error();
     const char* what = "debug_dense_cut";
-    if (!edge || !splits) return bad_arg(what, "null output");
+    if (!edge || !groups) return bad_arg(what, "null output");
     if (form < 0 || form > 2) return bad_arg(what, "unknown form");
     if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
     const DensePlan p = dense_plan(static_cast<DenseForm>(form), M, N, K, dtype);
-    *edge = p.kind == DENSE_FEW ? 0 : p.kind == DENSE_SMALL ? 64 : p.kind == DENSE_MID ? 128 : 256;
-    *splits = p.splits;
+    *edge = p.kind == DENSE_FEW ? 0 : p.kind == DENSE_SMALL ? 64 : p.kind == DENSE_BIG ? 256 : 128;
+    *groups = p.groups;
     return NFLOW_OK;
 }
 

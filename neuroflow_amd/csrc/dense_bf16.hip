@@ -1,37 +1,62 @@
-// dense_bf16.hip -- the tiled product of bf16 operands.
+// dense_bf16.hip -- the tiled product of bf16 operands: its tiles, and the copies
+// of operands that the LDS-DMA cannot fetch.
 #include "dense_dma.h"
 
 namespace nfq {
 namespace {
 
-using Small = DenseTile<bf16, 2, 2, 2, 2, 1>;     // 64 x 64, four waves
-using Mid = DenseTile<bf16, 2, 2, 4, 4, 1>;       // 128 x 128, four waves
-using DmaSmall = DenseTile<bf16, 2, 2, 2, 2, 3>;
-using DmaMid = DenseTile<bf16, 2, 2, 4, 4, 2>;
-using DmaBig = DenseTile<bf16, 2, 4, 8, 4, 2>;    // 256 x 256, eight waves, a workgroup per CU
-
-// Whether the LDS-DMA can fetch an operand: whole 16-byte groups at 16-byte
-// places, and a tile's rows within a buffer's range.
-bool dma_ok(const void* p, int64_t ld, int64_t inner) {
-    return aligned(p, 16) && ld % 8 == 0 && inner % 8 == 0 && ld < (INT64_C(1) << 21);
-}
+using Small = DenseTile<bf16, 2, 2, 2, 2, 3, 3>;    // 64 x 64, four waves, three workgroups a CU
+using Mid = DenseTile<bf16, 2, 2, 4, 4, 2>;         // 128 x 128, four waves, two workgroups a CU
+using Deep = DenseTile<bf16, 2, 4, 4, 2, 4>;        // 128 x 128, eight waves, a workgroup a CU, loads three stages ahead
+using Big = DenseTile<bf16, 2, 4, 8, 4, 2>;         // 256 x 256, eight waves, a workgroup a CU
 
 template <bool AX, bool BX>
 void launch(const DenseArgs& a, const DensePlan& p, float* part, hipStream_t st) {
-    if (dma_ok(a.A, a.lda, AX ? a.M : a.K) && dma_ok(a.B, a.ldb, BX ? a.N : a.K)) {
-        if (p.kind == DENSE_BIG) launch_dense_tile<bf16, DmaBig, &k_dense_dma<AX, BX, DmaBig>>(a, p.splits, part, st);
-        else if (p.kind == DENSE_MID) launch_dense_tile<bf16, DmaMid, &k_dense_dma<AX, BX, DmaMid>>(a, p.splits, part, st);
-        else launch_dense_tile<bf16, DmaSmall, &k_dense_dma<AX, BX, DmaSmall>>(a, p.splits, part, st);
-        return;
-    }
-    if (p.kind == DENSE_SMALL) launch_dense_tile<bf16, Small, &k_dense<bf16, AX, BX, Small>>(a, p.splits, part, st);
-    else launch_dense_tile<bf16, Mid, &k_dense<bf16, AX, BX, Mid>>(a, p.splits, part, st);
+    if (p.kind == DENSE_BIG) launch_dense_tile<bf16, Big, &k_dense_dma<AX, BX, Big>>(a, p, part, st);
+    else if (p.kind == DENSE_DEEP) launch_dense_tile<bf16, Deep, &k_dense_dma<AX, BX, Deep>>(a, p, part, st);
+    else if (p.kind == DENSE_MID) launch_dense_tile<bf16, Mid, &k_dense_dma<AX, BX, Mid>>(a, p, part, st);
+    else launch_dense_tile<bf16, Small, &k_dense_dma<AX, BX, Small>>(a, p, part, st);
+}
+
+// Up to three matrices copied to rows of dense_pitch(cols) values, zero past
+// cols: a wave takes 512 columns of four rows, 16 bytes a lane.
+struct PackArgs {
+    DensePack m[3];
+    int64_t first[3];       // group of four rows of each matrix
+};
+__global__ __launch_bounds__(256) void k_dense_pack(PackArgs a) {
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int w = id < a.first[1] ? 0 : id < a.first[2] ? 1 : 2;
+    const DensePack& m = a.m[w];
+    const int64_t row = 4 * (id - a.first[w]), pitch = dense_pitch(m.cols);
+    const int64_t c = static_cast<int64_t>(blockIdx.y) * 512 + 8 * (threadIdx.x & 63);
+    if (row >= m.rows || c >= m.cols) return;
+    const bf16* from = static_cast<const bf16*>(m.from) + row * m.ld + c;
+    bf16* to = static_cast<bf16*>(m.to) + row * pitch + c;
+    Raw8<bf16> v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r].load(from + r * m.ld, row + r < m.rows ? m.cols - c : 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (row + r < m.rows) *reinterpret_cast<Raw8<bf16>::vec*>(to + r * pitch) = v[r].q;
 }
 
 }  // namespace
 
-template <>
-void launch_dense<bf16>(const DenseArgs& a, DenseForm form, const DensePlan& p, float* part, hipStream_t st) {
+void launch_dense_pack(const DensePack (&m)[3], hipStream_t st) {
+    PackArgs a;
+    int64_t n = 0, cols = 0;
+    for (int i = 0; i < 3; ++i) {
+        cols = std::max(cols, m[i].cols);
+        a.m[i] = m[i];
+        a.first[i] = n;
+        n += (m[i].rows + 3) / 4;
+    }
+    hipLaunchKernelGGL(k_dense_pack, dim3(static_cast<unsigned>((n + 3) / 4), static_cast<unsigned>((cols + 511) / 512)),
+                       dim3(256), 0, st, a);
+}
+
+void launch_dense_bf16(const DenseArgs& a, DenseForm form, const DensePlan& p, float* part, hipStream_t st) {
     if (form == DENSE_FORWARD) launch<false, false>(a, p, part, st);
     else if (form == DENSE_DX) launch<false, true>(a, p, part, st);
     else launch<true, true>(a, p, part, st);

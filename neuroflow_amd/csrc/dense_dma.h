@@ -50,10 +50,10 @@ struct DenseFetch {
     __device__ __forceinline__ v4u range(int k, bool on) const {
         if constexpr (!ACROSS) {
             const int64_t left = rows - row0 < R ? rows - row0 : R;
-            return wide_desc(base, on ? (left - 1) * ld2 + 2 * K : 0);
+            return wide_desc(base, on ? (left - 1) * ld2 + 2 * dense_pitch(K) : 0);
         } else {
             const int64_t at = static_cast<int64_t>(k) * KB, left = K - at < KB ? K - at : KB;
-            return wide_desc(base + at * ld2, on ? (left - 1) * ld2 + 2 * (rows - row0) : 0);
+            return wide_desc(base + at * ld2, on ? (left - 1) * ld2 + 2 * (dense_pitch(rows) - row0) : 0);
         }
     }
     // Load c of stage k to `lds`, this operand's region.
@@ -76,18 +76,14 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_dma(DenseArg
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wid / Tile::WN, wn = wid % Tile::WN;
-    const int64_t t = gemm_tile_of_block(blockIdx.x, sh.blocks, 8);
-    const int split = sh.splits > 1 ? static_cast<int>(t % sh.splits) : 0;
-    const TilePos pos = tile_pos(sh.splits > 1 ? t / sh.splits : t, sh.tiles_m, sh.tiles_n, 4);
+    const uint32_t lds0 = wide_lds_addr(lds);
+    dense_each(sh, [&](int64_t tile, int k0, int k1, int slot) {
+    const TilePos pos = tile_pos(tile, sh.tiles_m, sh.tiles_n, 4);
     const int64_t m0 = pos.tm * Tile::BM, n0 = pos.tn * Tile::BN;
-    const int ks = static_cast<int>((a.K + 63) / 64);
-    const int k0 = split * sh.per, k1 = k0 + sh.per < ks ? k0 + sh.per : ks;
-
     const DenseFetch<AX, Tile::BM, Tile::WAVES> fa(a.A, a.lda, m0, a.M, a.K, wid);
     const DenseFetch<BX, Tile::BN, Tile::WAVES> fb(a.B, a.ldb, n0, a.N, a.K, wid);
     constexpr int NA = fa.N, LOADS = fa.N + fb.N;                  // loads of a wave: A's, of a stage
     static_assert((NS - 1) * LOADS < 64, "vmcnt field");
-    const uint32_t lds0 = wide_lds_addr(lds);
     // Load c of stage k, whose ranges are da and db, into the memory of stage s.
     auto load = [&](v4u da, v4u db, int k, int s, int c) {
         if (c < NA) fa.load(da, k, lds0 + s * Tile::STAGE, wid, c);
@@ -150,15 +146,8 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_dma(DenseArg
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // the empty loads past the last stage
     __syncthreads();
-    float* strip = reinterpret_cast<float*>(lds) + wid * Tile::STRIP;
-    const int64_t mw = m0 + arow, nw = n0 + brow;
-    if (sh.splits > 1) {
-        const DenseArgs p{nullptr, nullptr, 0, 0, a.M, a.N, a.K, nullptr, nullptr, 0, NFLOW_ACT_NONE,
-                          sh.part + split * a.M * a.N, a.N, nullptr, 0};
-        dense_store<float, Tile>(p, acc, strip, mw, nw);
-    } else {
-        dense_store<bf16, Tile>(a, acc, strip, mw, nw);
-    }
+    dense_leave<bf16, Tile>(a, sh, acc, reinterpret_cast<float*>(lds) + wid * Tile::STRIP, m0, n0, slot, wm, wn);
+    });
 }
 
 }  // namespace nfq

@@ -7,9 +7,13 @@
 // its pieces, and the workgroup joins them in LDS in the waves' order.  Rows need
 // no alignment.  Bound by reading the weight.
 #include "dense_kernel.h"
+#include "dense_split.h"
 
 namespace nfq {
 namespace {
+
+template <typename T>
+constexpr int dense_planes() { return std::is_same_v<T, float> ? 3 : 1; }
 
 // 32 k's of a row as operand planes.
 template <typename T>
@@ -57,39 +61,39 @@ __global__ __launch_bounds__(64 * W) void k_dense_few(DenseArgs a) {
 #pragma unroll
     for (int i = 0; i < RT; ++i)
         xrow[i] = static_cast<const T*>(a.A) + (16 * i + r < a.M ? 16 * i + r : 0) * a.lda;
+    // A piece of the weight and of the rows, AHEAD of the wave's pieces in flight.
+    constexpr int AHEAD = RT == 1 ? 4 : 2;
     struct Piece {
-        Raw8<T> v[H];
+        Raw8<T> w[H], x[RT][H];
     };
-    auto fetch = [&](const T* row, int k, Piece& o) {
+    auto fetch = [&](int k, Piece& o) {
+        if (k >= pieces) return;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             const int64_t c = static_cast<int64_t>(k) * KP + 32 * h + 8 * g;
-            if (k < pieces) o.v[h].load(row + c, a.K - c);
+            o.w[h].load(wrow + c, a.K - c);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) o.x[i][h].load(xrow[i] + c, a.K - c);
         }
     };
-    Piece wn[2];
-    fetch(wrow, wid, wn[0]);
-    fetch(wrow, wid + W, wn[1]);
-    auto step = [&](int k, const Piece& w) {
+    auto step = [&](const Piece& o) {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            const FewOperand<T> wp(w.v[h]);
+            const FewOperand<T> wp(o.w[h]);
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                Raw8<T> x;
-                const int64_t c = static_cast<int64_t>(k) * KP + 32 * h + 8 * g;
-                x.load(xrow[i] + c, a.K - c);
-                acc[i] = few_product<T>(wp, FewOperand<T>(x), acc[i]);
-            }
+            for (int i = 0; i < RT; ++i) acc[i] = few_product<T>(wp, FewOperand<T>(o.x[i][h]), acc[i]);
         }
     };
-    // Pieces in pairs, each asked for two of the wave's turns ahead.
-    for (int k = wid; k < pieces; k += 2 * W) {
-        step(k, wn[0]);
-        fetch(wrow, k + 2 * W, wn[0]);
-        if (k + W < pieces) {
-            step(k + W, wn[1]);
-            fetch(wrow, k + 3 * W, wn[1]);
+    Piece next[AHEAD];
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) fetch(wid + n * W, next[n]);
+    for (int k = wid; k < pieces; k += AHEAD * W) {
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) {
+            if (k + n * W < pieces) {
+                step(next[n]);
+                fetch(k + (n + AHEAD) * W, next[n]);
+            }
         }
     }
 #pragma unroll
@@ -118,8 +122,7 @@ void launch_rt(const DenseArgs& a, hipStream_t st) {
 template <typename T>
 void launch_dense_few(const DenseArgs& a, hipStream_t st) {
     if (a.M <= 16) launch_rt<T, 1>(a, st);
-    else if (a.M <= 32) launch_rt<T, 2>(a, st);
-    else launch_rt<T, 4>(a, st);
+    else launch_rt<T, 2>(a, st);
 }
 template void launch_dense_few<float>(const DenseArgs&, hipStream_t);
 template void launch_dense_few<bf16>(const DenseArgs&, hipStream_t);

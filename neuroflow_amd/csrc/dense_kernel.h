@@ -1,14 +1,11 @@
-// dense_kernel.h -- the tiled product of bf16 or fp32 operands on the matrix
-// cores.
+// dense_kernel.h -- what the tiled products of bf16 (dense_dma.h) and of fp32
+// operands (dense_f32.hip) on the matrix cores share.
 //
 //   z[m][n] = sum_k a[m][k] b[n][k] + bias[n] + r[m][n],   C = act(z)
 //
-// bf16 operands take v_mfma_f32_16x16x32_bf16: products exact, sums fp32.  An
-// fp32 operand is three bf16 planes, x = h + m + l: each plane is the rest
-// rounded to bf16's 8 bits, so 24 bits are held exactly, and six products (h h, h
-// m, m h, m m, h l, l h) leave out what is at most 2^-26 of the product: fp32
-// accuracy at a sixth of the bf16 rate, where the fp32 instruction has a
-// sixteenth.
+// Products are v_mfma_f32_16x16x32_bf16's: of bf16 values exact, sums fp32.  (The
+// 32 x 32 x 16 one has the higher rate on zeros and the lower one on data, where
+// power bounds the clock: 8192^3 in one run 863 us against 797.)
 //
 // An operand may lie along k or across it (the backward products read W, dz and
 // x where they are): the stage in LDS then has rows of k, and the operands come
@@ -25,38 +22,19 @@ namespace nfq {
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s* lds_v4s;
 
-template <typename T>
-constexpr int dense_planes() { return std::is_same_v<T, float> ? 3 : 1; }
-
-// Eight fp32 values as bf16 planes.  A value that would round to infinity keeps
-// a finite first plane; the planes of an infinity or a NaN are NaN past the first.
-__device__ __forceinline__ void dense_split(const float (&v)[8], v8bf (&p)[3]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float x = v[e];
-        const float top = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
-        const bf16 h = fabsf(x) < 0x1.ffp127f ? static_cast<bf16>(x) : static_cast<bf16>(top);
-        const float r = x - static_cast<float>(h);
-        const bf16 m = static_cast<bf16>(r);
-        p[0][e] = h;
-        p[1][e] = m;
-        p[2][e] = static_cast<bf16>(r - static_cast<float>(m));
-    }
-}
-
 // Tiles of BM x BN, WM x WN waves of TI x TJ 16 x 16 tiles each; a stage is KB
-// values of k of every row, NS stages.
+// values of k of every row in P planes, NS stages; OCC waves a SIMD.
 template <typename T, int WM_, int WN_, int TI_, int TJ_, int NS_, int OCC_ = 2>
 struct DenseTile {
     static constexpr int WM = WM_, WN = WN_, TI = TI_, TJ = TJ_, NS = NS_, OCC = OCC_;
-    static constexpr int P = dense_planes<T>();
-    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int P = std::is_same_v<T, float> ? 3 : 1, KB = std::is_same_v<T, float> ? 32 : 64;
+    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, PER_CU = 4 * OCC / WAVES;
     static constexpr int BM = 16 * TI * WM, BN = 16 * TJ * WN;
-    static constexpr int KB = std::is_same_v<T, float> ? 32 : 64;
     static constexpr int PLANE_A = BM * KB * 2, PLANE_B = BN * KB * 2;       // bytes
     static constexpr int STAGE = P * (PLANE_A + PLANE_B);
     static constexpr int STRIP_ROW = 16 * TJ + 4, STRIP = 16 * STRIP_ROW;   // floats of a wave's 16 rows on their way out
     static constexpr int LDS = NS * STAGE > WAVES * STRIP * 4 ? NS * STAGE : WAVES * STRIP * 4;
+    static_assert(PER_CU * LDS <= 160 * 1024, "a CU's LDS");
 };
 
 // Where 8 values lie in a plane: along k row `i` of the tile's R, group `c` of
@@ -97,51 +75,32 @@ __device__ __forceinline__ v8bf dense_fragment(const uint8_t* plane, int row0, i
     }
 }
 
-// An operand's share of a stage by way of registers: CH groups of 8 values a thread.
-template <typename T, bool ACROSS, int R, int KB, int THREADS>
-struct DenseStage {
-    static constexpr int CH = R * KB / 8 / THREADS;
-    static_assert(R * KB / 8 % THREADS == 0, "groups spread evenly");
-    static constexpr int PER = (ACROSS ? R : KB) / 8;              // groups of a row in memory
-    Raw8<T> v[CH];
-    // Rows row0 .. of `rows`, k's k0 .. of K.
-    __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t K) {
-        const bool inside = row0 + R <= rows && k0 + KB <= K;
-#pragma unroll
-        for (int q = 0; q < CH; ++q) {
-            const int id = threadIdx.x + THREADS * q, i = id / PER, c = 8 * (id % PER);
-            const int64_t major = (ACROSS ? k0 : row0) + i, minor = (ACROSS ? row0 : k0) + c;
-            const T* p = base + major * ld + minor;
-            if (inside) v[q].load(p, 8);
-            else v[q].load(p, major < (ACROSS ? K : rows) ? (ACROSS ? rows : K) - minor : 0);
-        }
-    }
-    __device__ __forceinline__ void store(uint8_t* planes) const {
-#pragma unroll
-        for (int q = 0; q < CH; ++q) {
-            const int id = threadIdx.x + THREADS * q;
-            uint8_t* to = planes + dense_place<ACROSS, R, KB>(id / PER, id % PER);
-            if constexpr (std::is_same_v<T, float>) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = v[q][e];
-                v8bf p[3];
-                dense_split(x, p);
-#pragma unroll
-                for (int s = 0; s < 3; ++s) *reinterpret_cast<v8bf*>(to + s * R * KB * 2) = p[s];
-            } else {
-                v8bf x;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = v[q].q[e];
-                *reinterpret_cast<v8bf*>(to) = x;
-            }
-        }
-    }
-};
-
 // Four outputs of a row from column n on: bias, residual, activation, one rounding.
 template <typename T>
 __device__ __forceinline__ void dense_finish(const DenseArgs& a, int64_t m, int64_t n, const v4f& s) {
+    typedef T v4t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (n + 3 < a.N) {
+        v4f z = s;
+        if (a.bias) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) z[v] += a.bias[n + v];
+        }
+        if (a.R) {
+            const v4t r = *reinterpret_cast<const v4t*>(static_cast<const T*>(a.R) + m * a.ldr + n);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) z[v] += to_f32(r[v]);
+        }
+        v4t y;
+        if (a.Z) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) y[v] = from_f32<T>(z[v]);
+            *reinterpret_cast<v4t*>(static_cast<T*>(a.Z) + m * a.ldz + n) = y;
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) y[v] = from_f32<T>(activate_rt(z[v], a.act));
+        *reinterpret_cast<v4t*>(static_cast<T*>(a.C) + m * a.ldc + n) = y;
+        return;
+    }
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
         if (n + v >= a.N) return;
@@ -153,14 +112,15 @@ __device__ __forceinline__ void dense_finish(const DenseArgs& a, int64_t m, int6
 }
 
 // V values at p, together where the row allows it.
-template <typename T, int V>
+template <typename T, bool STREAM, int V>
 __device__ __forceinline__ void dense_put(T* p, const float (&y)[V], bool vec, int64_t left) {
     if (vec) {
         typedef T vt __attribute__((ext_vector_type(V)));
         vt o;
 #pragma unroll
         for (int v = 0; v < V; ++v) o[v] = from_f32<T>(y[v]);
-        __builtin_nontemporal_store(o, reinterpret_cast<vt*>(p));
+        if constexpr (STREAM) __builtin_nontemporal_store(o, reinterpret_cast<vt*>(p));
+        else *reinterpret_cast<vt*>(p) = o;
     } else {
 #pragma unroll
         for (int v = 0; v < V; ++v)
@@ -170,7 +130,8 @@ __device__ __forceinline__ void dense_put(T* p, const float (&y)[V], bool vec, i
 
 // A wave's TI x TJ tiles of sums to rows m0 .., columns n0 .. of C, through its
 // strip of LDS, so that loads and stores are whole lines.
-template <typename T, typename Tile>
+// STREAM: non-temporal stores, of results; what the next launch reads stays in the caches.
+template <typename T, typename Tile, bool STREAM>
 __device__ __forceinline__ void dense_store(const DenseArgs& a, const v4f (&acc)[Tile::TI][Tile::TJ], float* strip,
                                             int64_t m0, int64_t n0) {
     constexpr int V = 16 / sizeof(T), LPR = 16 * Tile::TJ / V, RPI = 64 / LPR;   // values a lane, lanes a row, rows a store
@@ -214,7 +175,7 @@ __device__ __forceinline__ void dense_store(const DenseArgs& a, const v4f (&acc)
                     for (int v = 0; v < V; ++v) y[v] += v < left ? to_f32(rr[v]) : 0.0f;
                 }
             }
-            if (a.Z) dense_put<T, V>(static_cast<T*>(a.Z) + m * a.ldz + n, y, vecz, left);
+            if (a.Z) dense_put<T, STREAM, V>(static_cast<T*>(a.Z) + m * a.ldz + n, y, vecz, left);
             if (a.act == NFLOW_ACT_RELU) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) y[v] = activate<ACT_RELU>(y[v]);
@@ -222,7 +183,7 @@ __device__ __forceinline__ void dense_store(const DenseArgs& a, const v4f (&acc)
 #pragma unroll
                 for (int v = 0; v < V; ++v) y[v] = activate<ACT_GELU_TANH>(y[v]);
             }
-            dense_put<T, V>(static_cast<T*>(a.C) + m * a.ldc + n, y, vec, left);
+            dense_put<T, STREAM, V>(static_cast<T*>(a.C) + m * a.ldc + n, y, vec, left);
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -230,123 +191,104 @@ __device__ __forceinline__ void dense_store(const DenseArgs& a, const v4f (&acc)
     }
 }
 
+// ---- how a product is dealt out -------------------------------------------------------
+// Workgroup i computes whole tiles i, i + groups, ... (`whole` of them), and where
+// tiles are left, `rest` of them, their K steps are dealt out evenly: it takes
+// steps [i, i + 1) rest ksteps / groups of those tiles one after another, which
+// reach into at most two.  A part of a tile leaves its fp32 sums in a slot (two a
+// workgroup, BM x BN each), and a second launch joins a tile's slots in the
+// workgroups' order.
 struct DenseShare {
     int64_t tiles_m, tiles_n;
-    int splits, per;    // runs of `per` stages of K
-    float* part;        // (splits, M, N) sums, where splits > 1
-    int blocks;
+    int groups, whole, rest, ksteps;
+    float* part;
+    __host__ __device__ int64_t step_of(int i) const { return static_cast<int64_t>(i) * rest * ksteps / groups; }
 };
 
-// One stage's products: every 32 k's, the planes' products of the least first.
-template <typename T, bool AX, bool BX, typename Tile>
-__device__ __forceinline__ void dense_step(const uint8_t* st, v4f (&acc)[Tile::TI][Tile::TJ], int arow, int brow) {
-    constexpr int P = Tile::P, TI = Tile::TI, TJ = Tile::TJ, KB = Tile::KB;
-    const uint8_t* sb = st + P * Tile::PLANE_A;
-#pragma unroll
-    for (int k = 0; k < KB; k += 32) {
-        v8bf bf[P][TJ];
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-#pragma unroll
-            for (int j = 0; j < TJ; ++j)
-                bf[p][j] = dense_fragment<BX, Tile::BN, KB>(sb + p * Tile::PLANE_B, brow + 16 * j, k);
-#pragma unroll
-        for (int i = 0; i < TI; ++i) {
-            v8bf af[P];
-#pragma unroll
-            for (int p = 0; p < P; ++p) af[p] = dense_fragment<AX, Tile::BM, KB>(st + p * Tile::PLANE_A, arow + 16 * i, k);
-            if constexpr (P == 1) {
-#pragma unroll
-                for (int j = 0; j < TJ; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[0][j], af[0], acc[i][j], 0, 0, 0);
-            } else {
-                constexpr int pa[6] = {0, 2, 1, 0, 1, 0}, pb[6] = {2, 0, 1, 1, 0, 0};
-#pragma unroll
-                for (int q = 0; q < 6; ++q)
-#pragma unroll
-                    for (int j = 0; j < TJ; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[pb[q]][j], af[pa[q]], acc[i][j], 0, 0, 0);
-            }
+// Calls f(tile, first step, end, slot or -1) for the work of this workgroup, all
+// waves of it together at each call's start.  Neighbouring workgroups are on one
+// XCD (gemm_tile_of_block).
+template <typename F>
+__device__ __forceinline__ void dense_each(const DenseShare& sh, F f) {
+    const int i = gemm_tile_of_block(blockIdx.x, sh.groups, 8);
+    int64_t at = sh.rest ? sh.step_of(i) : 0;
+    const int64_t end = sh.rest ? sh.step_of(i + 1) : 0;
+    for (int n = 0; n < sh.whole || at < end; ++n) {
+        int64_t tile = static_cast<int64_t>(n) * sh.groups + i;
+        int k = 0, stop = sh.ksteps, slot = -1;
+        if (n >= sh.whole) {
+            const int64_t t = at / sh.ksteps;
+            k = static_cast<int>(at - t * sh.ksteps);
+            if (k + end - at < stop) stop = static_cast<int>(k + end - at);
+            tile = static_cast<int64_t>(sh.whole) * sh.groups + t;
+            if (k > 0 || stop < sh.ksteps) slot = 2 * i + n - sh.whole;
+            at += stop - k;
         }
+        if (n) __syncthreads();
+        f(tile, k, stop, slot);
     }
 }
 
-template <typename T, bool AX, bool BX, typename Tile>
-__global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense(DenseArgs a, DenseShare sh) {
-    constexpr int TI = Tile::TI, TJ = Tile::TJ, KB = Tile::KB;
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wid / Tile::WN, wn = wid % Tile::WN;
-    const int64_t t = gemm_tile_of_block(blockIdx.x, sh.blocks, 8);
-    const int split = sh.splits > 1 ? static_cast<int>(t % sh.splits) : 0;
-    const TilePos pos = tile_pos(sh.splits > 1 ? t / sh.splits : t, sh.tiles_m, sh.tiles_n, 4);
-    const int64_t m0 = pos.tm * Tile::BM, n0 = pos.tn * Tile::BN;
-    const int ks = static_cast<int>((a.K + KB - 1) / KB);
-    const int k0 = split * sh.per, k1 = k0 + sh.per < ks ? k0 + sh.per : ks;
-
-    v4f acc[TI][TJ];
-#pragma unroll
-    for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    DenseStage<T, AX, Tile::BM, KB, Tile::THREADS> ra;
-    DenseStage<T, BX, Tile::BN, KB, Tile::THREADS> rb;
-    auto load = [&](int k) {
-        ra.load(static_cast<const T*>(a.A), a.lda, m0, a.M, static_cast<int64_t>(k) * KB, a.K);
-        rb.load(static_cast<const T*>(a.B), a.ldb, n0, a.N, static_cast<int64_t>(k) * KB, a.K);
-    };
-    if (k0 < k1) load(k0);
-    for (int k = k0; k < k1; ++k) {
-        __syncthreads();                             // the stage's last readers are done
-        ra.store(lds);
-        rb.store(lds + Tile::P * Tile::PLANE_A);
-        __syncthreads();
-        if (k + 1 < k1) load(k + 1);
-        dense_step<T, AX, BX, Tile>(lds, acc, 16 * TI * wm, 16 * TJ * wn);
-    }
-    __syncthreads();
-    float* strip = reinterpret_cast<float*>(lds) + wid * Tile::STRIP;
-    const int64_t mw = m0 + 16 * TI * wm, nw = n0 + 16 * TJ * wn;
-    if (sh.splits > 1) {
-        const DenseArgs p{nullptr, nullptr, 0, 0, a.M, a.N, a.K, nullptr, nullptr, 0, NFLOW_ACT_NONE,
-                          sh.part + split * a.M * a.N, a.N, nullptr, 0};
-        dense_store<float, Tile>(p, acc, strip, mw, nw);
+// What becomes of a wave's sums: the results, or a slot's.
+template <typename T, typename Tile>
+__device__ __forceinline__ void dense_leave(const DenseArgs& a, const DenseShare& sh, const v4f (&acc)[Tile::TI][Tile::TJ],
+                                            float* strip, int64_t m0, int64_t n0, int slot, int wm, int wn) {
+    const int i = 16 * Tile::TI * wm, j = 16 * Tile::TJ * wn;
+    if (slot >= 0) {
+        const DenseArgs p{nullptr, nullptr, 0, 0, Tile::BM, Tile::BN, 0, nullptr, nullptr, 0, NFLOW_ACT_NONE,
+                          sh.part + static_cast<int64_t>(slot) * Tile::BM * Tile::BN, Tile::BN, nullptr, 0};
+        dense_store<float, Tile, false>(p, acc, strip, i, j);
     } else {
-        dense_store<T, Tile>(a, acc, strip, mw, nw);
+        dense_store<T, Tile, true>(a, acc, strip, m0 + i, n0 + j);
     }
 }
 
-// Sum of the splits' partial results, in their order, and the epilogue.
-template <typename T>
-__global__ __launch_bounds__(256) void k_dense_join(DenseArgs a, const float* __restrict__ part, int splits) {
-    const int64_t n4 = (a.N + 3) / 4, total = a.M * n4;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t m = i / n4, n = (i - m * n4) * 4;
-        v4f z{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < splits; ++s) {
-            const float* p = part + (s * a.M + m) * a.N + n;
+// The shared tiles' sums, over their slots in order, and the epilogue: a
+// workgroup for 16 rows of a tile.
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(256) void k_dense_join(DenseArgs a, DenseShare sh) {
+    const int t = blockIdx.x / (BM / 16), row0 = 16 * (blockIdx.x % (BM / 16));
+    const int64_t first = static_cast<int64_t>(t) * sh.ksteps, last = first + sh.ksteps;
+    int i = static_cast<int>(first * sh.groups / (static_cast<int64_t>(sh.rest) * sh.ksteps));   // may be one too low
+    while (sh.step_of(i + 1) <= first) ++i;
+    if (sh.step_of(i) <= first && sh.step_of(i + 1) >= last) return;         // one workgroup's: stored
+    const TilePos pos = tile_pos(static_cast<int64_t>(sh.whole) * sh.groups + t, sh.tiles_m, sh.tiles_n, 4);
+    const int64_t m0 = pos.tm * BM + row0, n0 = pos.tn * BN;
+    constexpr int Q = 16 * BN / 4 / 256;                                     // groups of four values a thread
+    v4f z[Q];
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-                if (n + v < a.N) z[v] += p[v];
-        }
-        dense_finish<T>(a, m, n, z);
+    for (int q = 0; q < Q; ++q) z[q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (; sh.step_of(i) < last; ++i) {
+        const int n = sh.step_of(i) / sh.ksteps < t ? 1 : 0;                 // its second part, if it began in the tile before
+        const float* p = sh.part + static_cast<int64_t>(2 * i + n) * BM * BN + row0 * BN;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) z[q] += *reinterpret_cast<const v4f*>(p + 4 * (threadIdx.x + 256 * q));
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int e = 4 * (threadIdx.x + 256 * q);
+        if (m0 + e / BN < a.M) dense_finish<T>(a, m0 + e / BN, n0 + e % BN, z[q]);
     }
 }
 
-// `kernel` over the tiles of the product and its splits, and their join.
+// `kernel` over a product as the plan has it, and the join of what is shared.
 template <typename T, typename Tile, auto kernel>
-void launch_dense_tile(const DenseArgs& a, int splits, float* part, hipStream_t st) {
+void launch_dense_tile(const DenseArgs& a, const DensePlan& p, float* part, hipStream_t st) {
     static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, Tile::LDS);
     (void)once;
-    const int64_t tm = (a.M + Tile::BM - 1) / Tile::BM, tn = (a.N + Tile::BN - 1) / Tile::BN;
+    const int64_t tm = (a.M + Tile::BM - 1) / Tile::BM, tn = (a.N + Tile::BN - 1) / Tile::BN, tiles = tm * tn;
     const int ks = static_cast<int>((a.K + Tile::KB - 1) / Tile::KB);
-    const DenseShare sh{tm, tn, splits, (ks + splits - 1) / splits, part, static_cast<int>(tm * tn * splits)};
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(sh.blocks)), dim3(Tile::THREADS), Tile::LDS, st, a, sh);
-    if (splits > 1)
-        hipLaunchKernelGGL((k_dense_join<T>), dim3(grid_for(a.M * ((a.N + 3) / 4), 256, 8)), dim3(256), 0, st, a, part,
-                           splits);
+    DenseShare sh{tm, tn, static_cast<int>(tiles), 1, 0, ks, part};
+    if (p.groups) {
+        sh.groups = p.groups;
+        sh.whole = static_cast<int>(tiles / p.groups);
+        sh.rest = static_cast<int>(tiles % p.groups);
+    }
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(sh.groups)), dim3(Tile::THREADS), Tile::LDS, st, a, sh);
+    if (sh.rest)
+        hipLaunchKernelGGL((k_dense_join<T, Tile::BM, Tile::BN>), dim3(static_cast<unsigned>(sh.rest * (Tile::BM / 16))),
+                           dim3(256), 0, st, a, sh);
 }
 
 }  // namespace nfq

@@ -32,21 +32,26 @@ struct GradTable {
 };
 static_assert(sizeof(GradTable) + 64 <= 4096, "a kernel's arguments");
 
-// Calls f(tensor, its chunk) for the chunks of this workgroup, in their order.
-template <typename F>
-__device__ __forceinline__ void each_chunk(const GradTable& t, int block, F f) {
-    int c = block * t.per;
-    const int end = c + t.per < t.chunks ? c + t.per : t.chunks;
-    if (c >= end) return;
-    int lo = 0, hi = t.tensors - 1;                 // the last tensor with first <= c: none there is empty
-    while (lo < hi) {
+// Calls f(tensor, its chunk) for the chunks of this workgroup, first to last or,
+// with BACK, last to first.
+template <bool BACK, typename F>
+__device__ __forceinline__ void each_chunk(const GradTable& t, F f) {
+    const int begin = blockIdx.x * t.per, end = begin + t.per < t.chunks ? begin + t.per : t.chunks;
+    if (begin >= end) return;
+    int c = BACK ? end - 1 : begin, lo = 0, hi = t.tensors - 1;
+    while (lo < hi) {                               // the last tensor with first <= c: none in the table is empty
         const int mid = (lo + hi + 1) / 2;
         if (t.first[mid] <= c) lo = mid;
         else hi = mid - 1;
     }
-    for (int i = lo; c < end; ++i) {
-        const int next = i + 1 < t.tensors ? t.first[i + 1] : t.chunks, stop = next < end ? next : end;
-        for (; c < stop; ++c) f(i, c - t.first[i]);
+    if constexpr (BACK) {
+        for (int i = lo; c >= begin; --i)
+            for (; c >= begin && c >= t.first[i]; --c) f(i, c - t.first[i]);
+    } else {
+        for (int i = lo; c < end; ++i) {
+            const int next = i + 1 < t.tensors ? t.first[i + 1] : t.chunks, stop = next < end ? next : end;
+            for (; c < stop; ++c) f(i, c - t.first[i]);
+        }
     }
 }
 
@@ -84,7 +89,7 @@ __device__ __forceinline__ double chunk_squares(const T* g, int64_t count, int64
 __global__ __launch_bounds__(kThreads) void k_grad_squares(GradTable t, double* __restrict__ part) {
     __shared__ double red[kThreads / 64];
     double s = 0.0;
-    each_chunk(t, blockIdx.x, [&](int i, int c) {
+    each_chunk<false>(t, [&](int i, int c) {
         const int64_t n = t.count[i], at = c * kChunk;
         s += n < 0 ? chunk_squares(static_cast<const bf16*>(t.grad[i]), -n, at)
                    : chunk_squares(static_cast<const float*>(t.grad[i]), n, at);
@@ -107,46 +112,62 @@ __global__ __launch_bounds__(kThreads) void k_grad_norm(const double* __restrict
     if (threadIdx.x == 0) *norm = static_cast<float>(n);
 }
 
+// Where a chunk's values are, and how many of them this thread's loads k reach.
 template <typename T>
-__device__ __forceinline__ void chunk_scale(const T* g, T* o, int64_t count, int64_t at, float f) {
+struct ChunkScale {
     Raw8<T> v[kVecs];
+    __device__ __forceinline__ void load(const void* g, int64_t count, int64_t at) {
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-        const int64_t c = at + 8 * (static_cast<int64_t>(threadIdx.x) + kThreads * k);
-        v[k].load(g + c, count - c);
+        for (int k = 0; k < kVecs; ++k) {
+            const int64_t c = at + 8 * (static_cast<int64_t>(threadIdx.x) + kThreads * k);
+            v[k].load(static_cast<const T*>(g) + c, count - c);
+        }
     }
+    __device__ __forceinline__ void store(void* o, int64_t count, int64_t at, float f) const {
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-        const int64_t c = at + 8 * (static_cast<int64_t>(threadIdx.x) + kThreads * k);
-        float y[8];
+        for (int k = 0; k < kVecs; ++k) {
+            const int64_t c = at + 8 * (static_cast<int64_t>(threadIdx.x) + kThreads * k);
+            float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = v[k][e] * f;
-        store8(o + c, count - c, y);
+            for (int e = 0; e < 8; ++e) y[e] = v[k][e] * f;
+            store8(static_cast<T*>(o) + c, count - c, y);
+        }
     }
-}
+};
 
+// A workgroup's last chunks first: what the first launch read last is still in
+// the Infinity Cache.  The first chunk's values are asked for ahead of the norm.
 __global__ __launch_bounds__(kThreads) void k_grad_scale(GradTable t, const double* __restrict__ part, int parts,
                                                          float max_norm, float* __restrict__ norm) {
     __shared__ double red[kThreads / 64];
-    const double n = total_norm(part, parts, red);
-    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
-    // A norm that is NaN is not below: the factor is NaN then, and 0 of an infinite one.
-    const bool keep = n <= static_cast<double>(max_norm);
-    const float f = keep ? 1.0f : static_cast<float>(static_cast<double>(max_norm) / n);
-    each_chunk(t, blockIdx.x, [&](int i, int c) {
-        const int64_t k = t.count[i], at = c * kChunk;
-        if (keep && t.out[i] == t.grad[i]) return;
-        if (k < 0) chunk_scale(static_cast<const bf16*>(t.grad[i]), static_cast<bf16*>(t.out[i]), -k, at, f);
-        else chunk_scale(static_cast<const float*>(t.grad[i]), static_cast<float*>(t.out[i]), k, at, f);
+    float f = 0.0f;
+    bool known = false, keep = false;
+    auto factor = [&] {
+        if (known) return;
+        known = true;
+        const double n = total_norm(part, parts, red);
+        if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
+        // A norm that is NaN is not below: the factor is NaN then, and 0 of an infinite one.
+        keep = n <= static_cast<double>(max_norm);
+        f = keep ? 1.0f : static_cast<float>(static_cast<double>(max_norm) / n);
+    };
+    each_chunk<true>(t, [&](int i, int c) {
+        const int64_t n = t.count[i], at = c * kChunk;
+        const bool here = t.out[i] == t.grad[i];
+        if (known && keep && here) return;
+        if (n < 0) {
+            ChunkScale<bf16> v;
+            v.load(t.grad[i], -n, at);
+            factor();
+            if (!(keep && here)) v.store(t.out[i], -n, at, f);
+        } else {
+            ChunkScale<float> v;
+            v.load(t.grad[i], n, at);
+            factor();
+            if (!(keep && here)) v.store(t.out[i], n, at, f);
+        }
     });
 }
-
-// The tensors with elements, kTable of them a launch.
-struct GradPlan {
-    std::vector<GradTable> tables;
-    std::vector<int> parts;                         // workgroups of each table's first launch
-    int total = 0;                                  // of all
-};
 
 int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
 
@@ -191,19 +212,11 @@ bool tangled(const nflow_grad_tensor* tensors, int count) {
     return false;
 }
 
-void seal(GradTable& t, GradPlan& p) {
-    const int blocks = std::min(t.chunks, kMaxParts);
-    t.per = (t.chunks + blocks - 1) / blocks;
-    p.parts.push_back((t.chunks + t.per - 1) / t.per);
-    p.total += p.parts.back();
-    p.tables.push_back(t);
-}
-
-GradPlan grad_plan(const nflow_grad_tensor* tensors, int count) {
-    GradPlan p;
-    GradTable t{};
-    for (int i = 0; i < count; ++i) {
-        const nflow_grad_tensor& g = tensors[i];
+// The next kTable tensors with elements, from `next` on; false when there are none.
+bool fill(GradTable& t, const nflow_grad_tensor* tensors, int count, int& next) {
+    t.tensors = t.chunks = 0;
+    for (; next < count && t.tensors < kTable; ++next) {
+        const nflow_grad_tensor& g = tensors[next];
         if (g.count == 0) continue;
         const int k = t.tensors++;
         t.grad[k] = g.grad;
@@ -211,31 +224,24 @@ GradPlan grad_plan(const nflow_grad_tensor* tensors, int count) {
         t.count[k] = g.dtype == NFLOW_DTYPE_BF16 ? -g.count : g.count;
         t.first[k] = t.chunks;
         t.chunks += static_cast<int>(chunks_of(g.count));
-        if (t.tensors == kTable) {
-            seal(t, p);
-            t = GradTable{};
-        }
     }
-    if (t.tensors) seal(t, p);
-    return p;
+    if (t.tensors == 0) return false;
+    const int blocks = std::min(t.chunks, kMaxParts);
+    t.per = (t.chunks + blocks - 1) / blocks;
+    return true;
 }
+int blocks_of(const GradTable& t) { return (t.chunks + t.per - 1) / t.per; }
 
-size_t grad_space_of(const GradPlan& p) { return round16(static_cast<size_t>(p.total) * sizeof(double)); }
+size_t grad_space(int count) { return static_cast<size_t>((count + kTable - 1) / kTable) * kMaxParts * sizeof(double); }
 
-void launch_squares(const GradPlan& p, double* part, hipStream_t st) {
-    for (size_t i = 0; i < p.tables.size(); ++i) {
-        hipLaunchKernelGGL(k_grad_squares, dim3(p.parts[i]), dim3(kThreads), 0, st, p.tables[i], part);
-        part += p.parts[i];
+// The launches of the norm; the partial sums' number, and the last table in t.
+int launch_squares(const nflow_grad_tensor* tensors, int count, double* part, GradTable& t, hipStream_t st) {
+    int parts = 0;
+    for (int next = 0; next < count && fill(t, tensors, count, next);) {
+        hipLaunchKernelGGL(k_grad_squares, dim3(blocks_of(t)), dim3(kThreads), 0, st, t, part + parts);
+        parts += blocks_of(t);
     }
-}
-
-template <typename F>
-int guarded(const char* what, F f) {
-    try {
-        return f();
-    } catch (const std::exception& e) {
-        return set_error(NFLOW_INTERNAL, std::string(what) + ": " + e.what());
-    }
+    return parts;
 }
 
 }  // namespace
@@ -245,16 +251,13 @@ using namespace nfq;
 
 extern "C" {
 
-int nflow_grad_workspace(const nflow_grad_tensor* tensors, int count, size_t* bytes) {
+int nflow_grad_workspace(int count, size_t* bytes) {
     clear_error();
-    const char* what = "grad_workspace";
-    if (!bytes) return bad_arg(what, "null output");
+    if (!bytes) return bad_arg("grad_workspace", "null output");
     *bytes = 0;
-    if (int rc = check_grads(what, tensors, count, false)) return rc;
-    return guarded(what, [&] {
-        *bytes = grad_space_of(grad_plan(tensors, count));
-        return static_cast<int>(NFLOW_OK);
-    });
+    if (count < 0) return bad_arg("grad_workspace", "bad count");
+    *bytes = grad_space(count);
+    return NFLOW_OK;
 }
 
 int nflow_grad_norm(const nflow_grad_tensor* tensors, int count, float* norm, void* workspace,
@@ -263,14 +266,12 @@ int nflow_grad_norm(const nflow_grad_tensor* tensors, int count, float* norm, vo
     const char* what = "grad_norm";
     if (int rc = check_grads(what, tensors, count, true)) return rc;
     if (!norm) return bad_arg(what, "null norm");
-    return guarded(what, [&] {
-        const GradPlan p = grad_plan(tensors, count);
-        if (int rc = check_workspace(what, workspace, workspace_bytes, grad_space_of(p))) return rc;
-        double* part = static_cast<double*>(workspace);
-        launch_squares(p, part, as_stream(stream));
-        hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(kThreads), 0, as_stream(stream), part, p.total, norm);
-        return launch_status(what);
-    });
+    if (int rc = check_workspace(what, workspace, workspace_bytes, grad_space(count))) return rc;
+    double* part = static_cast<double*>(workspace);
+    GradTable t;
+    const int parts = launch_squares(tensors, count, part, t, as_stream(stream));
+    hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(kThreads), 0, as_stream(stream), part, parts, norm);
+    return launch_status(what);
 }
 
 int nflow_grad_clip(const nflow_grad_tensor* tensors, int count, float max_norm, float* norm, void* workspace,
@@ -282,20 +283,23 @@ int nflow_grad_clip(const nflow_grad_tensor* tensors, int count, float max_norm,
     if (!(max_norm >= 0.0f)) return bad_arg(what, "max_norm must not be negative or NaN");
     for (int i = 0; i < count; ++i)
         if (tensors[i].count > 0 && !tensors[i].out) return bad_arg(what, "null out");
-    return guarded(what, [&] {
+    if (int rc = check_workspace(what, workspace, workspace_bytes, grad_space(count))) return rc;
+    try {
         if (tangled(tensors, count)) return bad_arg(what, "an out overlaps a gradient or another out");
-        const GradPlan p = grad_plan(tensors, count);
-        if (int rc = check_workspace(what, workspace, workspace_bytes, grad_space_of(p))) return rc;
-        double* part = static_cast<double*>(workspace);
-        hipStream_t st = as_stream(stream);
-        launch_squares(p, part, st);
-        if (p.tables.empty())
-            hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(kThreads), 0, st, part, 0, norm);
-        for (size_t i = 0; i < p.tables.size(); ++i)
-            hipLaunchKernelGGL(k_grad_scale, dim3(p.parts[i]), dim3(kThreads), 0, st, p.tables[i], part, p.total, max_norm,
-                               i == 0 ? norm : nullptr);
-        return launch_status(what);
-    });
+    } catch (const std::exception& e) {
+        return set_error(NFLOW_INTERNAL, std::string(what) + ": " + e.what());
+    }
+    double* part = static_cast<double*>(workspace);
+    hipStream_t st = as_stream(stream);
+    GradTable t;
+    const int parts = launch_squares(tensors, count, part, t, st);
+    if (parts == 0) hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(kThreads), 0, st, part, 0, norm);
+    // The norm goes out with one table's launch; t still holds the only table of a few tensors.
+    bool first = true;
+    for (int next = 0; parts > 0 && (count <= kTable ? first : next < count && fill(t, tensors, count, next)); first = false)
+        hipLaunchKernelGGL(k_grad_scale, dim3(blocks_of(t)), dim3(kThreads), 0, st, t, part, parts, max_norm,
+                           first ? norm : nullptr);
+    return launch_status(what);
 }
 
 }  // extern "C"
