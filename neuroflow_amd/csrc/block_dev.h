@@ -25,21 +25,6 @@ __device__ __forceinline__ float to_f32(bf16 v) { return static_cast<float>(v); 
 template <typename T>
 __device__ __forceinline__ T from_f32(float v) { return static_cast<T>(v); }   // bf16: nearest, ties to even
 
-// The first `left` < 8 elements at p and zeros: eight loads at once, those past
-// the last of the last (a load under each element's own condition waits for the
-// one before it, a few latencies in a row for the end of every odd row).
-template <typename T>
-__device__ __forceinline__ void load_some(const T* p, int64_t left, T (&v)[8]) {
-    const int n = static_cast<int>(left);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = T(0.0f);
-    if (n <= 0) return;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = p[e < n ? e : n - 1];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < n ? v[e] : T(0.0f);
-}
-
 // Eight consecutive elements at p as floats, of which the first `left` exist
 // (the rest are 0).  One or two 16-byte loads at any element alignment.
 template <typename T>
@@ -50,10 +35,8 @@ __device__ __forceinline__ void load8(const T* p, int64_t left, float (&v)[8]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = to_f32(q[e]);
     } else {
-        T q[8];
-        load_some(p, left, q);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = to_f32(q[e]);
+        for (int e = 0; e < 8; ++e) v[e] = e < left ? to_f32(p[e]) : 0.0f;
     }
 }
 
@@ -67,10 +50,8 @@ struct Raw8 {
         if (left >= 8) {
             q = *reinterpret_cast<const vec*>(p);
         } else {
-            T some[8];
-            load_some(p, left, some);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) q[e] = some[e];
+            for (int e = 0; e < 8; ++e) q[e] = e < left ? p[e] : T(0.0f);
         }
     }
     __device__ __forceinline__ float operator[](int e) const { return to_f32(q[e]); }

@@ -22,6 +22,7 @@ struct DenseArgs {
     int64_t ldc;
     void* Z;            // the sum ahead of the activation, or null
     int64_t ldz;
+    float* sums;        // of a(m, .) for every m, or null (of the dW form)
 };
 
 // Which operands lie across k: the layer's three products.
@@ -29,7 +30,7 @@ enum DenseForm { DENSE_FORWARD = 0, DENSE_DX = 1, DENSE_DW = 2 };
 
 // How a product is cut: the kernel or tile, and, unless 0, the workgroups that
 // the tiles and the K steps of what is left of them are dealt out to.
-enum DenseKind { DENSE_FEW, DENSE_SMALL, DENSE_MID, DENSE_DEEP, DENSE_BIG };
+enum DenseKind { DENSE_FEW, DENSE_SMALL, DENSE_TALL, DENSE_MID, DENSE_DEEP, DENSE_BIG };
 struct DensePlan {
     DenseKind kind;
     int groups;

@@ -48,22 +48,24 @@ __global__ __launch_bounds__(256) void k_dense_dz(DzArgs a) {
     const int64_t n = static_cast<int64_t>(blockIdx.x) * kDzCols + c, left = a.N - n;
     const int64_t m0 = blockIdx.y * a.rows_per, m1 = m0 + a.rows_per < a.M ? m0 + a.rows_per : a.M;
     float s[8] = {};
-    if (left > 0) {
+    auto run = [&](int64_t have) {
 #pragma unroll 4
         for (int64_t m = m0 + g; m < m1; m += kDzRows) {
             float d[8];
-            load8(static_cast<const T*>(a.dy) + m * a.lddy + n, left, d);
+            load8(static_cast<const T*>(a.dy) + m * a.lddy + n, have, d);
             if (a.act != NFLOW_ACT_NONE) {
                 float z[8];
-                load8(static_cast<const T*>(a.pre) + m * a.ldpre + n, left, z);
+                load8(static_cast<const T*>(a.pre) + m * a.ldpre + n, have, z);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) d[e] = act_grad(d[e], z[e], a.act);
-                store8(static_cast<T*>(a.dz) + m * a.lddz + n, left, d);
+                store8(static_cast<T*>(a.dz) + m * a.lddz + n, have, d);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[e] += d[e];
         }
-    }
+    };
+    if (left >= 8) run(8);                           // without the ends of rows in its loop: loads stay in flight
+    else if (left > 0) run(left);
     if (!a.part) return;
 #pragma unroll
     for (int e = 0; e < 8; e += 4) *reinterpret_cast<v4f*>(&join[g][c + e]) = v4f{s[e], s[e + 1], s[e + 2], s[e + 3]};
@@ -122,6 +124,7 @@ DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype)
         double alone, each, tile;
     };
     static const Cut of_bf16[] = {{DENSE_SMALL, 64, 64, 3, 0.233, 0.182, 0.7},
+                                  {DENSE_TALL, 128, 64, 2, 0.294, 0.273, 1.2},
                                   {DENSE_MID, 128, 128, 2, 0.613, 0.435, 2.4},
                                   {DENSE_DEEP, 128, 128, 1, 0.481, 0.476, 2.6},
                                   {DENSE_BIG, 256, 256, 1, 1.43, 1.50, 5.3}};
@@ -133,9 +136,9 @@ DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype)
     static const char* fk = getenv("DENSE_KIND");
     static const char* fs = getenv("DENSE_GROUPS");
     if (form == DENSE_FORWARD && M <= kDenseFewRows && (!fk || fk[0] == 'f')) return DensePlan{DENSE_FEW, 0, 0};
-    for (int i = 0; i < (f32 ? 3 : 4); ++i) {
+    for (int i = 0; i < (f32 ? 3 : 5); ++i) {
         const Cut& c = f32 ? of_f32[i] : of_bf16[i];
-        if (fk && fk[0] != (c.kind == DENSE_BIG ? 'b' : c.kind == DENSE_MID ? 'm' : c.kind == DENSE_DEEP ? 'd' : 's')) continue;
+        if (fk && fk[0] != (c.kind == DENSE_BIG ? 'b' : c.kind == DENSE_MID ? 'm' : c.kind == DENSE_DEEP ? 'd' : c.kind == DENSE_TALL ? 't' : 's')) continue;
         const double tiles = std::ceil(m / c.bm) * std::ceil(n / c.bn), per = std::ceil(tiles / cus);
         const double plain = steps * std::max(c.alone, per * c.each) + per * c.tile;
         if (plain < least && (!fs || atoi(fs) == 0)) {
@@ -152,7 +155,7 @@ DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype)
             const double time = share * std::max(c.alone, occ * c.each) + (t / groups + 2) * occ * c.tile + 3.0 + moved / 5e6;
             if (time < least) {
                 least = time;
-                best = DensePlan{c.kind, groups, static_cast<size_t>(2) * groups * c.bm * c.bn * sizeof(float)};
+                best = DensePlan{c.kind, groups, static_cast<size_t>(2) * groups * c.bm * (c.bn + 1) * sizeof(float)};
             }
         }
     }
@@ -293,7 +296,7 @@ int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t l
         return bad_arg(what, kShared);
     hipStream_t st = as_stream(stream);
     if (copies.n) launch_dense_pack(copies.m, st);
-    const DenseArgs a{px, pw, lx, lw, M, N, K, bias, residual, ldr, activation, y, ldy, pre, ldpre};
+    const DenseArgs a{px, pw, lx, lw, M, N, K, bias, residual, ldr, activation, y, ldy, pre, ldpre, nullptr};
     return product(what, DENSE_FORWARD, a, dtype, workspace, st);
 }
 
@@ -346,6 +349,9 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
     hipStream_t st = as_stream(stream);
     float* sums = reinterpret_cast<float*>(ws);
     const int64_t runs = dz_runs(M, N);
+    // With no activation dW's product sums dz's rows on its way; dz's own launch does else.
+    float* ride = !act && dW && K > 0 ? dbias : nullptr;
+    if (ride) dbias = nullptr;
     if (M > 0 && N > 0 && (act || dbias)) {
         const DzArgs a{dy, pre, dz, M, N, lddy, ldpre, lddz, activation, dbias ? sums : nullptr, (M + runs - 1) / runs};
         const dim3 grid(static_cast<unsigned>((N + kDzCols - 1) / kDzCols), static_cast<unsigned>(runs));
@@ -358,11 +364,11 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
     if (copies.n) launch_dense_pack(copies.m, st);
     if (int rc = launch_status(what)) return rc;
     if (dx && K > 0) {
-        const DenseArgs a{g, pw, lg, lw, M, K, N, nullptr, nullptr, 0, NFLOW_ACT_NONE, dx, lddx, nullptr, 0};
+        const DenseArgs a{g, pw, lg, lw, M, K, N, nullptr, nullptr, 0, NFLOW_ACT_NONE, dx, lddx, nullptr, 0, nullptr};
         if (int rc = product(what, DENSE_DX, a, dtype, ws + sp.sums, st)) return rc;
     }
     if (dW && K > 0) {
-        const DenseArgs a{g, px, lg, lx, N, K, M, nullptr, nullptr, 0, NFLOW_ACT_NONE, dW, lddw, nullptr, 0};
+        const DenseArgs a{g, px, lg, lx, N, K, M, nullptr, nullptr, 0, NFLOW_ACT_NONE, dW, lddw, nullptr, 0, ride};
         if (int rc = product(what, DENSE_DW, a, dtype, ws + sp.sums + sp.x, st)) return rc;
     }
     return NFLOW_OK;

@@ -7,12 +7,14 @@ namespace {
 
 using Small = DenseTile<bf16, 2, 2, 2, 2, 3, 3>;    // 64 x 64, four waves, three workgroups a CU
 using Mid = DenseTile<bf16, 2, 2, 4, 4, 2>;         // 128 x 128, four waves, two workgroups a CU
+using Tall = DenseTile<bf16, 2, 2, 4, 2, 3>;        // 128 x 64, four waves, two workgroups a CU
 using Deep = DenseTile<bf16, 2, 4, 4, 2, 4>;        // 128 x 128, eight waves, a workgroup a CU, loads three stages ahead
 using Big = DenseTile<bf16, 2, 4, 8, 4, 2>;         // 256 x 256, eight waves, a workgroup a CU
 
 template <bool AX, bool BX>
 void launch(const DenseArgs& a, const DensePlan& p, float* part, hipStream_t st) {
     if (p.kind == DENSE_BIG) launch_dense_tile<bf16, Big, &k_dense_dma<AX, BX, Big>>(a, p, part, st);
+    else if (p.kind == DENSE_TALL) launch_dense_tile<bf16, Tall, &k_dense_dma<AX, BX, Tall>>(a, p, part, st);
     else if (p.kind == DENSE_DEEP) launch_dense_tile<bf16, Deep, &k_dense_dma<AX, BX, Deep>>(a, p, part, st);
     else if (p.kind == DENSE_MID) launch_dense_tile<bf16, Mid, &k_dense_dma<AX, BX, Mid>>(a, p, part, st);
     else launch_dense_tile<bf16, Small, &k_dense_dma<AX, BX, Small>>(a, p, part, st);
@@ -35,7 +37,7 @@ __global__ __launch_bounds__(256) void k_dense_pack(PackArgs a) {
     bf16* to = static_cast<bf16*>(m.to) + row * pitch + c;
     Raw8<bf16> v[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r].load(from + r * m.ld, row + r < m.rows ? m.cols - c : 0);
+    for (int r = 0; r < 4; ++r) dense_load(v[r], from + r * m.ld, row + r < m.rows ? m.cols - c : 0);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
         if (row + r < m.rows) *reinterpret_cast<Raw8<bf16>::vec*>(to + r * pitch) = v[r].q;

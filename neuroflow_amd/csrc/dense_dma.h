@@ -96,6 +96,7 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_dma(DenseArg
 #pragma unroll
         for (int j = 0; j < TJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
+    DenseSums<Tile> sums(AX && a.sums && pos.tn == 0, wn);
     const int arow = 16 * TI * wm, brow = 16 * TJ * wn;
     v8bf xa[2][TI], xb[2][TJ];
     // Fragment e of half h of a stage: the TJ of B, then the TI of A, in the order of need.
@@ -107,6 +108,10 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_dma(DenseArg
 #pragma unroll
         for (int j = 0; j < TJ; ++j)
             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[h][j], xa[h][i], acc[i][j], 0, 0, 0);
+        if constexpr (AX) {
+            const v8bf one[1] = {xa[h][i]};
+            sums.add(i, one);
+        }
         __builtin_amdgcn_sched_barrier(0);
     };
     constexpr int F = TI + TJ, EACH = (F + TI - 1) / TI, LEACH = (LOADS + TI - 1) / TI;
@@ -145,6 +150,7 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_dma(DenseArg
         s = next;
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // the empty loads past the last stage
+    if constexpr (AX) sums.leave(a, sh, m0, slot, wm);
     __syncthreads();
     dense_leave<bf16, Tile>(a, sh, acc, reinterpret_cast<float*>(lds) + wid * Tile::STRIP, m0, n0, slot, wm, wn);
     });

@@ -28,7 +28,7 @@ struct DenseStage {
             const int64_t major = (ACROSS ? k0 : row0) + i, minor = (ACROSS ? row0 : k0) + c;
             const float* p = base + major * ld + minor;
             if (inside) v[q].load(p, 8);
-            else v[q].load(p, major < (ACROSS ? K : rows) ? (ACROSS ? rows : K) - minor : 0);
+            else dense_load(v[q], p, major < (ACROSS ? K : rows) ? (ACROSS ? rows : K) - minor : 0);
         }
     }
     __device__ __forceinline__ void store(uint8_t* planes) const {
@@ -59,7 +59,8 @@ struct StageProducts {
             for (int j = 0; j < Tile::TJ; ++j)
                 b[p][j] = dense_fragment<BX, Tile::BN, 32>(st + 3 * Tile::PLANE_A + p * Tile::PLANE_B, brow + 16 * j, 0);
     }
-    __device__ __forceinline__ void run(const uint8_t* st, v4f (&acc)[Tile::TI][Tile::TJ], int arow, int i0, int i1) const {
+    __device__ __forceinline__ void run(const uint8_t* st, v4f (&acc)[Tile::TI][Tile::TJ], DenseSums<Tile>& sums, int arow,
+                                        int i0, int i1) const {
 #pragma unroll
         for (int i = i0; i < i1; ++i) {
             v8bf a[3];
@@ -71,6 +72,7 @@ struct StageProducts {
 #pragma unroll
                 for (int j = 0; j < Tile::TJ; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[pb[q]][j], a[pa[q]], acc[i][j], 0, 0, 0);
+            if constexpr (AX) sums.add(i, a);
         }
     }
 };
@@ -104,6 +106,7 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_f32(DenseArg
             ra.store(lds + s * Tile::STAGE);
             rb.store(lds + s * Tile::STAGE + 3 * Tile::PLANE_A);
         };
+        DenseSums<Tile> sums(AX && a.sums && pos.tn == 0, wn);
         const int arow = 16 * TI * wm, brow = 16 * TJ * wn;
         load(k0);
         store(0);
@@ -118,14 +121,15 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_f32(DenseArg
                 store(s ^ 1);
                 load(k + 2);
             }
-            stage.run(st, acc, arow, 0, TI / 2);
+            stage.run(st, acc, sums, arow, 0, TI / 2);
             if (!first) {
                 store(s ^ 1);
                 load(k + 2);
             }
-            stage.run(st, acc, arow, TI / 2, TI);
+            stage.run(st, acc, sums, arow, TI / 2, TI);
             __syncthreads();
         }
+        if constexpr (AX) sums.leave(a, sh, m0, slot, wm);
         dense_leave<float, Tile>(a, sh, acc, reinterpret_cast<float*>(lds) + wid * Tile::STRIP, m0, n0, slot, wm, wn);
     });
 }

@@ -71,9 +71,9 @@ __global__ __launch_bounds__(64 * W) void k_dense_few(DenseArgs a) {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             const int64_t c = static_cast<int64_t>(k) * KP + 32 * h + 8 * g;
-            o.w[h].load(wrow + c, a.K - c);
+            dense_load(o.w[h], wrow + c, a.K - c);
 #pragma unroll
-            for (int i = 0; i < RT; ++i) o.x[i][h].load(xrow[i] + c, a.K - c);
+            for (int i = 0; i < RT; ++i) dense_load(o.x[i][h], xrow[i] + c, a.K - c);
         }
     };
     auto step = [&](const Piece& o) {

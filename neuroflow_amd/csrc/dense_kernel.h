@@ -111,11 +111,11 @@ __device__ __forceinline__ void dense_finish(const DenseArgs& a, int64_t m, int6
     }
 }
 
-// V values at p, together where the row allows it.
+// V values at p, together (at any element alignment) unless the row ends there.
 template <typename T, bool STREAM, int V>
-__device__ __forceinline__ void dense_put(T* p, const float (&y)[V], bool vec, int64_t left) {
-    if (vec) {
-        typedef T vt __attribute__((ext_vector_type(V)));
+__device__ __forceinline__ void dense_put(T* p, const float (&y)[V], int64_t left) {
+    if (left >= V) {
+        typedef T vt __attribute__((ext_vector_type(V), aligned(sizeof(T))));
         vt o;
 #pragma unroll
         for (int v = 0; v < V; ++v) o[v] = from_f32<T>(y[v]);
@@ -138,13 +138,28 @@ __device__ __forceinline__ void dense_store(const DenseArgs& a, const v4f (&acc)
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int row = lane / LPR, col = V * (lane % LPR);
     const int64_t n = n0 + col, left = a.N - n;
-    auto whole = [&](const void* p, int64_t ld) { return left >= V && ld % V == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-    const bool vec = whole(a.C, a.ldc), vecz = whole(a.Z, a.ldz), vecr = whole(a.R, a.ldr);
     float b[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) b[v] = a.bias && v < left ? a.bias[n + v] : 0.0f;
 #pragma unroll
     for (int i = 0; i < Tile::TI; ++i) {
+        // The residual's values first: they arrive under the strip's round trip.
+        typedef T vt __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+        vt res[16 / RPI];
+        if (a.R) {
+#pragma unroll
+            for (int q = 0; q < 16 / RPI; ++q) {
+                const int64_t m = m0 + 16 * i + RPI * q + row;
+                const T* p = static_cast<const T*>(a.R) + m * a.ldr + n;
+                if (m < a.M && left >= V) {
+                    res[q] = *reinterpret_cast<const vt*>(p);
+                } else {
+                    const int64_t have = m < a.M ? left : 0;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) res[q][v] = v < have ? p[v] : T(0.0f);
+                }
+            }
+        }
 #pragma unroll
         for (int j = 0; j < Tile::TJ; ++j)
             *reinterpret_cast<v4f*>(strip + r * Tile::STRIP_ROW + 16 * j + 4 * g) = acc[i][j];
@@ -162,20 +177,12 @@ __device__ __forceinline__ void dense_store(const DenseArgs& a, const v4f (&acc)
 #pragma unroll
                 for (int u = 0; u < 4; ++u) y[v + u] = z[u] + b[v + u];
             }
-            if (m >= a.M) continue;
             if (a.R) {
-                const T* rr = static_cast<const T*>(a.R) + m * a.ldr + n;
-                if (vecr) {
-                    typedef T vt __attribute__((ext_vector_type(V)));
-                    const vt x = *reinterpret_cast<const vt*>(rr);
 #pragma unroll
-                    for (int v = 0; v < V; ++v) y[v] += to_f32(x[v]);
-                } else {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) y[v] += v < left ? to_f32(rr[v]) : 0.0f;
-                }
+                for (int v = 0; v < V; ++v) y[v] += to_f32(res[q][v]);
             }
-            if (a.Z) dense_put<T, STREAM, V>(static_cast<T*>(a.Z) + m * a.ldz + n, y, vecz, left);
+            if (m >= a.M) continue;
+            if (a.Z) dense_put<T, STREAM, V>(static_cast<T*>(a.Z) + m * a.ldz + n, y, left);
             if (a.act == NFLOW_ACT_RELU) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) y[v] = activate<ACT_RELU>(y[v]);
@@ -183,12 +190,32 @@ __device__ __forceinline__ void dense_store(const DenseArgs& a, const v4f (&acc)
 #pragma unroll
                 for (int v = 0; v < V; ++v) y[v] = activate<ACT_GELU_TANH>(y[v]);
             }
-            dense_put<T, STREAM, V>(static_cast<T*>(a.C) + m * a.ldc + n, y, vec, left);
+            dense_put<T, STREAM, V>(static_cast<T*>(a.C) + m * a.ldc + n, y, left);
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
+}
+
+// Eight elements at p, of which the first `left` exist (the rest are 0).  At the
+// end of a row eight loads at once, those past the last of the last: under
+// conditions of their own each would wait for the one before it.
+template <typename T>
+__device__ __forceinline__ void dense_load(Raw8<T>& v, const T* p, int64_t left) {
+    if (left >= 8) {
+        v.load(p, 8);
+        return;
+    }
+    const int n = static_cast<int>(left);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v.q[e] = T(0.0f);
+    if (n <= 0) return;
+    T x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = p[e < n ? e : n - 1];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v.q[e] = e < n ? x[e] : T(0.0f);
 }
 
 // ---- how a product is dealt out -------------------------------------------------------
@@ -201,7 +228,7 @@ __device__ __forceinline__ void dense_store(const DenseArgs& a, const v4f (&acc)
 struct DenseShare {
     int64_t tiles_m, tiles_n;
     int groups, whole, rest, ksteps;
-    float* part;
+    float* part;        // 2 groups slots of BM x BN, then as many of BM: the sums of a's rows
     __host__ __device__ int64_t step_of(int i) const { return static_cast<int64_t>(i) * rest * ksteps / groups; }
 };
 
@@ -236,12 +263,47 @@ __device__ __forceinline__ void dense_leave(const DenseArgs& a, const DenseShare
     const int i = 16 * Tile::TI * wm, j = 16 * Tile::TJ * wn;
     if (slot >= 0) {
         const DenseArgs p{nullptr, nullptr, 0, 0, Tile::BM, Tile::BN, 0, nullptr, nullptr, 0, NFLOW_ACT_NONE,
-                          sh.part + static_cast<int64_t>(slot) * Tile::BM * Tile::BN, Tile::BN, nullptr, 0};
+                          sh.part + static_cast<int64_t>(slot) * Tile::BM * Tile::BN, Tile::BN, nullptr, 0, nullptr};
         dense_store<float, Tile, false>(p, acc, strip, i, j);
     } else {
         dense_store<T, Tile, true>(a, acc, strip, m0 + i, n0 + j);
     }
 }
+
+// The sums of a's rows ride along in the tiles of the first columns: a product
+// with ones for every row tile, the waves of a row of waves taking them in turn.
+template <typename Tile>
+struct DenseSums {
+    static constexpr int N = (Tile::TI + Tile::WN - 1) / Tile::WN;
+    v4f s[N];
+    int mine;           // the wave's column of waves, or one that no row tile has
+    __device__ __forceinline__ DenseSums(bool wanted, int wn) : mine(wanted ? wn : Tile::WN) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) s[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    template <int P>
+    __device__ __forceinline__ void add(int i, const v8bf (&a)[P]) {
+        if (i % Tile::WN != mine) return;
+        v8bf ones;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ones[e] = static_cast<bf16>(1.0f);
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p)
+            s[i / Tile::WN] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, a[p], s[i / Tile::WN], 0, 0, 0);
+    }
+    __device__ __forceinline__ void leave(const DenseArgs& a, const DenseShare& sh, int64_t m0, int slot, int wm) const {
+        const int r = threadIdx.x & 63;
+        if (mine == Tile::WN || r >= 16) return;
+        float* to = slot >= 0 ? sh.part + 2 * static_cast<int64_t>(sh.groups) * Tile::BM * Tile::BN +
+                                    static_cast<int64_t>(slot) * Tile::BM
+                              : a.sums + m0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = mine + n * Tile::WN, row = 16 * (Tile::TI * wm + i) + r;
+            if (i < Tile::TI && (slot >= 0 || m0 + row < a.M)) to[row] = s[n][0];
+        }
+    }
+};
 
 // The shared tiles' sums, over their slots in order, and the epilogue: a
 // workgroup for 16 rows of a tile.
@@ -258,8 +320,11 @@ __global__ __launch_bounds__(256) void k_dense_join(DenseArgs a, DenseShare sh) 
     v4f z[Q];
 #pragma unroll
     for (int q = 0; q < Q; ++q) z[q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const bool sums = a.sums && pos.tn == 0 && threadIdx.x < 16;
+    float s = 0.0f;
     for (; sh.step_of(i) < last; ++i) {
         const int n = sh.step_of(i) / sh.ksteps < t ? 1 : 0;                 // its second part, if it began in the tile before
+        if (sums) s += sh.part[(2 * static_cast<int64_t>(sh.groups) * BN + 2 * i + n) * BM + row0 + threadIdx.x];
         const float* p = sh.part + static_cast<int64_t>(2 * i + n) * BM * BN + row0 * BN;
 #pragma unroll
         for (int q = 0; q < Q; ++q) z[q] += *reinterpret_cast<const v4f*>(p + 4 * (threadIdx.x + 256 * q));
@@ -269,6 +334,7 @@ __global__ __launch_bounds__(256) void k_dense_join(DenseArgs a, DenseShare sh) 
         const int e = 4 * (threadIdx.x + 256 * q);
         if (m0 + e / BN < a.M) dense_finish<T>(a, m0 + e / BN, n0 + e % BN, z[q]);
     }
+    if (sums && m0 + threadIdx.x < a.M) a.sums[m0 + threadIdx.x] = s;
 }
 
 // `kernel` over a product as the plan has it, and the join of what is shared.
