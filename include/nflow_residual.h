@@ -126,10 +126,13 @@ int nflow_grad_workspace(int count, size_t* bytes);
 
 /* ---- for tests: which kernel a size takes (no GPU needed: 256 CUs without one) ---- */
 
-/* The tile edge of the linear layer's product at this size, or 0 for the few-row
- * kernel, and the workgroups that share tiles, or 0 where none does.  form: 0
- * forward, 1 dx, 2 dW. */
-int nflow_debug_dense_cut(int form, int64_t M, int64_t N, int64_t K, int dtype, int* edge, int* groups);
+/* The kernel of the linear layer's product at this size: 0 the few-row one, else
+ * tiles of 64 x 64 (1), 128 x 64 (2, bf16), 128 x 128 (3; 4 the same with its loads
+ * further ahead, bf16) or 256 x 256 (5; fp32 256 x 128); and the workgroups that
+ * tiles' K steps are dealt out to, or 0 where tiles stay whole.  form: 0 forward,
+ * 1 dx (M, K, N of the layer as M, N, K), 2 dW (N, K, M), 3 both in one launch (the
+ * layer's M, N, K; groups 0: they are not). */
+int nflow_debug_dense_cut(int form, int64_t M, int64_t N, int64_t K, int dtype, int* kernel, int* groups);
 
 #ifdef __cplusplus
 }

@@ -35,11 +35,14 @@ struct DensePlan {
     DenseKind kind;
     int groups;
     size_t bytes;       // of the shared tiles' partial results
+    double us;          // estimated
 };
 
 // The tiled product, one translation unit per type.
 void launch_dense_bf16(const DenseArgs& a, DenseForm form, const DensePlan& p, float* part, hipStream_t st);
 void launch_dense_f32(const DenseArgs& a, DenseForm form, const DensePlan& p, float* part, hipStream_t st);
+// dx and dW by one launch, their K steps dealt out to p.groups workgroups.
+void launch_dense_pair_f32(const DenseArgs& dx, const DenseArgs& dw, const DensePlan& p, float* part, hipStream_t st);
 
 // A bf16 operand as the tiled product can fetch it: whole 16-byte groups at
 // 16-byte places, and a tile's rows within a buffer's range.

@@ -114,49 +114,76 @@ int64_t dz_runs(int64_t M, int64_t N) {
 // steps of what is left shared evenly, every CU is as busy as the next, for the
 // shared parts' way through the caches and a second launch.  Fitted to MI355X
 // times at 256 to 1024 tiles of 16 and 64 steps.
+struct Cut {
+    DenseKind kind;
+    int bm, bn, per_cu;
+    double alone, each, tile;
+    double tiles(int64_t M, int64_t N) const {
+        return std::ceil(static_cast<double>(M) / bm) * std::ceil(static_cast<double>(N) / bn);
+    }
+    // `steps` of 64 k's evenly dealt out to `occ` workgroups a CU, in `pieces` of tiles
+    // each, of which `parts` in all are shared.
+    DensePlan shared(int occ, double steps, double pieces, double parts) const {
+        const int groups = occ * num_cus();
+        const size_t slot = static_cast<size_t>(bm) * (bn + 1) * sizeof(float);
+        const double us = (steps / groups + 0.5) * std::max(alone, occ * each) + pieces * occ * tile + 3.0 +
+                          2 * parts * static_cast<double>(slot) / 5e6;
+        return DensePlan{kind, groups, round16(2 * groups * slot), us};
+    }
+};
+const Cut kCutsBf16[] = {{DENSE_SMALL, 64, 64, 3, 0.233, 0.182, 0.7},
+                         {DENSE_TALL, 128, 64, 2, 0.294, 0.273, 1.2},
+                         {DENSE_MID, 128, 128, 2, 0.613, 0.435, 2.4},
+                         {DENSE_DEEP, 128, 128, 1, 0.481, 0.476, 2.6},
+                         {DENSE_BIG, 256, 256, 1, 1.43, 1.50, 5.3}};
+const Cut kCutsF32[] = {{DENSE_SMALL, 64, 64, 3, 0.98, 0.99, 0.7},
+                        {DENSE_MID, 128, 128, 1, 2.66, 2.66, 2.5},
+                        {DENSE_BIG, 256, 128, 1, 4.77, 4.77, 5.0}};
+template <typename F>
+void each_cut(int dtype, F f) {
+    if (dtype == NFLOW_DTYPE_F32) {
+        for (const Cut& c : kCutsF32) f(c);
+    } else {
+        for (const Cut& c : kCutsBf16) f(c);
+    }
+}
+double steps_of(int64_t K) { return static_cast<double>((K + 63) / 64); }
+
 DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype) {
-    const bool f32 = dtype == NFLOW_DTYPE_F32;
-    const double cus = num_cus(), m = static_cast<double>(M), n = static_cast<double>(N),
-                 steps = std::ceil(static_cast<double>(K) / 64);
-    struct Cut {
-        DenseKind kind;
-        int bm, bn, per_cu;
-        double alone, each, tile;
-    };
-    static const Cut of_bf16[] = {{DENSE_SMALL, 64, 64, 3, 0.233, 0.182, 0.7},
-                                  {DENSE_TALL, 128, 64, 2, 0.294, 0.273, 1.2},
-                                  {DENSE_MID, 128, 128, 2, 0.613, 0.435, 2.4},
-                                  {DENSE_DEEP, 128, 128, 1, 0.481, 0.476, 2.6},
-                                  {DENSE_BIG, 256, 256, 1, 1.43, 1.50, 5.3}};
-    static const Cut of_f32[] = {{DENSE_SMALL, 64, 64, 3, 0.98, 0.99, 0.7},
-                                 {DENSE_MID, 128, 128, 1, 2.66, 2.66, 2.5},
-                                 {DENSE_BIG, 256, 128, 1, 4.77, 4.77, 5.0}};
-    DensePlan best{DENSE_MID, 0, 0};
-    double least = HUGE_VAL;
-    static const char* fk = getenv("DENSE_KIND");
-    static const char* fs = getenv("DENSE_GROUPS");
-    if (form == DENSE_FORWARD && M <= kDenseFewRows && (!fk || fk[0] == 'f')) return DensePlan{DENSE_FEW, 0, 0};
-    for (int i = 0; i < (f32 ? 3 : 5); ++i) {
-        const Cut& c = f32 ? of_f32[i] : of_bf16[i];
-        if (fk && fk[0] != (c.kind == DENSE_BIG ? 'b' : c.kind == DENSE_MID ? 'm' : c.kind == DENSE_DEEP ? 'd' : c.kind == DENSE_TALL ? 't' : 's')) continue;
-        const double tiles = std::ceil(m / c.bm) * std::ceil(n / c.bn), per = std::ceil(tiles / cus);
-        const double plain = steps * std::max(c.alone, per * c.each) + per * c.tile;
-        if (plain < least && (!fs || atoi(fs) == 0)) {
-            least = plain;
-            best = DensePlan{c.kind, 0, 0};
-        }
+    if (form == DENSE_FORWARD && M <= kDenseFewRows) return DensePlan{DENSE_FEW, 0, 0, 0.0};
+    const double cus = num_cus(), steps = steps_of(K);
+    DensePlan best{DENSE_MID, 0, 0, HUGE_VAL};
+    each_cut(dtype, [&](const Cut& c) {
+        const double tiles = c.tiles(M, N), per = std::ceil(tiles / cus);
+        const double us = steps * std::max(c.alone, per * c.each) + per * c.tile;
+        if (us < best.us) best = DensePlan{c.kind, 0, 0, us};
         for (int occ = 1; occ <= c.per_cu; ++occ) {
-            const int groups = occ * static_cast<int>(cus);
-            if (fs && atoi(fs) != occ) continue;
-            const int64_t t = static_cast<int64_t>(tiles), rest = t % groups;
+            const int groups = occ * num_cus();
+            const int64_t whole = static_cast<int64_t>(tiles) / groups, rest = static_cast<int64_t>(tiles) % groups;
             if (rest == 0 || rest * steps < groups) continue;
-            const double share = (t / groups) * steps + rest * steps / groups + 0.5;
-            const double moved = 2.0 * (groups + rest) * c.bm * c.bn * 4;
-            const double time = share * std::max(c.alone, occ * c.each) + (t / groups + 2) * occ * c.tile + 3.0 + moved / 5e6;
-            if (time < least) {
-                least = time;
-                best = DensePlan{c.kind, groups, static_cast<size_t>(2) * groups * c.bm * (c.bn + 1) * sizeof(float)};
-            }
+            const DensePlan p = c.shared(occ, tiles * steps, static_cast<double>(whole + 2), static_cast<double>(groups + rest));
+            if (p.us < best.us) best = p;
+        }
+    });
+    return best;
+}
+
+// dx (M, K) and dW (N, K) of fp32 in one launch, where that is faster than the two
+// by themselves, which pay a launch more (us: 2048 x 2048 x 2048 171 against 196,
+// 20000 x 256 x 768 118 against 136); else groups is 0.  In bf16, where the parts of
+// shared tiles weigh six times as much against the products, it is not (4096 x
+// 1024 x 1024 44 against 45, 65536 x 1024 x 1024 343 against 302).
+DensePlan pair_plan(int64_t M, int64_t N, int64_t K, int dtype) {
+    DensePlan best{DENSE_MID, 0, 0, 0.0};
+    if (dtype != NFLOW_DTYPE_F32 || M <= 0 || N <= 0 || K <= 0) return best;
+    best.us = dense_plan(DENSE_DX, M, K, N, dtype).us + dense_plan(DENSE_DW, N, K, M, dtype).us + 3.0;
+    for (const Cut& c : kCutsF32) {
+        const double tx = c.tiles(M, K), tw = c.tiles(N, K), steps = tx * steps_of(N) + tw * steps_of(M);
+        for (int occ = 1; occ <= c.per_cu; ++occ) {
+            const double groups = occ * num_cus();
+            if (steps < 2 * groups) continue;
+            const DensePlan p = c.shared(occ, steps, std::ceil((tx + tw) / groups) + 1, 2 * groups);
+            if (p.us < best.us) best = p;
         }
     }
     return best;
@@ -235,11 +262,12 @@ bool clash(const Span& a, const Span& b, size_t e) {
 }
 
 struct BackwardSpace {
-    size_t sums, x, w;
+    size_t sums, x, w, both;
     BackwardSpace(int64_t M, int64_t N, int64_t K, int dtype)
         : sums(round16(static_cast<size_t>(M > 0 ? dz_runs(M, N) * N : 0) * sizeof(float))),
-          x(product_space(DENSE_DX, M, K, N, dtype)), w(product_space(DENSE_DW, N, K, M, dtype)) {}
-    size_t bytes() const { return sums + x + w; }
+          x(product_space(DENSE_DX, M, K, N, dtype)), w(product_space(DENSE_DW, N, K, M, dtype)),
+          both(pair_plan(M, N, K, dtype).bytes) {}
+    size_t bytes() const { return sums + std::max(x + w, both); }
 };
 
 // Whether the forward product of these sizes is a tiled one of bf16.
@@ -346,6 +374,7 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
         if (meet(*in, sdx, e) || meet(*in, sdw, e)) return bad_arg(what, kShared);
     if (meet(sdx, sdw, e) || meet(sx, sdz, e) || meet(sw, sdz, e) || clash(sdy, sdz, e) || clash(spr, sdz, e))
         return bad_arg(what, kShared);
+    if ((M == 0 || N == 0 || !(act || dx)) && !dW && !dbias) return NFLOW_OK;
     hipStream_t st = as_stream(stream);
     float* sums = reinterpret_cast<float*>(ws);
     const int64_t runs = dz_runs(M, N);
@@ -363,25 +392,27 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
                            M > 0 ? runs : 0, N, dbias);
     if (copies.n) launch_dense_pack(copies.m, st);
     if (int rc = launch_status(what)) return rc;
-    if (dx && K > 0) {
-        const DenseArgs a{g, pw, lg, lw, M, K, N, nullptr, nullptr, 0, NFLOW_ACT_NONE, dx, lddx, nullptr, 0, nullptr};
-        if (int rc = product(what, DENSE_DX, a, dtype, ws + sp.sums, st)) return rc;
+    if (K == 0) return NFLOW_OK;
+    const DenseArgs ax{g, pw, lg, lw, M, K, N, nullptr, nullptr, 0, NFLOW_ACT_NONE, dx, lddx, nullptr, 0, nullptr};
+    const DenseArgs aw{g, px, lg, lx, N, K, M, nullptr, nullptr, 0, NFLOW_ACT_NONE, dW, lddw, nullptr, 0, ride};
+    const DensePlan pair = pair_plan(M, N, K, dtype);
+    if (dx && dW && pair.groups) {
+        launch_dense_pair_f32(ax, aw, pair, reinterpret_cast<float*>(ws + sp.sums), st);
+        return launch_status(what);
     }
-    if (dW && K > 0) {
-        const DenseArgs a{g, px, lg, lx, N, K, M, nullptr, nullptr, 0, NFLOW_ACT_NONE, dW, lddw, nullptr, 0, ride};
-        if (int rc = product(what, DENSE_DW, a, dtype, ws + sp.sums + sp.x, st)) return rc;
-    }
-    return NFLOW_OK;
+    if (dx)
+        if (int rc = product(what, DENSE_DX, ax, dtype, ws + sp.sums, st)) return rc;
+    return dW ? product(what, DENSE_DW, aw, dtype, ws + sp.sums + sp.x, st) : NFLOW_OK;
 }
 
-int nflow_debug_dense_cut(int form, int64_t M, int64_t N, int64_t K, int dtype, int* edge, int* groups) {
+int nflow_debug_dense_cut(int form, int64_t M, int64_t N, int64_t K, int dtype, int* kernel, int* groups) {
     clear_error();
     const char* what = "debug_dense_cut";
-    if (!edge || !groups) return bad_arg(what, "null output");
-    if (form < 0 || form > 2) return bad_arg(what, "unknown form");
+    if (!kernel || !groups) return bad_arg(what, "null output");
+    if (form < 0 || form > 3) return bad_arg(what, "unknown form");
     if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
-    const DensePlan p = dense_plan(static_cast<DenseForm>(form), M, N, K, dtype);
-    *edge = p.kind == DENSE_FEW ? 0 : p.kind == DENSE_SMALL ? 64 : p.kind == DENSE_BIG ? 256 : 128;
+    const DensePlan p = form == 3 ? pair_plan(M, N, K, dtype) : dense_plan(static_cast<DenseForm>(form), M, N, K, dtype);
+    *kernel = static_cast<int>(p.kind);
     *groups = p.groups;
     return NFLOW_OK;
 }

@@ -11,13 +11,13 @@ using Tall = DenseTile<bf16, 2, 2, 4, 2, 3>;        // 128 x 64, four waves, two
 using Deep = DenseTile<bf16, 2, 4, 4, 2, 4>;        // 128 x 128, eight waves, a workgroup a CU, loads three stages ahead
 using Big = DenseTile<bf16, 2, 4, 8, 4, 2>;         // 256 x 256, eight waves, a workgroup a CU
 
-template <bool AX, bool BX>
+template <bool AX, bool BX, bool SUMS = false>
 void launch(const DenseArgs& a, const DensePlan& p, float* part, hipStream_t st) {
-    if (p.kind == DENSE_BIG) launch_dense_tile<bf16, Big, &k_dense_dma<AX, BX, Big>>(a, p, part, st);
-    else if (p.kind == DENSE_TALL) launch_dense_tile<bf16, Tall, &k_dense_dma<AX, BX, Tall>>(a, p, part, st);
-    else if (p.kind == DENSE_DEEP) launch_dense_tile<bf16, Deep, &k_dense_dma<AX, BX, Deep>>(a, p, part, st);
-    else if (p.kind == DENSE_MID) launch_dense_tile<bf16, Mid, &k_dense_dma<AX, BX, Mid>>(a, p, part, st);
-    else launch_dense_tile<bf16, Small, &k_dense_dma<AX, BX, Small>>(a, p, part, st);
+    if (p.kind == DENSE_BIG) launch_dense_tile<bf16, Big, &k_dense_dma<AX, BX, SUMS, Big>>(a, p, part, st);
+    else if (p.kind == DENSE_TALL) launch_dense_tile<bf16, Tall, &k_dense_dma<AX, BX, SUMS, Tall>>(a, p, part, st);
+    else if (p.kind == DENSE_DEEP) launch_dense_tile<bf16, Deep, &k_dense_dma<AX, BX, SUMS, Deep>>(a, p, part, st);
+    else if (p.kind == DENSE_MID) launch_dense_tile<bf16, Mid, &k_dense_dma<AX, BX, SUMS, Mid>>(a, p, part, st);
+    else launch_dense_tile<bf16, Small, &k_dense_dma<AX, BX, SUMS, Small>>(a, p, part, st);
 }
 
 // Up to three matrices copied to rows of dense_pitch(cols) values, zero past
@@ -61,6 +61,7 @@ void launch_dense_pack(const DensePack (&m)[3], hipStream_t st) {
 void launch_dense_bf16(const DenseArgs& a, DenseForm form, const DensePlan& p, float* part, hipStream_t st) {
     if (form == DENSE_FORWARD) launch<false, false>(a, p, part, st);
     else if (form == DENSE_DX) launch<false, true>(a, p, part, st);
+    else if (a.sums) launch<true, true, true>(a, p, part, st);
     else launch<true, true>(a, p, part, st);
 }
 

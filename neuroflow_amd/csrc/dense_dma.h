@@ -70,15 +70,15 @@ struct DenseFetch {
 // its memory takes the loads of the stage NS on, and the next stage, whose loads
 // are waited for there, gives its first fragments.  Reads and loads are spread
 // evenly, a few ahead of every row tile's products.
-template <bool AX, bool BX, typename Tile>
-__global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_dma(DenseArgs a, DenseShare sh) {
+// SUMS: with the sums of a's rows.
+template <bool AX, bool BX, bool SUMS, typename Tile>
+__device__ __forceinline__ void dense_dma_tile(const DenseArgs& a, const DenseSlots& sl, const TilePos& pos, int k0, int k1,
+                                               int slot) {
     constexpr int TI = Tile::TI, TJ = Tile::TJ, NS = Tile::NS;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wid / Tile::WN, wn = wid % Tile::WN;
     const uint32_t lds0 = wide_lds_addr(lds);
-    dense_each(sh, [&](int64_t tile, int k0, int k1, int slot) {
-    const TilePos pos = tile_pos(tile, sh.tiles_m, sh.tiles_n, 4);
     const int64_t m0 = pos.tm * Tile::BM, n0 = pos.tn * Tile::BN;
     const DenseFetch<AX, Tile::BM, Tile::WAVES> fa(a.A, a.lda, m0, a.M, a.K, wid);
     const DenseFetch<BX, Tile::BN, Tile::WAVES> fb(a.B, a.ldb, n0, a.N, a.K, wid);
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_dma(DenseArg
 #pragma unroll
         for (int j = 0; j < TJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-    DenseSums<Tile> sums(AX && a.sums && pos.tn == 0, wn);
+    DenseSums<Tile> sums(SUMS && pos.tn == 0, wn);
     const int arow = 16 * TI * wm, brow = 16 * TJ * wn;
     v8bf xa[2][TI], xb[2][TJ];
     // Fragment e of half h of a stage: the TJ of B, then the TI of A, in the order of need.
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_dma(DenseArg
 #pragma unroll
         for (int j = 0; j < TJ; ++j)
             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[h][j], xa[h][i], acc[i][j], 0, 0, 0);
-        if constexpr (AX) {
+        if constexpr (SUMS) {
             const v8bf one[1] = {xa[h][i]};
             sums.add(i, one);
         }
@@ -150,9 +150,16 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_dma(DenseArg
         s = next;
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // the empty loads past the last stage
-    if constexpr (AX) sums.leave(a, sh, m0, slot, wm);
+    if constexpr (SUMS) sums.leave(a, sl, m0, slot, wm);
     __syncthreads();
-    dense_leave<bf16, Tile>(a, sh, acc, reinterpret_cast<float*>(lds) + wid * Tile::STRIP, m0, n0, slot, wm, wn);
+    dense_leave<bf16, Tile>(a, sl, acc, reinterpret_cast<float*>(lds) + wid * Tile::STRIP, m0, n0, slot, wm, wn);
+}
+
+template <bool AX, bool BX, bool SUMS, typename Tile>
+__global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_dma(DenseArgs a, DenseShare sh) {
+    dense_each(sh, [&](int64_t tile, int k0, int k1, int slot) {
+        dense_dma_tile<AX, BX, SUMS, Tile>(a, DenseSlots{sh.part, sh.groups}, tile_pos(tile, sh.tiles_m, sh.tiles_n, 4), k0, k1,
+                                     slot);
     });
 }
 

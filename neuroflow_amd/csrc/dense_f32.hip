@@ -82,55 +82,71 @@ struct StageProducts {
 // waves splits before its products and the other between them, so that a SIMD's
 // two waves use the VALU and the matrix core in turn.
 template <bool AX, bool BX, typename Tile>
-__global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_f32(DenseArgs a, DenseShare sh) {
+__device__ __forceinline__ void dense_f32_tile(const DenseArgs& a, const DenseSlots& sl, const TilePos& pos, int k0, int k1,
+                                               int slot) {
     constexpr int TI = Tile::TI, TJ = Tile::TJ;
     static_assert(Tile::KB == 32 && Tile::P == 3 && Tile::NS == 2, "two stages of three planes");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wid / Tile::WN, wn = wid % Tile::WN;
-    dense_each(sh, [&](int64_t tile, int k0, int k1, int slot) {
-        const TilePos pos = tile_pos(tile, sh.tiles_m, sh.tiles_n, 4);
-        const int64_t m0 = pos.tm * Tile::BM, n0 = pos.tn * Tile::BN;
-        v4f acc[TI][TJ];
+    const int64_t m0 = pos.tm * Tile::BM, n0 = pos.tn * Tile::BN;
+            v4f acc[TI][TJ];
 #pragma unroll
-        for (int i = 0; i < TI; ++i)
+            for (int i = 0; i < TI; ++i)
 #pragma unroll
-            for (int j = 0; j < TJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        DenseStage<AX, Tile::BM, 32, Tile::THREADS> ra;
-        DenseStage<BX, Tile::BN, 32, Tile::THREADS> rb;
-        auto load = [&](int k) {
-            ra.load(static_cast<const float*>(a.A), a.lda, m0, a.M, static_cast<int64_t>(k) * 32, k < k1 ? a.K : 0);
-            rb.load(static_cast<const float*>(a.B), a.ldb, n0, a.N, static_cast<int64_t>(k) * 32, k < k1 ? a.K : 0);
-        };
-        auto store = [&](int s) {
-            ra.store(lds + s * Tile::STAGE);
-            rb.store(lds + s * Tile::STAGE + 3 * Tile::PLANE_A);
-        };
-        DenseSums<Tile> sums(AX && a.sums && pos.tn == 0, wn);
-        const int arow = 16 * TI * wm, brow = 16 * TJ * wn;
-        load(k0);
-        store(0);
-        load(k0 + 1);
-        __syncthreads();
-        int s = 0;
-        for (int k = k0; k < k1; ++k, s ^= 1) {
-            const uint8_t* st = lds + s * Tile::STAGE;
-            const StageProducts<AX, BX, Tile> stage(st, brow);
-            const bool first = wid < Tile::WAVES / 2;
-            if (first) {
-                store(s ^ 1);
-                load(k + 2);
-            }
-            stage.run(st, acc, sums, arow, 0, TI / 2);
-            if (!first) {
-                store(s ^ 1);
-                load(k + 2);
-            }
-            stage.run(st, acc, sums, arow, TI / 2, TI);
+                for (int j = 0; j < TJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            DenseStage<AX, Tile::BM, 32, Tile::THREADS> ra;
+            DenseStage<BX, Tile::BN, 32, Tile::THREADS> rb;
+            auto load = [&](int k) {
+                ra.load(static_cast<const float*>(a.A), a.lda, m0, a.M, static_cast<int64_t>(k) * 32, k < k1 ? a.K : 0);
+                rb.load(static_cast<const float*>(a.B), a.ldb, n0, a.N, static_cast<int64_t>(k) * 32, k < k1 ? a.K : 0);
+            };
+            auto store = [&](int s) {
+                ra.store(lds + s * Tile::STAGE);
+                rb.store(lds + s * Tile::STAGE + 3 * Tile::PLANE_A);
+            };
+            DenseSums<Tile> sums(AX && a.sums && pos.tn == 0, wn);
+            const int arow = 16 * TI * wm, brow = 16 * TJ * wn;
+            load(k0);
+            store(0);
+            load(k0 + 1);
             __syncthreads();
-        }
-        if constexpr (AX) sums.leave(a, sh, m0, slot, wm);
-        dense_leave<float, Tile>(a, sh, acc, reinterpret_cast<float*>(lds) + wid * Tile::STRIP, m0, n0, slot, wm, wn);
+            int s = 0;
+            for (int k = k0; k < k1; ++k, s ^= 1) {
+                const uint8_t* st = lds + s * Tile::STAGE;
+                const StageProducts<AX, BX, Tile> stage(st, brow);
+                const bool first = wid < Tile::WAVES / 2;
+                if (first) {
+                    store(s ^ 1);
+                    load(k + 2);
+                }
+                stage.run(st, acc, sums, arow, 0, TI / 2);
+                if (!first) {
+                    store(s ^ 1);
+                    load(k + 2);
+                }
+                stage.run(st, acc, sums, arow, TI / 2, TI);
+                __syncthreads();
+            }
+            if constexpr (AX) sums.leave(a, sl, m0, slot, wm);
+            dense_leave<float, Tile>(a, sl, acc, reinterpret_cast<float*>(lds) + wid * Tile::STRIP, m0, n0, slot, wm, wn);
+}
+
+template <bool AX, bool BX, typename Tile>
+__global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_f32(DenseArgs a, DenseShare sh) {
+    dense_each(sh, [&](int64_t tile, int k0, int k1, int slot) {
+        dense_f32_tile<AX, BX, Tile>(a, DenseSlots{sh.part, sh.groups}, tile_pos(tile, sh.tiles_m, sh.tiles_n, 4), k0, k1,
+                                     slot);
+    });
+}
+
+template <typename Tile>
+__global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_f32_pair(DensePair pr) {
+    dense_each_pair(pr, [&](int which, int64_t tile, int k0, int k1, int slot) {
+        const TilePos pos = tile_pos(tile, pr.tiles_m[which], pr.tiles_n[which], 4);
+        const DenseSlots sl{pr.part, pr.groups};
+        if (which == 0) dense_f32_tile<false, true, Tile>(pr.a[0], sl, pos, k0, k1, slot);
+        else dense_f32_tile<true, true, Tile>(pr.a[1], sl, pos, k0, k1, slot);
     });
 }
 
@@ -151,6 +167,12 @@ void launch_dense_f32(const DenseArgs& a, DenseForm form, const DensePlan& p, fl
     if (form == DENSE_FORWARD) launch<false, false>(a, p, part, st);
     else if (form == DENSE_DX) launch<false, true>(a, p, part, st);
     else launch<true, true>(a, p, part, st);
+}
+
+void launch_dense_pair_f32(const DenseArgs& dx, const DenseArgs& dw, const DensePlan& p, float* part, hipStream_t st) {
+    if (p.kind == DENSE_SMALL) launch_dense_pair_tile<float, Small, &k_dense_f32_pair<Small>>(dx, dw, p, part, st);
+    else if (p.kind == DENSE_MID) launch_dense_pair_tile<float, Mid, &k_dense_f32_pair<Mid>>(dx, dw, p, part, st);
+    else launch_dense_pair_tile<float, Big, &k_dense_f32_pair<Big>>(dx, dw, p, part, st);
 }
 
 }  // namespace nfq

@@ -225,10 +225,14 @@ __device__ __forceinline__ void dense_load(Raw8<T>& v, const T* p, int64_t left)
 // reach into at most two.  A part of a tile leaves its fp32 sums in a slot (two a
 // workgroup, BM x BN each), and a second launch joins a tile's slots in the
 // workgroups' order.
+struct DenseSlots {
+    float* part;        // 2 groups slots of BM x BN, then as many of BM: the sums of a's rows
+    int groups;
+};
 struct DenseShare {
     int64_t tiles_m, tiles_n;
     int groups, whole, rest, ksteps;
-    float* part;        // 2 groups slots of BM x BN, then as many of BM: the sums of a's rows
+    float* part;
     __host__ __device__ int64_t step_of(int i) const { return static_cast<int64_t>(i) * rest * ksteps / groups; }
 };
 
@@ -258,7 +262,7 @@ __device__ __forceinline__ void dense_each(const DenseShare& sh, F f) {
 
 // What becomes of a wave's sums: the results, or a slot's.
 template <typename T, typename Tile>
-__device__ __forceinline__ void dense_leave(const DenseArgs& a, const DenseShare& sh, const v4f (&acc)[Tile::TI][Tile::TJ],
+__device__ __forceinline__ void dense_leave(const DenseArgs& a, const DenseSlots& sh, const v4f (&acc)[Tile::TI][Tile::TJ],
                                             float* strip, int64_t m0, int64_t n0, int slot, int wm, int wn) {
     const int i = 16 * Tile::TI * wm, j = 16 * Tile::TJ * wn;
     if (slot >= 0) {
@@ -291,7 +295,7 @@ struct DenseSums {
         for (int p = P - 1; p >= 0; --p)
             s[i / Tile::WN] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, a[p], s[i / Tile::WN], 0, 0, 0);
     }
-    __device__ __forceinline__ void leave(const DenseArgs& a, const DenseShare& sh, int64_t m0, int slot, int wm) const {
+    __device__ __forceinline__ void leave(const DenseArgs& a, const DenseSlots& sh, int64_t m0, int slot, int wm) const {
         const int r = threadIdx.x & 63;
         if (mine == Tile::WN || r >= 16) return;
         float* to = slot >= 0 ? sh.part + 2 * static_cast<int64_t>(sh.groups) * Tile::BM * Tile::BN +
@@ -305,16 +309,12 @@ struct DenseSums {
     }
 };
 
-// The shared tiles' sums, over their slots in order, and the epilogue: a
-// workgroup for 16 rows of a tile.
-template <typename T, int BM, int BN>
-__global__ __launch_bounds__(256) void k_dense_join(DenseArgs a, DenseShare sh) {
-    const int t = blockIdx.x / (BM / 16), row0 = 16 * (blockIdx.x % (BM / 16));
-    const int64_t first = static_cast<int64_t>(t) * sh.ksteps, last = first + sh.ksteps;
-    int i = static_cast<int>(first * sh.groups / (static_cast<int64_t>(sh.rest) * sh.ksteps));   // may be one too low
-    while (sh.step_of(i + 1) <= first) ++i;
-    if (sh.step_of(i) <= first && sh.step_of(i + 1) >= last) return;         // one workgroup's: stored
-    const TilePos pos = tile_pos(static_cast<int64_t>(sh.whole) * sh.groups + t, sh.tiles_m, sh.tiles_n, 4);
+// Sixteen rows of a shared tile from row0 on: the sum of its slots, of workgroups i,
+// i + 1, ... up to the tile's last step, and the epilogue.  begin(i): a
+// workgroup's first step; its slot is its second where that lies ahead of the tile.
+template <typename T, int BM, int BN, typename Begin>
+__device__ __forceinline__ void dense_join(const DenseArgs& a, const DenseSlots& sl, const TilePos& pos, int row0, int i,
+                                           int64_t first, int64_t last, Begin begin) {
     const int64_t m0 = pos.tm * BM + row0, n0 = pos.tn * BN;
     constexpr int Q = 16 * BN / 4 / 256;                                     // groups of four values a thread
     v4f z[Q];
@@ -322,10 +322,10 @@ __global__ __launch_bounds__(256) void k_dense_join(DenseArgs a, DenseShare sh) 
     for (int q = 0; q < Q; ++q) z[q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     const bool sums = a.sums && pos.tn == 0 && threadIdx.x < 16;
     float s = 0.0f;
-    for (; sh.step_of(i) < last; ++i) {
-        const int n = sh.step_of(i) / sh.ksteps < t ? 1 : 0;                 // its second part, if it began in the tile before
-        if (sums) s += sh.part[(2 * static_cast<int64_t>(sh.groups) * BN + 2 * i + n) * BM + row0 + threadIdx.x];
-        const float* p = sh.part + static_cast<int64_t>(2 * i + n) * BM * BN + row0 * BN;
+    for (; i < sl.groups && begin(i) < last; ++i) {
+        const int64_t slot = 2 * i + (begin(i) < first ? 1 : 0);
+        if (sums) s += sl.part[(2 * static_cast<int64_t>(sl.groups) * BN + slot) * BM + row0 + threadIdx.x];
+        const float* p = sl.part + slot * BM * BN + row0 * BN;
 #pragma unroll
         for (int q = 0; q < Q; ++q) z[q] += *reinterpret_cast<const v4f*>(p + 4 * (threadIdx.x + 256 * q));
     }
@@ -337,12 +337,99 @@ __global__ __launch_bounds__(256) void k_dense_join(DenseArgs a, DenseShare sh) 
     if (sums && m0 + threadIdx.x < a.M) a.sums[m0 + threadIdx.x] = s;
 }
 
-// `kernel` over a product as the plan has it, and the join of what is shared.
-template <typename T, typename Tile, auto kernel>
-void launch_dense_tile(const DenseArgs& a, const DensePlan& p, float* part, hipStream_t st) {
+// A workgroup for 16 rows of the tile that workgroup i begins within, if it is
+// the first to.
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(256) void k_dense_join(DenseArgs a, DenseShare sh) {
+    const int i = blockIdx.x / (BM / 16) + 1;
+    const int64_t at = sh.step_of(i), t = at / sh.ksteps, first = t * sh.ksteps;
+    if (at == first || sh.step_of(i - 1) > first) return;
+    const TilePos pos = tile_pos(static_cast<int64_t>(sh.whole) * sh.groups + t, sh.tiles_m, sh.tiles_n, 4);
+    dense_join<T, BM, BN>(a, DenseSlots{sh.part, sh.groups}, pos, 16 * (blockIdx.x % (BM / 16)), i - 1, first,
+                          first + sh.ksteps, [&](int w) { return sh.step_of(w); });
+}
+
+// ---- two products in one launch ------------------------------------------------------------
+// dx and dW with all of their K steps dealt out evenly in one row, dx's tiles
+// first: one launch and one join where each by itself would leave CUs idle at
+// its end and more parts of tiles behind.
+struct DensePair {
+    DenseArgs a[2];
+    int64_t tiles_m[2], tiles_n[2];
+    int ksteps[2];
+    int64_t first[2], steps;     // step at which each begins, and all of them
+    int groups;
+    float* part;
+    __host__ __device__ int64_t step_of(int i) const { return i * steps / groups; }
+    // The product, tile and first step of the tile that step `at` is in.
+    __device__ __forceinline__ int64_t tile_of(int64_t at, int& which, int64_t& begin) const {
+        which = at >= first[1] ? 1 : 0;
+        const int64_t t = (at - first[which]) / ksteps[which];
+        begin = first[which] + t * ksteps[which];
+        return t;
+    }
+};
+
+// Calls f(product, its tile, first step, end, slot or -1) for this workgroup's work.
+template <typename F>
+__device__ __forceinline__ void dense_each_pair(const DensePair& pr, F f) {
+    const int i = gemm_tile_of_block(blockIdx.x, pr.groups, 8);
+    const int64_t from = pr.step_of(i), end = pr.step_of(i + 1);
+    for (int64_t at = from; at < end;) {
+        int which;
+        int64_t begin;
+        const int64_t t = pr.tile_of(at, which, begin);
+        const int ks = pr.ksteps[which], k = static_cast<int>(at - begin);
+        const int stop = end - begin < ks ? static_cast<int>(end - begin) : ks;
+        if (at > from) __syncthreads();
+        f(which, t, k, stop, k == 0 && stop == ks ? -1 : 2 * i + (at > from ? 1 : 0));
+        at = begin + stop;
+    }
+}
+
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(256) void k_dense_join_pair(DensePair pr) {
+    const int i = blockIdx.x / (BM / 16) + 1;
+    const int64_t at = pr.step_of(i);
+    if (at >= pr.steps) return;
+    int which;
+    int64_t first;
+    const int64_t t = pr.tile_of(at, which, first);
+    if (at == first || pr.step_of(i - 1) > first) return;
+    const TilePos pos = tile_pos(t, pr.tiles_m[which], pr.tiles_n[which], 4);
+    dense_join<T, BM, BN>(pr.a[which], DenseSlots{pr.part, pr.groups}, pos, 16 * (blockIdx.x % (BM / 16)), i - 1, first,
+                          first + pr.ksteps[which], [&](int w) { return pr.step_of(w); });
+}
+
+// Lets `kernel` have its tile's LDS.
+template <typename Tile, auto kernel>
+void dense_lds() {
     static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, Tile::LDS);
     (void)once;
+}
+
+// dx and dW by `kernel`, and their join.
+template <typename T, typename Tile, auto kernel>
+void launch_dense_pair_tile(const DenseArgs& dx, const DenseArgs& dw, const DensePlan& p, float* part, hipStream_t st) {
+    dense_lds<Tile, kernel>();
+    DensePair pr{{dx, dw}, {}, {}, {}, {}, 0, p.groups, part};
+    for (int j = 0; j < 2; ++j) {
+        pr.tiles_m[j] = (pr.a[j].M + Tile::BM - 1) / Tile::BM;
+        pr.tiles_n[j] = (pr.a[j].N + Tile::BN - 1) / Tile::BN;
+        pr.ksteps[j] = static_cast<int>((pr.a[j].K + Tile::KB - 1) / Tile::KB);
+        pr.first[j] = pr.steps;
+        pr.steps += pr.tiles_m[j] * pr.tiles_n[j] * pr.ksteps[j];
+    }
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(p.groups)), dim3(Tile::THREADS), Tile::LDS, st, pr);
+    hipLaunchKernelGGL((k_dense_join_pair<T, Tile::BM, Tile::BN>),
+                       dim3(static_cast<unsigned>((p.groups - 1) * (Tile::BM / 16))), dim3(256), 0, st, pr);
+}
+
+// `kernel` over a product as the plan has it, and the join of what is shared.
+template <typename T, typename Tile, auto kernel>
+void launch_dense_tile(const DenseArgs& a, const DensePlan& p, float* part, hipStream_t st) {
+    dense_lds<Tile, kernel>();
     const int64_t tm = (a.M + Tile::BM - 1) / Tile::BM, tn = (a.N + Tile::BN - 1) / Tile::BN, tiles = tm * tn;
     const int ks = static_cast<int>((a.K + Tile::KB - 1) / Tile::KB);
     DenseShare sh{tm, tn, static_cast<int>(tiles), 1, 0, ks, part};
@@ -353,8 +440,8 @@ void launch_dense_tile(const DenseArgs& a, const DensePlan& p, float* part, hipS
     }
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(sh.groups)), dim3(Tile::THREADS), Tile::LDS, st, a, sh);
     if (sh.rest)
-        hipLaunchKernelGGL((k_dense_join<T, Tile::BM, Tile::BN>), dim3(static_cast<unsigned>(sh.rest * (Tile::BM / 16))),
-                           dim3(256), 0, st, a, sh);
+        hipLaunchKernelGGL((k_dense_join<T, Tile::BM, Tile::BN>),
+                           dim3(static_cast<unsigned>((sh.groups - 1) * (Tile::BM / 16))), dim3(256), 0, st, a, sh);
 }
 
 }  // namespace nfq

@@ -11,7 +11,14 @@ from residual_reference import DTYPES, U, act, act_bound, gen, half, rows, withi
 from residual_reference import dense as product, dense_bound
 
 pytestmark = pytest.mark.gpu
-# (M, K, N): few rows, tiles of 64, 128 and 256 (from a tile for every CU on), splits of K, odd everything.
+# (M, K, N): one row to thousands, odd everything; CUTS are the least that take every
+# kernel and every way of dealing its tiles out, forward and backward (test_every_cut_is_met).
+CUTS = [(33, 200, 4100), (33, 1025, 5003), (33, 2050, 3000), (33, 5003, 1537), (72, 72, 4100), (72, 130, 12000), (72, 4100, 72),
+        (130, 72, 12000), (130, 12000, 72), (200, 33, 4100), (200, 1000, 8192), (200, 1025, 3000), (200, 1300, 4100),
+        (200, 4100, 33), (200, 4100, 1300), (200, 8192, 1000), (257, 4100, 12000), (257, 12000, 4100), (1000, 1000, 1537),
+        (1000, 1025, 4100), (1000, 4100, 1025), (1025, 33, 5003), (1025, 200, 3000), (1025, 3000, 200), (1025, 4100, 1000),
+        (1025, 5003, 33), (1300, 200, 4100), (1537, 33, 5003), (1537, 5003, 33), (2050, 33, 3000), (2050, 3000, 33),
+        (3000, 257, 8192), (4100, 72, 72), (8192, 200, 1000), (12000, 4100, 257), (65536, 1000, 1000), (40000, 1280, 2000), (40000, 2000, 1280)]
 SIZES = [(1, 1, 1), (1, 4096, 4096), (2, 7, 3), (5, 100, 33), (16, 64, 16), (17, 200, 130), (33, 513, 64), (64, 31, 257),
          (65, 64, 64), (66, 1, 65), (100, 1000, 20), (129, 65, 127), (200, 2021, 301), (257, 128, 1000), (300, 8192, 136),
          (1000, 33, 1), (1537, 200, 1001), (2200, 96, 2056), (4099, 72, 2050), (2100, 2100, 40), (70, 2100, 2100),
@@ -260,19 +267,51 @@ def test_same_bits_streams_and_graph(gpu):
 
 
 def test_every_cut_is_met(gpu):
-    """The sizes above take every kernel that the cut chooses from, of each form."""
     met = set()
-    edge, splits = C.c_int(), C.c_int()
-    for M, K, N in SIZES + [(8192, 130, 66), (9000, 256, 256)]:
+    kernel, groups = C.c_int(), C.c_int()
+    for M, K, N in SIZES + CUTS:
         for dt in (0, 1):
-            for form, size in enumerate(((M, N, K), (M, K, N), (N, K, M))):
-                assert _lib.lib().nflow_debug_dense_cut(form, *size, dt, C.byref(edge), C.byref(splits)) == _lib.OK
-                met.add((form, dt, edge.value, splits.value > 0))
+            for form, size in enumerate(((M, N, K), (M, K, N), (N, K, M), (M, N, K))):
+                assert _lib.lib().nflow_debug_dense_cut(form, *size, dt, C.byref(kernel), C.byref(groups)) == _lib.OK
+                met.add((form, dt, kernel.value, groups.value > 0))
+    want = {(0, dt, 0, False) for dt in (0, 1)}                         # few rows
     for form in range(3):
-        for dt in (0, 1):
-            for kind in ((0, False),) if form == 0 else ():
-                assert (form, dt, *kind) in met
-            assert {(64, True), (128, False)} <= {(e, s) for f, d, e, s in met if (f, d) == (form, dt)}, (form, dt, met)
+        want |= {(form, 0, k, shared) for k in (1, 3, 5) for shared in (False, True)}
+        want |= {(form, 1, k, False) for k in (1, 2, 3, 4, 5)} | {(form, 1, k, True) for k in (1, 2, 4, 5)}
+    want |= {(3, 0, k, True) for k in (1, 3, 5)}
+    assert want <= met, sorted(want - met)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N", CUTS)
+def test_cuts(gpu, M, K, N, dtype):
+    """Every kernel, forward and backward, on whole numbers (every result known)
+    and on operands that are, in bf16, 16-byte aligned in rows of their own stride."""
+    g = gen(M)
+    up = lambda n: (n + 7) // 8 * 8
+    def whole(rows, cols, lo, hi, keep=None):
+        buf = torch.full((rows, up(cols)), float("nan"), device="cuda", dtype=dtype)
+        v = torch.randint(lo, hi, (rows, cols), generator=g, device="cuda").float()
+        if keep is not None:                                             # a few columns alone are not zero
+            v[:, torch.randperm(cols, generator=g, device="cuda")[keep:]] = 0
+        buf[:, :cols] = v
+        return buf[:, :cols]
+    few = 60 if dtype == torch.float32 else None
+    top = 2 ** 17 if dtype == torch.float32 else 3
+    x, W = whole(M, K, -top, top), whole(N, K, -1, 2, few)
+    y, pre = dense.linear(x, W, None, "relu", return_pre=True)
+    want = x.double() @ W.double().t()
+    assert torch.equal(pre, want.to(dtype)) and torch.equal(y, want.clamp(min=0).to(dtype))
+    dy = whole(M, N, -1, 2, few)
+    if few is not None:
+        dy[torch.randperm(M, generator=g, device="cuda")[few:]] = 0
+    W = whole(N, K, -top, top)
+    dx, dW, db, dz = dense.linear_backward(dy, x, W)
+    assert torch.equal(dx, (dy.double() @ W.double()).to(dtype))
+    assert torch.equal(dW, (dy.double().t() @ x.double()).to(dtype))
+    assert torch.equal(db, dy.double().sum(0).float())
+    again = dense.linear_backward(dy.contiguous(), x.contiguous(), W.contiguous())
+    assert all(torch.equal(a, b) for a, b in zip((dx, dW, db), again))
 
 
 def test_refusals(gpu):
