@@ -182,7 +182,9 @@ DensePlan pair_plan(int64_t M, int64_t N, int64_t K, int dtype) {
         for (int occ = 1; occ <= c.per_cu; ++occ) {
             const double groups = occ * num_cus();
             if (steps < 2 * groups) continue;
-            const DensePlan p = c.shared(occ, steps, std::ceil((tx + tw) / groups) + 1, 2 * groups);
+            // Tiles of one length in whole rounds: none is shared.
+            const bool even = steps_of(N) == steps_of(M) && std::fmod(tx + tw, groups) == 0.0;
+            const DensePlan p = c.shared(occ, steps, std::ceil((tx + tw) / groups) + (even ? 0 : 1), even ? 0 : 2 * groups);
             if (p.us < best.us) best = p;
         }
     }

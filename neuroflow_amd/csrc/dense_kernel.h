@@ -309,44 +309,56 @@ struct DenseSums {
     }
 };
 
-// Sixteen rows of a shared tile from row0 on: the sum of its slots, of workgroups i,
-// i + 1, ... up to the tile's last step, and the epilogue.  begin(i): a
-// workgroup's first step; its slot is its second where that lies ahead of the tile.
-template <typename T, int BM, int BN, typename Begin>
+// kJoinRows rows of a shared tile from row0 on: the sum of its slots, of
+// workgroups i .. stop - 1, and the epilogue.  `late`: the tile is the second that
+// workgroup i had a part of.  Bound by the slots' bytes, from the caches.
+constexpr int kJoinRows = 8;
+template <typename T, int BM, int BN>
 __device__ __forceinline__ void dense_join(const DenseArgs& a, const DenseSlots& sl, const TilePos& pos, int row0, int i,
-                                           int64_t first, int64_t last, Begin begin) {
+                                           int stop, bool late) {
     const int64_t m0 = pos.tm * BM + row0, n0 = pos.tn * BN;
-    constexpr int Q = 16 * BN / 4 / 256;                                     // groups of four values a thread
-    v4f z[Q];
-#pragma unroll
-    for (int q = 0; q < Q; ++q) z[q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    const bool sums = a.sums && pos.tn == 0 && threadIdx.x < 16;
+    constexpr int Q = kJoinRows * BN / 4, TH = Q < 256 ? Q : 256, PER = Q / TH;   // groups of four values, threads, of each
+    const bool sums = a.sums && pos.tn == 0 && threadIdx.x < kJoinRows;
+    v4f z[PER];
     float s = 0.0f;
-    for (; i < sl.groups && begin(i) < last; ++i) {
-        const int64_t slot = 2 * i + (begin(i) < first ? 1 : 0);
-        if (sums) s += sl.part[(2 * static_cast<int64_t>(sl.groups) * BN + slot) * BM + row0 + threadIdx.x];
-        const float* p = sl.part + slot * BM * BN + row0 * BN;
 #pragma unroll
-        for (int q = 0; q < Q; ++q) z[q] += *reinterpret_cast<const v4f*>(p + 4 * (threadIdx.x + 256 * q));
-    }
+    for (int q = 0; q < PER; ++q) z[q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (static_cast<int>(threadIdx.x) < TH) {
+#pragma unroll 4
+        for (int w = i; w < stop; ++w) {
+            const int64_t slot = 2 * static_cast<int64_t>(w) + (w == i && late ? 1 : 0);
+            const float* p = sl.part + slot * BM * BN + row0 * BN;
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-        const int e = 4 * (threadIdx.x + 256 * q);
-        if (m0 + e / BN < a.M) dense_finish<T>(a, m0 + e / BN, n0 + e % BN, z[q]);
+            for (int q = 0; q < PER; ++q) z[q] += *reinterpret_cast<const v4f*>(p + 4 * (threadIdx.x + TH * q));
+            if (sums) s += sl.part[(2 * static_cast<int64_t>(sl.groups) * BN + slot) * BM + row0 + threadIdx.x];
+        }
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int e = 4 * (threadIdx.x + TH * q);
+            if (m0 + e / BN < a.M) dense_finish<T>(a, m0 + e / BN, n0 + e % BN, z[q]);
+        }
     }
     if (sums && m0 + threadIdx.x < a.M) a.sums[m0 + threadIdx.x] = s;
 }
+// The first workgroup, of `groups` that `steps` are dealt out to, that begins at
+// step `at` or past it.
+__host__ __device__ inline int dense_from(int64_t at, int64_t steps, int groups) {
+    return static_cast<int>((at * groups + steps - 1) / steps);
+}
 
-// A workgroup for 16 rows of the tile that workgroup i begins within, if it is
-// the first to.
+// A workgroup for kJoinRows rows of a tile of those that are left.
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void k_dense_join(DenseArgs a, DenseShare sh) {
-    const int i = blockIdx.x / (BM / 16) + 1;
-    const int64_t at = sh.step_of(i), t = at / sh.ksteps, first = t * sh.ksteps;
-    if (at == first || sh.step_of(i - 1) > first) return;
-    const TilePos pos = tile_pos(static_cast<int64_t>(sh.whole) * sh.groups + t, sh.tiles_m, sh.tiles_n, 4);
-    dense_join<T, BM, BN>(a, DenseSlots{sh.part, sh.groups}, pos, 16 * (blockIdx.x % (BM / 16)), i - 1, first,
-                          first + sh.ksteps, [&](int w) { return sh.step_of(w); });
+    const int t = blockIdx.x / (BM / kJoinRows);
+    const int64_t first = static_cast<int64_t>(t) * sh.ksteps, last = first + sh.ksteps, all = static_cast<int64_t>(sh.rest) * sh.ksteps;
+    int i = dense_from(first, all, sh.groups);
+    const bool late = sh.step_of(i) > first;
+    if (late) --i;                                                       // began in the tile before
+    const int stop = dense_from(last, all, sh.groups);
+    if (stop == i + 1) return;                                           // one workgroup's: stored
+    dense_join<T, BM, BN>(a, DenseSlots{sh.part, sh.groups},
+                          tile_pos(static_cast<int64_t>(sh.whole) * sh.groups + t, sh.tiles_m, sh.tiles_n, 4),
+                          kJoinRows * (blockIdx.x % (BM / kJoinRows)), i, stop, late);
 }
 
 // ---- two products in one launch ------------------------------------------------------------
@@ -387,18 +399,19 @@ __device__ __forceinline__ void dense_each_pair(const DensePair& pr, F f) {
     }
 }
 
+// The same for the tile that workgroup i begins within, if it is the first to.
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void k_dense_join_pair(DensePair pr) {
-    const int i = blockIdx.x / (BM / 16) + 1;
+    const int i = blockIdx.x / (BM / kJoinRows) + 1;
     const int64_t at = pr.step_of(i);
-    if (at >= pr.steps) return;
     int which;
     int64_t first;
     const int64_t t = pr.tile_of(at, which, first);
-    if (at == first || pr.step_of(i - 1) > first) return;
-    const TilePos pos = tile_pos(t, pr.tiles_m[which], pr.tiles_n[which], 4);
-    dense_join<T, BM, BN>(pr.a[which], DenseSlots{pr.part, pr.groups}, pos, 16 * (blockIdx.x % (BM / 16)), i - 1, first,
-                          first + pr.ksteps[which], [&](int w) { return pr.step_of(w); });
+    const int64_t before = pr.step_of(i - 1);
+    if (at == first || before > first) return;
+    dense_join<T, BM, BN>(pr.a[which], DenseSlots{pr.part, pr.groups}, tile_pos(t, pr.tiles_m[which], pr.tiles_n[which], 4),
+                          kJoinRows * (blockIdx.x % (BM / kJoinRows)), i - 1,
+                          dense_from(first + pr.ksteps[which], pr.steps, pr.groups), before < first);
 }
 
 // Lets `kernel` have its tile's LDS.
@@ -423,7 +436,7 @@ void launch_dense_pair_tile(const DenseArgs& dx, const DenseArgs& dw, const Dens
     }
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(p.groups)), dim3(Tile::THREADS), Tile::LDS, st, pr);
     hipLaunchKernelGGL((k_dense_join_pair<T, Tile::BM, Tile::BN>),
-                       dim3(static_cast<unsigned>((p.groups - 1) * (Tile::BM / 16))), dim3(256), 0, st, pr);
+                       dim3(static_cast<unsigned>((p.groups - 1) * (Tile::BM / kJoinRows))), dim3(256), 0, st, pr);
 }
 
 // `kernel` over a product as the plan has it, and the join of what is shared.
@@ -441,7 +454,7 @@ void launch_dense_tile(const DenseArgs& a, const DensePlan& p, float* part, hipS
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(sh.groups)), dim3(Tile::THREADS), Tile::LDS, st, a, sh);
     if (sh.rest)
         hipLaunchKernelGGL((k_dense_join<T, Tile::BM, Tile::BN>),
-                           dim3(static_cast<unsigned>((sh.groups - 1) * (Tile::BM / 16))), dim3(256), 0, st, a, sh);
+                           dim3(static_cast<unsigned>(sh.rest * (Tile::BM / kJoinRows))), dim3(256), 0, st, a, sh);
 }
 
 }  // namespace nfq
