@@ -72,6 +72,22 @@ __device__ __forceinline__ void store8(T* p, int64_t left, const float (&v)[8]) 
     }
 }
 
+// The same past the caches, for results that no kernel reads soon: what the call
+// still reads keeps its place there (us: RMS norm with the residual 32768 x 256
+// fp32 25.9 -> 24.9, 16384 x 4096 bf16 into FP8 101.4 -> 98.5; clipping 1.3 GB 784
+// -> 746).
+template <typename T>
+__device__ __forceinline__ void store8_stream(T* p, int64_t left, const float (&v)[8]) {
+    if (left >= 8) {
+        typename Raw8<T>::vec q;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = from_f32<T>(v[e]);
+        __builtin_nontemporal_store(q, reinterpret_cast<typename Raw8<T>::vec*>(p));
+    } else {
+        store8(p, left, v);
+    }
+}
+
 // ---- 128-block scale ----------------------------------------------------------
 
 // Below this a block's codes would need a subnormal scale, whose inverse

@@ -241,7 +241,10 @@ struct DenseShare {
 // XCD (gemm_tile_of_block).
 template <typename F>
 __device__ __forceinline__ void dense_each(const DenseShare& sh, F f) {
-    const int i = gemm_tile_of_block(blockIdx.x, sh.groups, 8);
+    int i = gemm_tile_of_block(blockIdx.x, sh.groups, 8);
+    // Where every tile has as many workgroups, neighbours take the same steps of
+    // different tiles: an XCD then reads a run of k of both operands once.
+    if (sh.rest > 0 && sh.whole == 0 && sh.groups % sh.rest == 0) i = i % sh.rest * (sh.groups / sh.rest) + i / sh.rest;
     int64_t at = sh.rest ? sh.step_of(i) : 0;
     const int64_t end = sh.rest ? sh.step_of(i + 1) : 0;
     for (int n = 0; n < sh.whole || at < end; ++n) {

@@ -72,7 +72,7 @@ __global__ __launch_bounds__(row_threads<L>()) void k_rms(RmsArgs a, int64_t per
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
                     const int c = 8 * (t + L * j);
-                    store8(static_cast<T*>(a.sum) + m * a.ldsum + c, on ? D - c : 0, v[j]);
+                    store8_stream(static_cast<T*>(a.sum) + m * a.ldsum + c, on ? D - c : 0, v[j]);
                 }
             }
         }
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(row_threads<L>()) void k_rms(RmsArgs a, int64_t per
                 const float sc = blk_scale(max16(amax));
                 const v2u q8 = blk_codes8(v[j], blk_inverse(sc));
                 if (on && c / kBlk < kb) {
-                    *reinterpret_cast<v2u*>(a.codes + m * kb * kBlk + c) = q8;
+                    __builtin_nontemporal_store(q8, reinterpret_cast<v2u*>(a.codes + m * kb * kBlk + c));
                     if (t % 16 == 0) a.scales[c / kBlk * a.M + m] = sc;
                 }
             }
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(TH) void k_rms_grad(RmsGradArgs a) {
                     o[e] = rstd * __builtin_fmaf(-h[j][e], c2, g[j][e]);
                     if constexpr (ADD) o[e] += s[j][e];
                 }
-                store8(dt + c, D - c, o);
+                store8_stream(dt + c, D - c, o);
             }
         }
     }
