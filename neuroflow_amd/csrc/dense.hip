@@ -197,8 +197,12 @@ size_t product_space(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype)
 
 int product(const char* what, DenseForm form, const DenseArgs& a, int dtype, void* ws, hipStream_t st) {
     if (a.M == 0 || a.N == 0) return NFLOW_OK;
+    bool many = false;
     const DensePlan p = dense_plan(form, a.M, a.N, a.K, dtype);
     const bool b16 = dtype == NFLOW_DTYPE_BF16;
+    // A launch has at most 2^32 threads: 512 for each tile (of 64 x 64 or more) dealt out whole.
+    each_cut(dtype, [&](const Cut& c) { many |= c.kind == p.kind && !p.groups && c.tiles(a.M, a.N) > (1 << 23) - 1; });
+    if (many) return bad_arg(what, "too many results for one launch");
     if (p.kind == DENSE_FEW) {
         if (b16) launch_dense_few<bf16>(a, st);
         else launch_dense_few<float>(a, st);
@@ -233,7 +237,7 @@ int check_sizes(const char* what, int64_t M, int64_t N, int64_t K, int dtype) {
     if (M < 0 || N < 0 || K < 0) return bad_arg(what, "bad dims");
     if (!dtype_ok(dtype)) return bad_arg(what, "unknown dtype");
     const int64_t top = std::max(std::max(M, N), K);
-    if (K > NFLOW_DENSE_MAX_K || N > NFLOW_DENSE_MAX_K || top > INT64_C(1) << 40)
+    if (K > NFLOW_DENSE_MAX_K || N > NFLOW_DENSE_MAX_K || top > INT64_C(1) << 35)
         return bad_arg(what, "more than NFLOW_DENSE_MAX_K columns, or too many rows");
     auto many = [](int64_t m, int64_t n) { return ((m + 63) / 64) * ((n + 63) / 64) > INT32_MAX / 16; };
     if (many(M, N) || many(M, K) || many(N, K)) return bad_arg(what, "too many results for one launch");

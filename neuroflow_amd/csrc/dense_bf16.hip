@@ -25,22 +25,25 @@ void launch(const DenseArgs& a, const DensePlan& p, float* part, hipStream_t st)
 struct PackArgs {
     DensePack m[3];
     int64_t first[3];       // group of four rows of each matrix
+    int64_t groups;
 };
 __global__ __launch_bounds__(256) void k_dense_pack(PackArgs a) {
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int w = id < a.first[1] ? 0 : id < a.first[2] ? 1 : 2;
-    const DensePack& m = a.m[w];
-    const int64_t row = 4 * (id - a.first[w]), pitch = dense_pitch(m.cols);
-    const int64_t c = static_cast<int64_t>(blockIdx.y) * 512 + 8 * (threadIdx.x & 63);
-    if (row >= m.rows || c >= m.cols) return;
-    const bf16* from = static_cast<const bf16*>(m.from) + row * m.ld + c;
-    bf16* to = static_cast<bf16*>(m.to) + row * pitch + c;
-    Raw8<bf16> v[4];
+    int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (; id < a.groups; id += static_cast<int64_t>(gridDim.x) * 4) {
+        const int w = id < a.first[1] ? 0 : id < a.first[2] ? 1 : 2;
+        const DensePack& m = a.m[w];
+        const int64_t row = 4 * (id - a.first[w]), pitch = dense_pitch(m.cols);
+        const int64_t c = static_cast<int64_t>(blockIdx.y) * 512 + 8 * (threadIdx.x & 63);
+        if (c >= m.cols) continue;
+        const bf16* from = static_cast<const bf16*>(m.from) + row * m.ld + c;
+        bf16* to = static_cast<bf16*>(m.to) + row * pitch + c;
+        Raw8<bf16> v[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) dense_load(v[r], from + r * m.ld, row + r < m.rows ? m.cols - c : 0);
+        for (int r = 0; r < 4; ++r) dense_load(v[r], from + r * m.ld, row + r < m.rows ? m.cols - c : 0);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (row + r < m.rows) *reinterpret_cast<Raw8<bf16>::vec*>(to + r * pitch) = v[r].q;
+        for (int r = 0; r < 4; ++r)
+            if (row + r < m.rows) *reinterpret_cast<Raw8<bf16>::vec*>(to + r * pitch) = v[r].q;
+    }
 }
 
 }  // namespace
@@ -54,8 +57,9 @@ void launch_dense_pack(const DensePack (&m)[3], hipStream_t st) {
         a.first[i] = n;
         n += (m[i].rows + 3) / 4;
     }
-    hipLaunchKernelGGL(k_dense_pack, dim3(static_cast<unsigned>((n + 3) / 4), static_cast<unsigned>((cols + 511) / 512)),
-                       dim3(256), 0, st, a);
+    a.groups = n;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((n + 3) / 4, 1 << 20)), static_cast<unsigned>((cols + 511) / 512));
+    hipLaunchKernelGGL(k_dense_pack, grid, dim3(256), 0, st, a);
 }
 
 void launch_dense_bf16(const DenseArgs& a, DenseForm form, const DensePlan& p, float* part, hipStream_t st) {

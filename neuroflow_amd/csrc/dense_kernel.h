@@ -417,12 +417,16 @@ __global__ __launch_bounds__(256) void k_dense_join_pair(DensePair pr) {
                           dense_from(first + pr.ksteps[which], pr.steps, pr.groups), before < first);
 }
 
-// Lets `kernel` have its tile's LDS.
+// Lets `kernel` have its tile's LDS, once on every device.
 template <typename Tile, auto kernel>
 void dense_lds() {
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, Tile::LDS);
-    (void)once;
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return;
+    const uint64_t bit = uint64_t{1} << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return;
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, Tile::LDS);
+    done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 // dx and dW by `kernel`, and their join.

@@ -62,7 +62,7 @@ def test_forward(gpu, M, K, N, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("M,K,N", [(3, 50, 40), (70, 130, 90), (150, 64, 200), (700, 320, 384)])
+@pytest.mark.parametrize("M,K,N", [(3, 50, 40), (70, 130, 90), (150, 64, 200), (700, 320, 384), (150, 200, 136), (1000, 72, 520)])
 @pytest.mark.parametrize("extra", [(1, None, None), (None, 3, 1), (8, 8, 8), (5, 7, 9)])
 def test_strides(gpu, M, K, N, dtype, extra):
     """Rows apart at any element alignment, with NaN between them."""
@@ -196,11 +196,17 @@ def test_backward(gpu, M, K, N, dtype, kind):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("M,K,N", [(37, 50, 41), (300, 129, 250)])
+@pytest.mark.parametrize("M,K,N", [(37, 50, 41), (300, 129, 250), (203, 136, 200), (1003, 520, 72)])
 @pytest.mark.parametrize("extra", [(1, 3, 5), (8, 16, 8)])
-def test_backward_strides(gpu, M, K, N, dtype, extra):
+@pytest.mark.parametrize("apart", [2, 8])
+def test_backward_strides(gpu, M, K, N, dtype, extra, apart):
     x, W, _, pre = operands(M, K, N, dtype, 8, extra)
-    dy = rows(M, N, dtype, gen(9), 0.1, N + 2)
+    dy = rows(M, N, dtype, gen(9), 0.1, N + apart)
+    full, want_x, mag_x, want_w, mag_w = reference_backward(dy, x, W, "none", None, dtype)
+    dx, dW, db, _ = dense.linear_backward(dy, x, W)
+    within(dx, want_x, dense_bound(mag_x, N, dtype) + want_x.abs() * half(dtype) * 1.01 + 2.0 ** -133)
+    within(dW, want_w, dense_bound(mag_w, M, dtype) + want_w.abs() * half(dtype) * 1.01 + 2.0 ** -133)
+    within(db, full.sum(0), full.abs().sum(0) * (M / 8 + 300) * U)
     got = dense.linear_backward(dy, x, W, "gelu", pre=pre)
     want = dense.linear_backward(dy.contiguous(), x.contiguous(), W.contiguous(), "gelu", pre=pre.contiguous())
     assert all(torch.equal(a, b) for a, b in zip(got, want))
