@@ -74,7 +74,7 @@ int nflow_rms_norm_backward_workspace(int64_t M, int64_t D, size_t* bytes);
  * does.  y may be residual at the same row stride; y and pre may share no other
  * memory with an input or one another.  A bf16 operand x or W whose address, row
  * stride and row are not whole 16-byte groups is copied into the workspace first
- * (but for a few rows, M <= 32): `copies` asks for the room, if any may be such. */
+ * (where few rows do without: the function says): `copies` asks for the room, if any may be such. */
 int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* W, int64_t ldw,
                        int64_t N, const float* bias, const void* residual, int64_t ldr, int activation, void* y,
                        int64_t ldy, void* pre, int64_t ldpre, void* workspace, size_t workspace_bytes,

@@ -149,9 +149,26 @@ void each_cut(int dtype, F f) {
 }
 double steps_of(int64_t K) { return static_cast<double>((K + 63) / 64); }
 
+// A call of k_dense_few's, in us: a weight's pieces of 128 bytes, sixteen waves a CU,
+// or its way from HBM.
+double few_us(int64_t M, int64_t N, int64_t K, int dtype) {
+    const double bytes = static_cast<double>(K) * dtype_size(dtype), columns = std::ceil(static_cast<double>(N) / 16);
+    const double full = columns / num_cus(), pieces = std::ceil(bytes / 128) * std::ceil(full) / 16;
+    return 3.0 + std::max(N * bytes / 5e6, pieces * (0.95 + 0.5 * std::min(full, 1.0) + 0.052 * M));
+}
+
 DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype) {
-    if (form == DENSE_FORWARD && M <= kDenseFewRows) return DensePlan{DENSE_FEW, 0, 0, 0.0};
     const double cus = num_cus(), steps = steps_of(K);
+    // Few rows: the kernel for them unless the tiles' are estimated faster, for their
+    // call's launches or for the weight at the rate they read it, as they are with much
+    // to sum in few columns or a large weight.  Measured, us a call, few against tiles:
+    // bf16, one row of 4096 -> 4096 7.9 : 14.0, of 16384 -> 256 19.5 : 15.7; 32 rows of
+    // 1024 -> 4096 5.5 : 7.6, of 4096 -> 16384 52.7 : 34.0; fp32, 32 rows of 4096 -> 4096
+    // 26.3 : 41.9, of 4096 -> 256 24.4 : 16.5.
+    const bool rows_few = form == DENSE_FORWARD && M <= kDenseFewRows;
+    const double few = rows_few ? few_us(M, N, K, dtype) : HUGE_VAL;
+    const double read = static_cast<double>(N) * K / (dtype == NFLOW_DTYPE_F32 ? 0.5e6 : 2e6);
+    if (few <= std::max(4.0 + std::min(6.0, 0.2 * steps), read)) return DensePlan{DENSE_FEW, 0, 0, few};   // the least of tiles
     DensePlan best{DENSE_MID, 0, 0, HUGE_VAL};
     each_cut(dtype, [&](const Cut& c) {
         const double tiles = c.tiles(M, N), per = std::ceil(tiles / cus);
@@ -165,6 +182,7 @@ DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype)
             if (p.us < best.us) best = p;
         }
     });
+    if (rows_few && few <= std::max(best.us + (best.groups ? 7.0 : 4.0), read)) best = DensePlan{DENSE_FEW, 0, 0, few};
     return best;
 }
 
@@ -173,10 +191,10 @@ DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype)
 // 20000 x 256 x 768 118 against 136); else groups is 0.  In bf16, where the parts of
 // shared tiles weigh six times as much against the products, it is not (4096 x
 // 1024 x 1024 44 against 45, 65536 x 1024 x 1024 343 against 302).
-DensePlan pair_plan(int64_t M, int64_t N, int64_t K, int dtype) {
+DensePlan pair_plan(int64_t M, int64_t N, int64_t K, int dtype, const DensePlan& x, const DensePlan& w) {
     DensePlan best{DENSE_MID, 0, 0, 0.0};
     if (dtype != NFLOW_DTYPE_F32 || M <= 0 || N <= 0 || K <= 0) return best;
-    best.us = dense_plan(DENSE_DX, M, K, N, dtype).us + dense_plan(DENSE_DW, N, K, M, dtype).us + 3.0;
+    best.us = x.us + w.us + 3.0;
     for (const Cut& c : kCutsF32) {
         const double tx = c.tiles(M, K), tw = c.tiles(N, K), steps = tx * steps_of(N) + tw * steps_of(M);
         for (int occ = 1; occ <= c.per_cu; ++occ) {
@@ -191,14 +209,9 @@ DensePlan pair_plan(int64_t M, int64_t N, int64_t K, int dtype) {
     return best;
 }
 
-size_t product_space(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype) {
-    return M > 0 && N > 0 && K > 0 ? dense_plan(form, M, N, K, dtype).bytes : 0;
-}
-
-int product(const char* what, DenseForm form, const DenseArgs& a, int dtype, void* ws, hipStream_t st) {
+int product(const char* what, DenseForm form, const DensePlan& p, const DenseArgs& a, int dtype, void* ws, hipStream_t st) {
     if (a.M == 0 || a.N == 0) return NFLOW_OK;
     bool many = false;
-    const DensePlan p = dense_plan(form, a.M, a.N, a.K, dtype);
     const bool b16 = dtype == NFLOW_DTYPE_BF16;
     // A launch has at most 2^32 threads: 512 for each tile (of 64 x 64 or more) dealt out whole.
     each_cut(dtype, [&](const Cut& c) { many |= c.kind == p.kind && !p.groups && c.tiles(a.M, a.N) > (1 << 23) - 1; });
@@ -267,19 +280,30 @@ bool clash(const Span& a, const Span& b, size_t e) {
     return a.p && b.p && a.cols > 0 && rows_clash(a.p, a.ld, b.p, b.ld, a.rows, a.cols, e);
 }
 
-struct BackwardSpace {
-    size_t sums, x, w, both;
-    BackwardSpace(int64_t M, int64_t N, int64_t K, int dtype)
-        : sums(round16(static_cast<size_t>(M > 0 ? dz_runs(M, N) * N : 0) * sizeof(float))),
-          x(product_space(DENSE_DX, M, K, N, dtype)), w(product_space(DENSE_DW, N, K, M, dtype)),
-          both(pair_plan(M, N, K, dtype).bytes) {}
-    size_t bytes() const { return sums + std::max(x + w, both); }
+// What a call launches and the room it takes.
+struct ForwardPlan {
+    DensePlan p;
+    size_t parts = 0;
+    bool tiled = false;      // on operands that the DMA fetches
+    ForwardPlan(int64_t M, int64_t N, int64_t K, int dtype) : p(dense_plan(DENSE_FORWARD, M, N, K, dtype)) {
+        if (M == 0 || N == 0 || K == 0) return;
+        parts = p.bytes;
+        tiled = dtype == NFLOW_DTYPE_BF16 && p.kind != DENSE_FEW;
+    }
 };
-
-// Whether the forward product of these sizes is a tiled one of bf16.
-bool forward_copies(int64_t M, int64_t N, int64_t K, int dtype) {
-    return dtype == NFLOW_DTYPE_BF16 && M > 0 && N > 0 && K > 0 && dense_plan(DENSE_FORWARD, M, N, K, dtype).kind != DENSE_FEW;
-}
+struct BackwardPlan {
+    DensePlan x, w, pair;
+    size_t sums = 0, x_parts = 0, bytes;
+    BackwardPlan(int64_t M, int64_t N, int64_t K, int dtype)
+        : x(dense_plan(DENSE_DX, M, K, N, dtype)), w(dense_plan(DENSE_DW, N, K, M, dtype)),
+          pair(pair_plan(M, N, K, dtype, x, w)) {
+        if (M > 0) sums = round16(static_cast<size_t>(dz_runs(M, N) * N) * sizeof(float));
+        bytes = sums;
+        if (M == 0 || N == 0 || K == 0) return;
+        x_parts = x.bytes;
+        bytes += std::max(x.bytes + w.bytes, pair.bytes);
+    }
+};
 
 constexpr const char* kShared = "a result shares memory with an input or another result";
 
@@ -296,8 +320,8 @@ int nflow_dense_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, int
     if (!bytes) return bad_arg(what, "null output");
     *bytes = 0;
     if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
-    *bytes = product_space(DENSE_FORWARD, M, N, K, dtype);
-    if (copies && forward_copies(M, N, K, dtype)) *bytes += copy_space(M, K) + copy_space(N, K);
+    const ForwardPlan plan(M, N, K, dtype);
+    *bytes = plan.parts + (copies && plan.tiled ? copy_space(M, K) + copy_space(N, K) : 0);
     return NFLOW_OK;
 }
 
@@ -311,15 +335,15 @@ int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     if (int rc = check_act(what, activation)) return rc;
     if (ldx < K || ldw < K || ldy < N || (residual && ldr < N) || (pre && ldpre < N))
         return bad_arg(what, "row stride smaller than a row");
-    const size_t parts = product_space(DENSE_FORWARD, M, N, K, dtype);
+    const ForwardPlan plan(M, N, K, dtype);
     Copies copies;
     const void *px = x, *pw = W;
     int64_t lx = ldx, lw = ldw;
-    if (forward_copies(M, N, K, dtype)) {
-        copies.take(px, lx, M, K, static_cast<uint8_t*>(workspace) + parts);
-        copies.take(pw, lw, N, K, static_cast<uint8_t*>(workspace) + parts);
+    if (plan.tiled) {
+        copies.take(px, lx, M, K, static_cast<uint8_t*>(workspace) + plan.parts);
+        copies.take(pw, lw, N, K, static_cast<uint8_t*>(workspace) + plan.parts);
     }
-    if (int rc = check_workspace(what, workspace, workspace_bytes, parts + copies.bytes)) return rc;
+    if (int rc = check_workspace(what, workspace, workspace_bytes, plan.parts + copies.bytes)) return rc;
     if (M == 0 || N == 0) return NFLOW_OK;
     if (!y) return bad_arg(what, "null y");
     if (K > 0 && (!x || !W)) return bad_arg(what, "null x or W");
@@ -331,7 +355,7 @@ int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     hipStream_t st = as_stream(stream);
     if (copies.n) launch_dense_pack(copies.m, st);
     const DenseArgs a{px, pw, lx, lw, M, N, K, bias, residual, ldr, activation, y, ldy, pre, ldpre, nullptr};
-    return product(what, DENSE_FORWARD, a, dtype, workspace, st);
+    return product(what, DENSE_FORWARD, plan.p, a, dtype, workspace, st);
 }
 
 int nflow_dense_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, int copies, size_t* bytes) {
@@ -340,7 +364,7 @@ int nflow_dense_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int d
     if (!bytes) return bad_arg(what, "null output");
     *bytes = 0;
     if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
-    *bytes = BackwardSpace(M, N, K, dtype).bytes();
+    *bytes = BackwardPlan(M, N, K, dtype).bytes;
     if (copies && dtype == NFLOW_DTYPE_BF16) *bytes += copy_space(M, N) + copy_space(N, K) + copy_space(M, K);
     return NFLOW_OK;
 }
@@ -358,17 +382,17 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
     if (lddy < N || (dW && ldx < K) || (dx && ldw < K) || (act && (ldpre < N || lddz < N)) || (dx && lddx < K) ||
         (dW && lddw < K))
         return bad_arg(what, "row stride smaller than a row");
-    const BackwardSpace sp(M, N, K, dtype);
+    const BackwardPlan plan(M, N, K, dtype);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     Copies copies;
     const void *g = act ? dz : dy, *px = x, *pw = W;
     int64_t lg = act ? lddz : lddy, lx = ldx, lw = ldw;
     if (dtype == NFLOW_DTYPE_BF16 && M > 0 && N > 0 && K > 0) {
-        if (dx || dW) copies.take(g, lg, M, N, ws + sp.bytes());
-        if (dx) copies.take(pw, lw, N, K, ws + sp.bytes());
-        if (dW) copies.take(px, lx, M, K, ws + sp.bytes());
+        if (dx || dW) copies.take(g, lg, M, N, ws + plan.bytes);
+        if (dx) copies.take(pw, lw, N, K, ws + plan.bytes);
+        if (dW) copies.take(px, lx, M, K, ws + plan.bytes);
     }
-    if (int rc = check_workspace(what, workspace, workspace_bytes, sp.bytes() + copies.bytes)) return rc;
+    if (int rc = check_workspace(what, workspace, workspace_bytes, plan.bytes + copies.bytes)) return rc;
     if (M > 0 && N > 0) {
         if (!dy || (act && (!pre || !dz))) return bad_arg(what, "null dy, pre or dz");
         if (K > 0 && ((dx && !W) || (dW && !x))) return bad_arg(what, "null x or W");
@@ -401,14 +425,13 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
     if (K == 0) return NFLOW_OK;
     const DenseArgs ax{g, pw, lg, lw, M, K, N, nullptr, nullptr, 0, NFLOW_ACT_NONE, dx, lddx, nullptr, 0, nullptr};
     const DenseArgs aw{g, px, lg, lx, N, K, M, nullptr, nullptr, 0, NFLOW_ACT_NONE, dW, lddw, nullptr, 0, ride};
-    const DensePlan pair = pair_plan(M, N, K, dtype);
-    if (dx && dW && pair.groups) {
-        launch_dense_pair_f32(ax, aw, pair, reinterpret_cast<float*>(ws + sp.sums), st);
+    if (dx && dW && plan.pair.groups) {
+        launch_dense_pair_f32(ax, aw, plan.pair, reinterpret_cast<float*>(ws + plan.sums), st);
         return launch_status(what);
     }
     if (dx)
-        if (int rc = product(what, DENSE_DX, ax, dtype, ws + sp.sums, st)) return rc;
-    return dW ? product(what, DENSE_DW, aw, dtype, ws + sp.sums + sp.x, st) : NFLOW_OK;
+        if (int rc = product(what, DENSE_DX, plan.x, ax, dtype, ws + plan.sums, st)) return rc;
+    return dW ? product(what, DENSE_DW, plan.w, aw, dtype, ws + plan.sums + plan.x_parts, st) : NFLOW_OK;
 }
 
 int nflow_debug_dense_cut(int form, int64_t M, int64_t N, int64_t K, int dtype, int* kernel, int* groups) {
@@ -417,7 +440,7 @@ int nflow_debug_dense_cut(int form, int64_t M, int64_t N, int64_t K, int dtype, 
     if (!kernel || !groups) return bad_arg(what, "null output");
     if (form < 0 || form > 3) return bad_arg(what, "unknown form");
     if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
-    const DensePlan p = form == 3 ? pair_plan(M, N, K, dtype) : dense_plan(static_cast<DenseForm>(form), M, N, K, dtype);
+    const DensePlan p = form == 3 ? BackwardPlan(M, N, K, dtype).pair : dense_plan(static_cast<DenseForm>(form), M, N, K, dtype);
     *kernel = static_cast<int>(p.kind);
     *groups = p.groups;
     return NFLOW_OK;

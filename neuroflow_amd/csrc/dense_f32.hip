@@ -90,46 +90,46 @@ __device__ __forceinline__ void dense_f32_tile(const DenseArgs& a, const DenseSl
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wid / Tile::WN, wn = wid % Tile::WN;
     const int64_t m0 = pos.tm * Tile::BM, n0 = pos.tn * Tile::BN;
-            v4f acc[TI][TJ];
+    v4f acc[TI][TJ];
 #pragma unroll
-            for (int i = 0; i < TI; ++i)
+    for (int i = 0; i < TI; ++i)
 #pragma unroll
-                for (int j = 0; j < TJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            DenseStage<AX, Tile::BM, 32, Tile::THREADS> ra;
-            DenseStage<BX, Tile::BN, 32, Tile::THREADS> rb;
-            auto load = [&](int k) {
-                ra.load(static_cast<const float*>(a.A), a.lda, m0, a.M, static_cast<int64_t>(k) * 32, k < k1 ? a.K : 0);
-                rb.load(static_cast<const float*>(a.B), a.ldb, n0, a.N, static_cast<int64_t>(k) * 32, k < k1 ? a.K : 0);
-            };
-            auto store = [&](int s) {
-                ra.store(lds + s * Tile::STAGE);
-                rb.store(lds + s * Tile::STAGE + 3 * Tile::PLANE_A);
-            };
-            DenseSums<Tile> sums(AX && a.sums && pos.tn == 0, wn);
-            const int arow = 16 * TI * wm, brow = 16 * TJ * wn;
-            load(k0);
-            store(0);
-            load(k0 + 1);
-            __syncthreads();
-            int s = 0;
-            for (int k = k0; k < k1; ++k, s ^= 1) {
-                const uint8_t* st = lds + s * Tile::STAGE;
-                const StageProducts<AX, BX, Tile> stage(st, brow);
-                const bool first = wid < Tile::WAVES / 2;
-                if (first) {
-                    store(s ^ 1);
-                    load(k + 2);
-                }
-                stage.run(st, acc, sums, arow, 0, TI / 2);
-                if (!first) {
-                    store(s ^ 1);
-                    load(k + 2);
-                }
-                stage.run(st, acc, sums, arow, TI / 2, TI);
-                __syncthreads();
-            }
-            if constexpr (AX) sums.leave(a, sl, m0, slot, wm);
-            dense_leave<float, Tile>(a, sl, acc, reinterpret_cast<float*>(lds) + wid * Tile::STRIP, m0, n0, slot, wm, wn);
+        for (int j = 0; j < TJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    DenseStage<AX, Tile::BM, 32, Tile::THREADS> ra;
+    DenseStage<BX, Tile::BN, 32, Tile::THREADS> rb;
+    auto load = [&](int k) {
+        ra.load(static_cast<const float*>(a.A), a.lda, m0, a.M, static_cast<int64_t>(k) * 32, k < k1 ? a.K : 0);
+        rb.load(static_cast<const float*>(a.B), a.ldb, n0, a.N, static_cast<int64_t>(k) * 32, k < k1 ? a.K : 0);
+    };
+    auto store = [&](int s) {
+        ra.store(lds + s * Tile::STAGE);
+        rb.store(lds + s * Tile::STAGE + 3 * Tile::PLANE_A);
+    };
+    DenseSums<Tile> sums(AX && a.sums && pos.tn == 0, wn);
+    const int arow = 16 * TI * wm, brow = 16 * TJ * wn;
+    load(k0);
+    store(0);
+    load(k0 + 1);
+    __syncthreads();
+    int s = 0;
+    for (int k = k0; k < k1; ++k, s ^= 1) {
+        const uint8_t* st = lds + s * Tile::STAGE;
+        const StageProducts<AX, BX, Tile> stage(st, brow);
+        const bool first = wid < Tile::WAVES / 2;
+        if (first) {
+            store(s ^ 1);
+            load(k + 2);
+        }
+        stage.run(st, acc, sums, arow, 0, TI / 2);
+        if (!first) {
+            store(s ^ 1);
+            load(k + 2);
+        }
+        stage.run(st, acc, sums, arow, TI / 2, TI);
+        __syncthreads();
+    }
+    if constexpr (AX) sums.leave(a, sl, m0, slot, wm);
+    dense_leave<float, Tile>(a, sl, acc, reinterpret_cast<float*>(lds) + wid * Tile::STRIP, m0, n0, slot, wm, wn);
 }
 
 template <bool AX, bool BX, typename Tile>

@@ -29,6 +29,12 @@ struct RmsArgs {
 // The layout of k_norm: L threads hold a row, thread t the eight values from
 // column 8 (t + L j) on.  x and the residual are read once, the next row's while
 // this one is worked on; the sum of squares is about 0, so one reduction a row.
+// The norm is of t in fp32; what is stored as the sum is t rounded once.
+//
+// HBM bound.  32768 x 256 fp32 with residual and sum 22.6 us (134 MB, 5.9 TB/s:
+// part of it stays in the Infinity Cache), 16384 x 4096 bf16 to FP8 98 us (472 MB,
+// 4.8 TB/s; 19.5 VALU instructions a value, the VALU busy a third of the time).  The
+// sum goes past the caches (store8_stream): the next kernel reads y.
 template <typename T, bool FP8, bool RES, int L, int NV>
 __global__ __launch_bounds__(row_threads<L>()) void k_rms(RmsArgs a, int64_t per) {
     constexpr int G = row_threads<L>() / L;              // rows a workgroup holds
@@ -166,9 +172,15 @@ struct RmsGradArgs {
 };
 
 // ---- backward, rows in registers ---------------------------------------------------
-// The layout of k_norm_grad: dt needs one sum over the row, of g h; dweight is a
-// sum over rows of dy h, which every thread keeps for its columns over all of its
-// rows and a workgroup joins over its G rows in LDS at the end.
+// The layout of k_norm_grad: with h = t rstd and g = dy w, dt = rstd (g - h mean(g h))
+// + dsum needs one sum over the row; dweight is a sum over rows of dy h, which every
+// thread keeps for its columns over all of its rows and a workgroup joins over its
+// G rows in LDS at the end, and a second launch over the workgroups in their order.
+//
+// HBM bound: 16384 x 4096 bf16 with dsum 95 us (537 MB, 5.6 TB/s: three parts read
+// to one written) and 4.7 for the join of 256 partial rows.  AHEAD, the next row's
+// loads under this one's work, where its registers leave the occupancy: else the
+// workgroup's other waves hide them.
 template <typename T, bool ADD, int L, int NV, int TH, bool AHEAD>
 __global__ __launch_bounds__(TH) void k_rms_grad(RmsGradArgs a) {
     constexpr int G = TH / L, W = TH / 64;

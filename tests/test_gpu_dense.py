@@ -22,7 +22,7 @@ CUTS = [(33, 200, 4100), (33, 1025, 5003), (33, 2050, 3000), (33, 5003, 1537), (
 SIZES = [(1, 1, 1), (1, 4096, 4096), (2, 7, 3), (5, 100, 33), (16, 64, 16), (17, 200, 130), (33, 513, 64), (64, 31, 257),
          (65, 64, 64), (66, 1, 65), (100, 1000, 20), (129, 65, 127), (200, 2021, 301), (257, 128, 1000), (300, 8192, 136),
          (1000, 33, 1), (1537, 200, 1001), (2200, 96, 2056), (4099, 72, 2050), (2100, 2100, 40), (70, 2100, 2100),
-         (4096, 256, 4096)]
+         (4096, 256, 4096), (1, 16384, 100), (7, 16391, 65), (20, 8192, 1000)]
 
 
 def weight(N, K, dtype, g, stride=None):
