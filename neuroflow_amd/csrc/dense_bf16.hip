@@ -5,6 +5,10 @@
 namespace nfq {
 namespace {
 
+// A larger tile reads its operands fewer times and has more products to each LDS read,
+// a smaller one leaves fewer CUs idle; two workgroups a CU hide one's start and stores
+// under the other's products, four stages in LDS what one's loads take.  dense_plan
+// chooses by the time of a K step, measured with each.
 using Small = DenseTile<bf16, 2, 2, 2, 2, 3, 3>;    // 64 x 64, four waves, three workgroups a CU
 using Mid = DenseTile<bf16, 2, 2, 4, 4, 2>;         // 128 x 128, four waves, two workgroups a CU
 using Tall = DenseTile<bf16, 2, 2, 4, 2, 3>;        // 128 x 64, four waves, two workgroups a CU
@@ -21,7 +25,9 @@ void launch(const DenseArgs& a, const DensePlan& p, float* part, hipStream_t st)
 }
 
 // Up to three matrices copied to rows of dense_pitch(cols) values, zero past
-// cols: a wave takes 512 columns of four rows, 16 bytes a lane.
+// cols: a wave takes 512 columns of four rows, 16 bytes a lane.  Bound by a load's way
+// and a store's: 1537 x 2021 and 1001 x 2021 (21 MB in all) 9.3 us under a trace.  With
+// it the layer of these takes 31 us a call; by way of registers to LDS, without, 42.
 struct PackArgs {
     DensePack m[3];
     int64_t first[3];       // group of four rows of each matrix

@@ -1,5 +1,11 @@
 // dense_dma.h -- the tiled product of bf16 operands that the LDS-DMA can fetch:
 // 16-byte aligned, a whole number of 8 values in every row.
+//
+// Bound by the matrix cores and the clock they run at under load: 8192 x 8192 x
+// 8192 with bias and GELU 777 us (1415 TFLOP/s, MFMA 74% of the SIMD-cycles, VALU 28%,
+// LDS conflicts under 1%), a library product alone 685 to 718.  Over few K steps a
+// tile's start and stores weigh: dx of 65536 x 1024 x 1024, 16 steps, MFMA 41%; dW of
+// it, 128 workgroups' steps a tile, 52%.
 #pragma once
 
 #include "dense_kernel.h"

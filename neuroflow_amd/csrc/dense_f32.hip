@@ -6,6 +6,12 @@
 // of the bf16 rate, where the fp32 instruction has a sixteenth.  The planes are
 // formed once per workgroup, on the way from memory to LDS through registers, so
 // operands need no alignment and no launch ahead.
+//
+// Bound by forming the planes beside the products: 4096 x 4096 x 4096 620 us (222
+// TFLOP/s; the fp32 library's product 153), where six bf16 products at a library's 1350
+// TFLOP/s are 611.  Over fewer K steps a tile's start and stores weigh: 5003 x 1000 ->
+// 1544 backward, the pair of products 233 us under a trace, MFMA 40% of the SIMD-cycles,
+// VALU 46%; 32768 x 256 -> 256, eight steps of 32 a tile, 33 us a call, MFMA 25%, VALU 30%.
 #include "dense_kernel.h"
 #include "dense_split.h"
 
@@ -150,7 +156,9 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_f32_pair(Den
     });
 }
 
-using Small = DenseTile<float, 2, 2, 2, 2, 2>;     // 64 x 64, four waves, two workgroups a CU
+// As with bf16, larger tiles split each value fewer times: 256 x 128 once for 256 or 128
+// products, 64 x 64 once for 64 (4.8 us a step of 64 k's against 8 times 0.98).
+using Small = DenseTile<float, 2, 2, 2, 2, 2>;     // 64 x 64, four waves, up to three workgroups a CU
 using Mid = DenseTile<float, 2, 4, 4, 2, 2>;       // 128 x 128, eight waves, a workgroup a CU
 using Big = DenseTile<float, 4, 2, 4, 4, 2>;       // 256 x 128, eight waves, a workgroup a CU
 
