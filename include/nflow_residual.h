@@ -69,11 +69,12 @@ int nflow_rms_norm_backward_workspace(int64_t M, int64_t D, size_t* bytes);
  * activation, as in nflow_layer_forward_residual.  pre takes z, which the
  * backward pass of an activation needs.  bias, residual and pre may be NULL.
  * Sums are fp32; bf16 products are exact.  fp32 products are formed from three
- * bf16 parts of each operand, which hold it exactly, without the three smallest
- * of nine (2^-26 of a product); an infinite operand gives NaN there, as a NaN
- * does.  y may be residual at the same row stride; y and pre may share no other
+ * bf16 parts of each operand, which hold it exactly (below 2^-110 to 2^-134, half
+ * a step of bf16's subnormals), without the three smallest of nine (2^-26 of a
+ * product); an infinite operand gives NaN there, as a NaN does.  y may be residual at the same row stride; y and pre may share no other
  * memory with an input or one another.  A bf16 operand x or W whose address, row
- * stride and row are not whole 16-byte groups is copied into the workspace first
+ * stride and row are not whole 16-byte groups, or whose stride is
+ * NFLOW_DENSE_MAX_K or more, is copied into the workspace first
  * (where few rows do without: the function says): `copies` asks for the room, if any may be such. */
 int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* W, int64_t ldw,
                        int64_t N, const float* bias, const void* residual, int64_t ldr, int activation, void* y,

@@ -90,7 +90,7 @@ inline py::tuple rms_norm_backward(const Tensor& dy, const Tensor& x, const Mayb
 
 // Whether a bf16 operand may have to be copied (nflow_dense_linear).
 inline bool odd(const Tensor& t, const Matrix& m) {
-    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) != 0 || m.ld % 8 != 0 || m.cols % 8 != 0;
+    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) != 0 || m.ld % 8 != 0 || m.cols % 8 != 0 || m.ld >= NFLOW_DENSE_MAX_K;
 }
 
 // A weight (N, K) of x's type.

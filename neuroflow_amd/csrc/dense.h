@@ -47,7 +47,7 @@ void launch_dense_pair_f32(const DenseArgs& dx, const DenseArgs& dw, const Dense
 // A bf16 operand as the tiled product can fetch it: whole 16-byte groups at
 // 16-byte places, and a tile's rows within a buffer's range.
 inline bool dense_fetchable(const void* p, int64_t ld, int64_t cols) {
-    return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0 && ld < (INT64_C(1) << 21);
+    return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0 && ld < NFLOW_DENSE_MAX_K;
 }
 // Others are copied into rows of this many values.
 __host__ __device__ inline int64_t dense_pitch(int64_t cols) { return (cols + 7) / 8 * 8; }

@@ -6,7 +6,8 @@ x, W, the residual and the results are CUDA tensors of one type; x, the residual
 and dy are contiguous (leading axes are rows) or 2-D with a contiguous last axis
 and any row stride, W is (N, K).  bias and its gradient are float32.  Sums are
 fp32; float32 products are formed from three bfloat16 parts of each operand, to
-fp32 accuracy (an infinite operand gives NaN there).  A call runs on the current
+fp32 accuracy (an infinite operand gives NaN there, and one below 2^-110 is held to
+2^-134).  A call runs on the current
 stream of the current device, on which all of its tensors have to be; scratch
 comes from torch's allocator.  A wrong type raises TypeError, a wrong shape or
 device ValueError, a status of the library NflowError.  Nothing records an

@@ -159,6 +159,39 @@ def test_infinities_stay_in_their_rows(gpu, dtype, M):
     assert torch.equal(got[0], torch.full((3,), big * 0.5, device="cuda", dtype=dtype)) and not bool(got[1:].any())
 
 
+@pytest.mark.parametrize("M,K,N", [(1, 300, 50), (80, 256, 64), (600, 256, 512)])
+@pytest.mark.parametrize("exponent", [-112, -124, -130])
+def test_tiny_operands(gpu, M, K, N, exponent):
+    """fp32 operands whose last parts are subnormals of bf16, whose step is 2^-133:
+    each operand is off by at most half of it."""
+    g = gen(M)
+    x = torch.randn(M, K, generator=g, device="cuda") * 2.0 ** exponent
+    W = torch.randn(N, K, generator=g, device="cuda") * 2.0 ** 20
+    for a, b in ((x, W), (W, x)):
+        z, mag = product(a, b)
+        tiny = 2.0 ** -134 * (a.double().abs().sum(1)[:, None] + b.double().abs().sum(1)[None, :])
+        within(dense.linear(a, b), z, dense_bound(mag, K, torch.float32) + z.abs() * half(torch.float32) * 1.01 + tiny)
+
+
+@pytest.mark.parametrize("M", [1, 40])
+def test_rows_far_apart(gpu, M):
+    """Strides that the tiled product of bf16 does not take, in whole 16-byte groups,
+    and rows as long."""
+    g, apart = gen(M), 2 ** 21
+    x, W = (torch.zeros(n, apart, device="cuda", dtype=torch.bfloat16) for n in (M, 40))
+    for t in (x, W):
+        t[:, :64] = torch.randint(-8, 9, (len(t), 64), generator=g, device="cuda")
+    xd, Wd = x[:, :64].double(), W[:, :64].double()
+    want = (xd @ Wd.t()).to(torch.bfloat16)
+    assert torch.equal(dense.linear(x[:, :64], W[:, :64]), want)
+    assert torch.equal(dense.linear(x, W), want)
+    dy = torch.randint(-1, 2, (M, 40), generator=g, device="cuda").bfloat16()
+    for c in (64, apart):
+        dx, dW, _, _ = dense.linear_backward(dy, x[:, :c], W[:, :c])
+        assert torch.equal(dx[:, :64], (dy.double() @ Wd).to(torch.bfloat16)) and not bool(dx[:, 64:].any())
+        assert torch.equal(dW[:, :64], (dy.double().t() @ xd).to(torch.bfloat16)) and not bool(dW[:, 64:].any())
+
+
 def reference_backward(dy, x, W, kind, pre, dtype):
     """The formula's gradients with dz as the products take it (rounded), and
     their terms' magnitudes; dz before that."""
