@@ -24,10 +24,28 @@ void launch(const DenseArgs& a, const DensePlan& p, float* part, hipStream_t st)
     else launch_dense_tile<bf16, Small, &k_dense_dma<AX, BX, SUMS, Small>>(a, p, part, st);
 }
 
+// Eight values moved down by n, zeros after them.
+__device__ __forceinline__ Raw8<bf16>::vec values_down(const Raw8<bf16>::vec& v, int n) {
+    union {
+        Raw8<bf16>::vec v;
+        uint64_t u[2];
+    } x{v};
+    if (n >= 4) {
+        x.u[0] = x.u[1];
+        x.u[1] = 0;
+        n -= 4;
+    }
+    if (n > 0) {
+        x.u[0] = x.u[0] >> (16 * n) | x.u[1] << (64 - 16 * n);
+        x.u[1] >>= 16 * n;
+    }
+    return x.v;
+}
+
 // Up to three matrices copied to rows of dense_pitch(cols) values, zero past
 // cols: a wave takes 512 columns of four rows, 16 bytes a lane.  Bound by a load's way
-// and a store's: 1537 x 2021 and 1001 x 2021 (21 MB in all) 9.3 us under a trace.  With
-// it the layer of these takes 31 us a call; by way of registers to LDS, without, 42.
+// and a store's: 1537 x 2021 and 1001 x 2021 (21 MB in all) 9 us under a trace.  With
+// it the layer of these takes 30 us a call; by way of registers to LDS, without, 42.
 struct PackArgs {
     DensePack m[3];
     int64_t first[3];       // group of four rows of each matrix
@@ -43,12 +61,20 @@ __global__ __launch_bounds__(256) void k_dense_pack(PackArgs a) {
         if (c >= m.cols) continue;
         const bf16* from = static_cast<const bf16*>(m.from) + row * m.ld + c;
         bf16* to = static_cast<bf16*>(m.to) + row * pitch + c;
+        // The end of a row by the eight values that end there, moved down: one load as anywhere.
+        const int over = c + 8 > m.cols ? static_cast<int>(c + 8 - m.cols) : 0;
         Raw8<bf16> v[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) dense_load(v[r], from + r * m.ld, row + r < m.rows ? m.cols - c : 0);
+        for (int r = 0; r < 4; ++r) {
+            const int64_t at = row + r < m.rows ? r * m.ld : 0;
+            if (m.cols >= 8) v[r].load(from + at - over, 8);
+            else dense_load(v[r], from + at, m.cols - c);
+        }
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r) {
+            if (m.cols >= 8) v[r].q = values_down(v[r].q, over);
             if (row + r < m.rows) *reinterpret_cast<Raw8<bf16>::vec*>(to + r * pitch) = v[r].q;
+        }
     }
 }
 
