@@ -117,32 +117,37 @@ int64_t dz_runs(int64_t M, int64_t N) {
 // CU has ceil(tiles / CUs) of them.  Dealt out to `groups` workgroups, with the K
 // steps of what is left shared evenly, every CU is as busy as the next, for the
 // shared parts' way through the caches and a second launch.  Fitted to MI355X
-// times at 256 to 1024 tiles of 16 and 64 steps.
+// times at 256 to 1024 tiles of 16 and 64 steps.  `across`: a step of the backward
+// products to one of the forward's, in fp32, whose planes of operands across k go to
+// LDS and come from it in more pieces (us, by tiles of 64, 128 and 256: 1024 x 1024 x 1024
+// backward 62, 43, 43; 83 x 1536 x 1024 31, 26, 35; 64 x 1536 x 1024 22, 24, 36).
 struct Cut {
     DenseKind kind;
     int bm, bn, per_cu;
-    double alone, each, tile;
+    double alone, each, tile, across;
+    double step(DenseForm form, double per) const {
+        return (form == DENSE_FORWARD ? 1.0 : across) * std::max(alone, per * each);
+    }
     double tiles(int64_t M, int64_t N) const {
         return std::ceil(static_cast<double>(M) / bm) * std::ceil(static_cast<double>(N) / bn);
     }
-    // `steps` of 64 k's evenly dealt out to `occ` workgroups a CU, in `pieces` of tiles
-    // each, of which `parts` in all are shared.
-    DensePlan shared(int occ, double steps, double pieces, double parts) const {
-        const int groups = occ * num_cus();
+    // `steps` of 64 k's evenly dealt out to `groups` workgroups, `occ` a CU, in `pieces` of
+    // tiles each, of which `parts` in all are shared, `deep` to a tile.
+    DensePlan shared(DenseForm form, int occ, int groups, double steps, double pieces, double parts, double deep) const {
         const size_t slot = static_cast<size_t>(bm) * (bn + 1) * sizeof(float);
-        const double us = (steps / groups + 0.5) * std::max(alone, occ * each) + pieces * occ * tile + 3.0 +
-                          2 * parts * static_cast<double>(slot) / 5e6;
+        const double us = (steps / groups + 0.5) * step(form, occ) + pieces * occ * tile + 3.0 +
+                          2 * parts * static_cast<double>(slot) / 5e6 + 0.07 * deep;
         return DensePlan{kind, groups, round16(2 * groups * slot), us};
     }
 };
-const Cut kCutsBf16[] = {{DENSE_SMALL, 64, 64, 3, 0.233, 0.182, 0.7},
-                         {DENSE_TALL, 128, 64, 2, 0.294, 0.273, 1.2},
-                         {DENSE_MID, 128, 128, 2, 0.613, 0.435, 2.4},
-                         {DENSE_DEEP, 128, 128, 1, 0.481, 0.476, 2.6},
-                         {DENSE_BIG, 256, 256, 1, 1.43, 1.50, 5.3}};
-const Cut kCutsF32[] = {{DENSE_SMALL, 64, 64, 3, 0.98, 0.99, 0.7},
-                        {DENSE_MID, 128, 128, 1, 2.66, 2.66, 2.5},
-                        {DENSE_BIG, 256, 128, 1, 4.77, 4.77, 5.0}};
+const Cut kCutsBf16[] = {{DENSE_SMALL, 64, 64, 3, 0.233, 0.182, 0.7, 1.0},
+                         {DENSE_TALL, 128, 64, 2, 0.294, 0.273, 1.2, 1.0},
+                         {DENSE_MID, 128, 128, 2, 0.613, 0.435, 2.4, 1.0},
+                         {DENSE_DEEP, 128, 128, 1, 0.481, 0.476, 2.6, 1.0},
+                         {DENSE_BIG, 256, 256, 1, 1.43, 1.50, 5.3, 1.0}};
+const Cut kCutsF32[] = {{DENSE_SMALL, 64, 64, 3, 0.98, 0.99, 0.7, 2.5},
+                        {DENSE_MID, 128, 128, 1, 2.66, 2.66, 2.5, 1.12},
+                        {DENSE_BIG, 256, 128, 1, 4.77, 4.77, 5.0, 1.0}};
 template <typename F>
 void each_cut(int dtype, F f) {
     if (dtype == NFLOW_DTYPE_F32) {
@@ -176,14 +181,20 @@ DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype)
     DensePlan best{DENSE_MID, 0, 0, HUGE_VAL};
     each_cut(dtype, [&](const Cut& c) {
         const double tiles = c.tiles(M, N), per = std::ceil(tiles / cus);
-        const double us = steps * std::max(c.alone, per * c.each) + per * c.tile;
+        const double us = steps * c.step(form, per) + per * c.tile;
         if (us < best.us) best = DensePlan{c.kind, 0, 0, us};
         for (int occ = 1; occ <= c.per_cu; ++occ) {
-            const int groups = occ * num_cus();
-            const int64_t whole = static_cast<int64_t>(tiles) / groups, rest = static_cast<int64_t>(tiles) % groups;
-            if (rest == 0 || rest * steps < groups) continue;
-            const DensePlan p = c.shared(occ, tiles * steps, static_cast<double>(whole + 2), static_cast<double>(groups + rest));
-            if (p.us < best.us) best = p;
+            // Every workgroup that fits, or where there is little to share some steps to each.
+            for (int least = occ == 1 ? 8 : 1; least > 0; least /= 2) {
+                const double most = least == 1 ? occ * cus : std::floor(tiles * steps / least);
+                if (most > occ * cus || (least > 1 && most <= tiles)) continue;
+                const int groups = static_cast<int>(most);
+                const int64_t whole = static_cast<int64_t>(tiles) / groups, rest = static_cast<int64_t>(tiles) % groups;
+                if (rest == 0 || rest * steps < groups) continue;
+                const DensePlan p = c.shared(form, occ, groups, tiles * steps, static_cast<double>(whole + 2),
+                                             static_cast<double>(groups + rest), static_cast<double>(groups) / rest);
+                if (p.us < best.us) best = p;
+            }
         }
     });
     if (rows_few && few <= std::max(best.us + (best.groups ? 7.0 : 4.0), read)) best = DensePlan{DENSE_FEW, 0, 0, few};
@@ -202,11 +213,13 @@ DensePlan pair_plan(int64_t M, int64_t N, int64_t K, int dtype, const DensePlan&
     for (const Cut& c : kCutsF32) {
         const double tx = c.tiles(M, K), tw = c.tiles(N, K), steps = tx * steps_of(N) + tw * steps_of(M);
         for (int occ = 1; occ <= c.per_cu; ++occ) {
-            const double groups = occ * num_cus();
-            if (steps < 2 * groups) continue;
+            const int groups = static_cast<int>(std::min<double>(occ * num_cus(), std::floor(steps / 2)));
+            if (groups < 2 || (occ > 1 && groups <= num_cus())) continue;
             // Tiles of one length in whole rounds: none is shared.
             const bool even = steps_of(N) == steps_of(M) && std::fmod(tx + tw, groups) == 0.0;
-            const DensePlan p = c.shared(occ, steps, std::ceil((tx + tw) / groups) + (even ? 0 : 1), even ? 0 : 2 * groups);
+            const double deep = std::max(steps_of(N), steps_of(M)) * groups / steps;
+            const DensePlan p = c.shared(DENSE_DW, occ, groups, steps, std::ceil((tx + tw) / groups) + (even ? 0 : 1),
+                                         even ? 0 : 2.0 * groups, even ? 0 : deep);
             if (p.us < best.us) best = p;
         }
     }

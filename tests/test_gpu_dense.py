@@ -18,7 +18,9 @@ CUTS = [(33, 200, 4100), (33, 1025, 5003), (33, 2050, 3000), (33, 5003, 1537), (
         (200, 4100, 33), (200, 4100, 1300), (200, 8192, 1000), (257, 4100, 12000), (257, 12000, 4100), (1000, 1000, 1537),
         (1000, 1025, 4100), (1000, 4100, 1025), (1025, 33, 5003), (1025, 200, 3000), (1025, 3000, 200), (1025, 4100, 1000),
         (1025, 5003, 33), (1300, 200, 4100), (1537, 33, 5003), (1537, 5003, 33), (2050, 33, 3000), (2050, 3000, 33),
-        (3000, 257, 8192), (4100, 72, 72), (8192, 200, 1000), (12000, 4100, 257), (65536, 1000, 1000), (40000, 1280, 2000), (40000, 2000, 1280)]
+        (3000, 257, 8192), (4100, 72, 72), (8192, 200, 1000), (12000, 4100, 257), (65536, 1000, 1000), (40000, 1280, 2000), (40000, 2000, 1280),
+        (200, 4100, 2050), (200, 2050, 4100), (4100, 2050, 200),
+        (42, 64, 2792), (60, 512, 80), (64, 8192, 64), (495, 768, 118), (1000, 100, 100)]   # few steps to share
 SIZES = [(1, 1, 1), (1, 4096, 4096), (2, 7, 3), (5, 100, 33), (16, 64, 16), (17, 200, 130), (33, 513, 64), (64, 31, 257),
          (65, 64, 64), (66, 1, 65), (100, 1000, 20), (129, 65, 127), (200, 2021, 301), (257, 128, 1000), (300, 8192, 136),
          (1000, 33, 1), (1537, 200, 1001), (2200, 96, 2056), (4099, 72, 2050), (2100, 2100, 40), (70, 2100, 2100),
