@@ -314,7 +314,8 @@ struct DenseSums {
 
 // kJoinRows rows of a shared tile from row0 on: the sum of its slots, of
 // workgroups i .. stop - 1, and the epilogue.  `late`: the tile is the second that
-// workgroup i had a part of.  Bound by the slots' bytes, from the caches.
+// workgroup i had a part of.  Bound by the slots' bytes, from the caches, or their
+// latency: 128 slots of a tile of 64 x 64 13 us, where each waits for the last 40.
 constexpr int kJoinRows = 8;
 template <typename T, int BM, int BN>
 __device__ __forceinline__ void dense_join(const DenseArgs& a, const DenseSlots& sl, const TilePos& pos, int row0, int i,
@@ -322,26 +323,43 @@ __device__ __forceinline__ void dense_join(const DenseArgs& a, const DenseSlots&
     const int64_t m0 = pos.tm * BM + row0, n0 = pos.tn * BN;
     constexpr int Q = kJoinRows * BN / 4, TH = Q < 256 ? Q : 256, PER = Q / TH;   // groups of four values, threads, of each
     const bool sums = a.sums && pos.tn == 0 && threadIdx.x < kJoinRows;
+    auto slot_of = [&](int w) { return 2 * static_cast<int64_t>(w) + (w == i && late ? 1 : 0); };
     v4f z[PER];
-    float s = 0.0f;
 #pragma unroll
     for (int q = 0; q < PER; ++q) z[q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (static_cast<int>(threadIdx.x) < TH) {
-#pragma unroll 4
-        for (int w = i; w < stop; ++w) {
-            const int64_t slot = 2 * static_cast<int64_t>(w) + (w == i && late ? 1 : 0);
-            const float* p = sl.part + slot * BM * BN + row0 * BN;
+        // Many slots' loads at once, the last of them read again in place of those past it.
+        int w = i;
+        auto some = [&](auto many) {
+            constexpr int B = decltype(many)::value;
+            v4f v[B][PER];
 #pragma unroll
-            for (int q = 0; q < PER; ++q) z[q] += *reinterpret_cast<const v4f*>(p + 4 * (threadIdx.x + TH * q));
-            if (sums) s += sl.part[(2 * static_cast<int64_t>(sl.groups) * BN + slot) * BM + row0 + threadIdx.x];
-        }
+            for (int n = 0; n < B; ++n) {
+                const float* p = sl.part + slot_of(w + n < stop ? w + n : stop - 1) * BM * BN + row0 * BN;
+#pragma unroll
+                for (int q = 0; q < PER; ++q) v[n][q] = *reinterpret_cast<const v4f*>(p + 4 * (threadIdx.x + TH * q));
+            }
+#pragma unroll
+            for (int n = 0; n < B; ++n)
+#pragma unroll
+                for (int q = 0; q < PER; ++q)
+                    if (w + n < stop) z[q] += v[n][q];
+            w += B;
+        };
+        while (w + 16 / PER <= stop) some(std::integral_constant<int, 16 / PER>{});
+        while (w < stop) some(std::integral_constant<int, 4>{});
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
             const int e = 4 * (threadIdx.x + TH * q);
             if (m0 + e / BN < a.M) dense_finish<T>(a, m0 + e / BN, n0 + e % BN, z[q]);
         }
     }
-    if (sums && m0 + threadIdx.x < a.M) a.sums[m0 + threadIdx.x] = s;
+    if (!sums) return;
+    float s = 0.0f;
+#pragma unroll 16
+    for (int w = i; w < stop; ++w)
+        s += sl.part[(2 * static_cast<int64_t>(sl.groups) * BN + slot_of(w)) * BM + row0 + threadIdx.x];
+    if (m0 + threadIdx.x < a.M) a.sums[m0 + threadIdx.x] = s;
 }
 // The first workgroup, of `groups` that `steps` are dealt out to, that begins at
 // step `at` or past it.
