@@ -10,7 +10,7 @@
 // Bound by forming the planes beside the products: 4096 x 4096 x 4096 620 us (222
 // TFLOP/s; the fp32 library's product 153), where six bf16 products at a library's 1350
 // TFLOP/s are 611.  Over fewer K steps a tile's start and stores weigh: 5003 x 1000 ->
-// 1544 backward, the pair of products 233 us under a trace, MFMA 40% of the SIMD-cycles,
+// 1544 backward, the pair of products 202 us under a trace, MFMA 48% of the SIMD-cycles,
 // VALU 46%; 32768 x 256 -> 256, eight steps of 32 a tile, 33 us a call, MFMA 25%, VALU 30%.
 #include "dense_kernel.h"
 #include "dense_split.h"
