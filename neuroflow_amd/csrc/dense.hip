@@ -145,7 +145,7 @@ const Cut kCutsBf16[] = {{DENSE_SMALL, 64, 64, 3, 0.233, 0.182, 0.7, 1.0},
                          {DENSE_MID, 128, 128, 2, 0.613, 0.435, 2.4, 1.0},
                          {DENSE_DEEP, 128, 128, 1, 0.481, 0.476, 2.6, 1.0},
                          {DENSE_BIG, 256, 256, 1, 1.43, 1.50, 5.3, 1.0}};
-const Cut kCutsF32[] = {{DENSE_SMALL, 64, 64, 3, 0.98, 0.99, 0.7, 2.5},
+const Cut kCutsF32[] = {{DENSE_SMALL, 64, 64, 3, 1.45, 0.90, 1.0, 1.7},
                         {DENSE_MID, 128, 128, 1, 2.66, 2.66, 2.5, 1.12},
                         {DENSE_BIG, 256, 128, 1, 4.77, 4.77, 5.0, 1.0}};
 template <typename F>
