@@ -172,11 +172,11 @@ DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype)
     // call's launches or for the weight at the rate they read it, as they are with much
     // to sum in few columns or a large weight.  Measured, us a call, few against tiles:
     // bf16, one row of 4096 -> 4096 7.9 : 14.0, of 16384 -> 256 19.5 : 15.7; 32 rows of
-    // 1024 -> 4096 5.5 : 7.6, of 4096 -> 16384 52.7 : 34.0; fp32, 32 rows of 4096 -> 4096
-    // 26.3 : 41.9, of 4096 -> 256 24.4 : 16.5.
+    // 1024 -> 4096 5.5 : 7.6, of 4096 -> 16384 52.7 : 34.0; fp32, 16 rows of 4096 -> 4096
+    // 19.0 : 26.5, 32 of 4096 -> 256 24.4 : 11.6, of 16384 -> 4096 93.7 : 89.6.
     const bool rows_few = form == DENSE_FORWARD && M <= kDenseFewRows;
     const double few = rows_few ? few_us(M, N, K, dtype) : HUGE_VAL;
-    const double read = static_cast<double>(N) * K / (dtype == NFLOW_DTYPE_F32 ? 0.5e6 : 2e6);
+    const double read = static_cast<double>(N) * K / (dtype == NFLOW_DTYPE_F32 ? 0.75e6 : 2e6);
     if (few <= std::max(4.0 + std::min(6.0, 0.2 * steps), read)) return DensePlan{DENSE_FEW, 0, 0, few};   // the least of tiles
     DensePlan best{DENSE_MID, 0, 0, HUGE_VAL};
     each_cut(dtype, [&](const Cut& c) {

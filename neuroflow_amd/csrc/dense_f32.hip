@@ -157,7 +157,7 @@ __global__ __launch_bounds__(Tile::THREADS, Tile::OCC) void k_dense_f32_pair(Den
 }
 
 // As with bf16, larger tiles split each value fewer times: 256 x 128 once for 256 or 128
-// products, 64 x 64 once for 64 (4.8 us a step of 64 k's against 8 times 0.98).
+// products, 64 x 64 once for 64 (4.8 us a step of 64 k's against 8 times 0.9).
 using Small = DenseTile<float, 2, 2, 2, 2, 2>;     // 64 x 64, four waves, up to three workgroups a CU
 using Mid = DenseTile<float, 2, 4, 4, 2, 2>;       // 128 x 128, eight waves, a workgroup a CU
 using Big = DenseTile<float, 4, 2, 4, 4, 2>;       // 256 x 128, eight waves, a workgroup a CU
