@@ -41,5 +41,7 @@ CALLS = {
 
 @pytest.mark.parametrize("name", CALLS)
 def test_another_device_is_refused(name):
+    if torch.cuda.is_available() and torch.cuda.device_count() < 2:
+        pytest.skip("the second device has to exist where one does")
     with pytest.raises(ValueError, match="device|cuda:1"):
         CALLS[name]()
