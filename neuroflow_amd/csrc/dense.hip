@@ -421,7 +421,8 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
         if (meet(*in, sdx, e) || meet(*in, sdw, e)) return bad_arg(what, kShared);
     if (meet(sdx, sdw, e) || meet(sx, sdz, e) || meet(sw, sdz, e) || clash(sdy, sdz, e) || clash(spr, sdz, e))
         return bad_arg(what, kShared);
-    if ((M == 0 || N == 0 || !(act || dx)) && !dW && !dbias) return NFLOW_OK;
+    // Every result that is wanted is empty.  (dx of no columns of dz is not: zeros.)
+    if ((M == 0 || (N == 0 ? !dx : !(act || dx))) && !dW && !dbias) return NFLOW_OK;
     hipStream_t st = as_stream(stream);
     float* sums = reinterpret_cast<float*>(ws);
     const int64_t runs = dz_runs(M, N);
