@@ -25,6 +25,13 @@ struct RmsArgs {
     float* rstd;
 };
 
+// The first `left` of eight codes, zero past them.  The values there are 0 times
+// the row's rstd, which is a NaN or an infinity for some rows.
+__device__ __forceinline__ v2u codes_below(v2u q, int left) {
+    const uint64_t keep = left > 0 ? (uint64_t{1} << (8 * left)) - 1 : 0;
+    return v2u{q[0] & static_cast<uint32_t>(keep), q[1] & static_cast<uint32_t>(keep >> 32)};
+}
+
 // ---- rows in registers --------------------------------------------------------
 // The layout of k_norm: L threads hold a row, thread t the eight values from
 // column 8 (t + L j) on.  x and the residual are read once, the next row's while
@@ -103,7 +110,8 @@ __global__ __launch_bounds__(row_threads<L>()) void k_rms(RmsArgs a, int64_t per
 #pragma unroll
                 for (int e = 0; e < 8; ++e) amax = amax_of(amax, v[j][e]);
                 const float sc = blk_scale(max16(amax));
-                const v2u q8 = blk_codes8(v[j], blk_inverse(sc));
+                v2u q8 = blk_codes8(v[j], blk_inverse(sc));
+                if (D - c < 8) q8 = codes_below(q8, D - c);
                 if (on && c / kBlk < kb) {
                     __builtin_nontemporal_store(q8, reinterpret_cast<v2u*>(a.codes + m * kb * kBlk + c));
                     if (t % 16 == 0) a.scales[c / kBlk * a.M + m] = sc;
