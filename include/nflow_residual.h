@@ -70,9 +70,10 @@ int nflow_rms_norm_backward_workspace(int64_t M, int64_t D, size_t* bytes);
  * backward pass of an activation needs.  bias, residual and pre may be NULL.
  * Sums are fp32; bf16 products are exact.  fp32 products are formed from three
  * bf16 parts of each operand, which hold it exactly (below 2^-110 to 2^-134, half
- * a step of bf16's subnormals), without the three smallest of nine (2^-26 of a
- * product); an infinite operand gives NaN there, as a NaN does.  y may be residual at the same row stride; y and pre may share no other
- * memory with an input or one another.  A bf16 operand x or W whose address, row
+ * a step of bf16's subnormals), without the three smallest of nine (at most 2^-24 of
+ * a product, half a step of fp32); an infinite operand gives NaN there, as a NaN
+ * does, with ReLU too.  y may be residual at the same row stride; y and pre may
+ * share no other memory with an input or one another.  A bf16 operand x or W whose address, row
  * stride and row are not whole 16-byte groups, or whose stride is
  * NFLOW_DENSE_MAX_K or more, is copied into the workspace first
  * (where few rows do without: the function says): `copies` asks for the room, if any may be such. */

@@ -5,7 +5,7 @@
 // 8192 with bias and GELU 777 us (1415 TFLOP/s, MFMA 74% of the SIMD-cycles, VALU 28%,
 // LDS conflicts under 1%), a library product alone 685 to 718.  Over few K steps a
 // tile's start and stores weigh: dx of 65536 x 1024 x 1024, 16 steps, MFMA 41%; dW of
-// it, 128 workgroups' steps a tile, 52%.
+// it, whose 16 tiles 16 workgroups share each, 52%.
 #pragma once
 
 #include "dense_kernel.h"

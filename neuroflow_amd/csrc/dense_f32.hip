@@ -1,9 +1,10 @@
 // dense_f32.hip -- the tiled product of fp32 operands.
 //
 // An fp32 value is three bf16 planes, x = h + m + l: each the rest rounded to
-// bf16's 8 bits, so the 24 bits are held exactly, and six products (h h, h m, m h,
-// m m, h l, l h) leave out at most 2^-26 of the product: fp32 accuracy at a sixth
-// of the bf16 rate, where the fp32 instruction has a sixteenth.  The planes are
+// bf16's 8 bits, so the 24 bits are held exactly.  Six products (h h, h m, m h, m m,
+// h l, l h) leave out m l, l m and l l: of a value in [1, 2) |m| <= 2^-8 and |l| <=
+// 2^-17, so at most 2^-24 of the product, half a step of fp32.  That is fp32 accuracy at a
+// sixth of the bf16 rate, where the fp32 instruction has a sixteenth.  The planes are
 // formed once per workgroup, on the way from memory to LDS through registers, so
 // operands need no alignment and no launch ahead.
 //
