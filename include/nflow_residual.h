@@ -73,10 +73,11 @@ int nflow_rms_norm_backward_workspace(int64_t M, int64_t D, size_t* bytes);
  * a step of bf16's subnormals), without the three smallest of nine (at most 2^-24 of
  * a product, half a step of fp32); an infinite operand gives NaN there, as a NaN
  * does, with ReLU too.  y may be residual at the same row stride; y and pre may
- * share no other memory with an input or one another.  A bf16 operand x or W whose address, row
- * stride and row are not whole 16-byte groups, or whose stride is
- * NFLOW_DENSE_MAX_K or more, is copied into the workspace first
- * (where few rows do without: the function says): `copies` asks for the room, if any may be such. */
+ * share no other memory with an input or one another.  A bf16 operand x or W whose
+ * address, row stride and row are not whole 16-byte groups, or whose stride is
+ * NFLOW_DENSE_MAX_K or more, is copied into the workspace first, but for a call of few
+ * rows that is faster without.  `copies` asks for the room: 0 where neither is such, 2
+ * where those that are lie at addresses and strides of whole 4-byte words, else 1. */
 int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* W, int64_t ldw,
                        int64_t N, const float* bias, const void* residual, int64_t ldr, int activation, void* y,
                        int64_t ldy, void* pre, int64_t ldpre, void* workspace, size_t workspace_bytes,

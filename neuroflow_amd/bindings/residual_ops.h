@@ -88,10 +88,13 @@ inline py::tuple rms_norm_backward(const Tensor& dy, const Tensor& x, const Mayb
 
 // ---- the linear layer in bf16 or fp32 ----
 
-// Whether a bf16 operand may have to be copied (nflow_dense_linear).
-inline bool odd(const Tensor& t, const Matrix& m) {
-    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) != 0 || m.ld % 8 != 0 || m.cols % 8 != 0 || m.ld >= NFLOW_DENSE_MAX_K;
+// `copies` of nflow_dense_linear for a bf16 operand, and for two of them.
+inline int odd(const Tensor& t, const Matrix& m) {
+    const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    if ((at & 15) == 0 && m.ld % 8 == 0 && m.cols % 8 == 0 && m.ld < NFLOW_DENSE_MAX_K) return 0;
+    return (at & 3) == 0 && m.ld % 2 == 0 ? 2 : 1;
 }
+inline int odd(int a, int b) { return a == 1 || b == 1 ? 1 : a | b; }
 
 // A weight (N, K) of x's type.
 inline Matrix weight_of(const Tensor& W, const Tensor& x, int64_t cols, const char* of) {
@@ -130,7 +133,7 @@ inline py::tuple dense_linear(const Tensor& x, const Tensor& W, const Maybe& bia
     }
     if (return_pre) pre = empty(size, x, x.scalar_type());
     size_t n = 0;
-    ok(api.nflow_dense_linear_workspace(m.rows, N, m.cols, dt, odd(x, m) || odd(W, w), &n), "dense_linear");
+    ok(api.nflow_dense_linear_workspace(m.rows, N, m.cols, dt, odd(odd(x, m), odd(W, w)), &n), "dense_linear");
     const Tensor ws = scratch(n, x);
     ok(api.nflow_dense_linear(data(x), dt, m.rows, m.cols, m.ld, data(W), w.ld, N, b, residual ? data(*residual) : nullptr,
                               r.ld, act, data(y), yl.ld, data(pre), N, data(ws), n, stream_of(x)), "dense_linear");

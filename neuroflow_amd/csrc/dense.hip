@@ -158,26 +158,9 @@ void each_cut(int dtype, F f) {
 }
 double steps_of(int64_t K) { return static_cast<double>((K + 63) / 64); }
 
-// A call of k_dense_few's, in us: a weight's pieces of 128 bytes, sixteen waves a CU,
-// or its way from HBM.
-double few_us(int64_t M, int64_t N, int64_t K, int dtype) {
-    const double bytes = static_cast<double>(K) * dtype_size(dtype), columns = std::ceil(static_cast<double>(N) / 16);
-    const double full = columns / num_cus(), pieces = std::ceil(bytes / 128) * std::ceil(full) / 16;
-    return 3.0 + std::max(N * bytes / 5e6, pieces * (0.95 + 0.5 * std::min(full, 1.0) + 0.052 * M));
-}
-
-DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype) {
+// The least estimated time of tiles.
+DensePlan tiles_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype) {
     const double cus = num_cus(), steps = steps_of(K);
-    // Few rows: the kernel for them unless the tiles' are estimated faster, for their
-    // call's launches or for the weight at the rate they read it, as they are with much
-    // to sum in few columns or a large weight.  Measured, us a call, few against tiles:
-    // bf16, one row of 4096 -> 4096 7.9 : 14.0, of 16384 -> 256 19.5 : 15.7; 32 rows of
-    // 1024 -> 4096 5.5 : 7.6, of 4096 -> 16384 52.7 : 34.0; fp32, 16 rows of 4096 -> 4096
-    // 19.0 : 26.5, 32 of 4096 -> 256 24.4 : 11.6, of 16384 -> 4096 93.7 : 89.6.
-    const bool rows_few = form == DENSE_FORWARD && M <= kDenseFewRows;
-    const double few = rows_few ? few_us(M, N, K, dtype) : HUGE_VAL;
-    const double read = static_cast<double>(N) * K / (dtype == NFLOW_DTYPE_F32 ? 0.75e6 : 2e6);
-    if (few <= std::max(4.0 + std::min(6.0, 0.2 * steps), read)) return DensePlan{DENSE_FEW, 0, 0, few};   // the least of tiles
     DensePlan best{DENSE_MID, 0, 0, HUGE_VAL};
     each_cut(dtype, [&](const Cut& c) {
         const double tiles = c.tiles(M, N), per = std::ceil(tiles / cus);
@@ -197,8 +180,64 @@ DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype)
             }
         }
     });
-    if (rows_few && few <= std::max(best.us + (best.groups ? 7.0 : 4.0), read)) best = DensePlan{DENSE_FEW, 0, 0, few};
     return best;
+}
+
+// ---- few rows ----------------------------------------------------------------------------
+
+// How a bf16 operand's rows lie: as the tiles' DMA takes them, at whole 4-byte words or
+// at any element.  Of the latter two the tiles take copies; k_dense_few, which reads
+// operands in place, is held up by rows off whole words.  (fp32 operands: as the DMA
+// takes them, for all that it matters.)
+enum Lie { LIE_GROUPS, LIE_WORDS, LIE_ANY };
+Lie lie_of(const void* p, int64_t ld, int64_t cols, int dtype) {
+    if (dtype != NFLOW_DTYPE_BF16 || dense_fetchable(p, ld, cols)) return LIE_GROUPS;
+    return aligned(p, 4) && ld % 2 == 0 ? LIE_WORDS : LIE_ANY;
+}
+
+size_t copy_space(int64_t rows, int64_t cols) { return round16(static_cast<size_t>(rows * dense_pitch(cols)) * 2); }
+
+// x (M, K) and W (N, K) of a forward product, few rows of x.
+struct FewRows {
+    int64_t M, N, K;
+    int dtype;
+    // A call of k_dense_few's, in us: a weight's pieces of 128 bytes, sixteen waves a CU, or
+    // its way from HBM.  A piece waits for 16 rows of the weight and M of x, for each of
+    // x's 0.052 us in whole groups, 0.077 in words, 0.18 at any element.
+    double us(Lie x, Lie w) const {
+        const double bytes = static_cast<double>(K) * dtype_size(dtype), columns = std::ceil(static_cast<double>(N) / 16);
+        const double full = columns / num_cus(), pieces = std::ceil(bytes / 128) * std::ceil(full) / 16;
+        const double row = x == LIE_GROUPS ? 0.052 : x == LIE_WORDS ? 0.077 : 0.18;
+        const double weight = w == LIE_ANY ? 3.1 : 0.95 + 0.5 * std::min(full, 1.0);
+        return 3.0 + std::max(N * bytes / 5e6, pieces * (weight + row * M));
+    }
+    // The tiles' copies of what they cannot fetch: room, and us.
+    size_t copied(Lie x, Lie w) const { return (x ? copy_space(M, K) : 0) + (w ? copy_space(N, K) : 0); }
+    double copy_us(Lie x, Lie w) const { return x || w ? 3.3 + 2 * static_cast<double>(copied(x, w)) / 5e6 : 0.0; }
+    // Whether it is estimated faster than tiles whose call is estimated at `tiles` us: they
+    // gain with much to sum in few columns or with a large weight, by the rate that they read
+    // it at, and lose their copies.  Measured, us a call, few against tiles: bf16, one row
+    // of 4096 -> 4096 7.9 : 14.0, of 16384 -> 256 19.5 : 15.7; 32 rows of 1024 -> 4096 5.5 :
+    // 7.6, of 4096 -> 16384 52.7 : 34.0; of rows in words, 17 of 16382 -> 16384 185 : 367, 32 of
+    // 4094 -> 1024 13.7 : 17.4; at any element, one of 1023 -> 16384 15.7 : 22.5, 17 of 4095 ->
+    // 1024 27.9 : 17.4, 32 of 8191 -> 4096 75.9 : 43.1.  fp32, 16 rows of 4096 -> 4096
+    // 19.0 : 26.5, 32 of 4096 -> 256 24.4 : 11.6, of 16384 -> 4096 93.7 : 89.6.
+    bool faster(Lie x, Lie w, double tiles) const {
+        const double read = static_cast<double>(N) * K / (dtype == NFLOW_DTYPE_F32 ? 0.75e6 : 2e6);
+        return us(x, w) <= std::max(tiles, read) + copy_us(x, w);
+    }
+    // Tiles' calls: the least that any is, and a plan's.
+    double least() const { return 4.0 + std::min(6.0, 0.2 * steps_of(K)); }
+    static double call(const DensePlan& tiles) { return tiles.us + (tiles.groups ? 7.0 : 4.0); }
+};
+
+DensePlan dense_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype, Lie x = LIE_GROUPS, Lie w = LIE_GROUPS) {
+    if (form != DENSE_FORWARD || M > kDenseFewRows) return tiles_plan(form, M, N, K, dtype);
+    const FewRows f{M, N, K, dtype};
+    const DensePlan few{DENSE_FEW, 0, 0, f.us(x, w)};
+    if (f.faster(x, w, f.least())) return few;
+    const DensePlan tiles = tiles_plan(form, M, N, K, dtype);
+    return f.faster(x, w, FewRows::call(tiles)) ? few : tiles;
 }
 
 // dx (M, K) and dW (N, K) of fp32 in one launch, where that is faster than the two
@@ -244,8 +283,6 @@ int product(const char* what, DenseForm form, const DensePlan& p, const DenseArg
 }
 
 // ---- operands that the tiled product of bf16 cannot fetch where they lie ---------------------
-
-size_t copy_space(int64_t rows, int64_t cols) { return round16(static_cast<size_t>(rows * dense_pitch(cols)) * 2); }
 
 // Operands on their way into a product; those that need it are copied to `to`, all by one launch.
 struct Copies {
@@ -302,12 +339,30 @@ struct ForwardPlan {
     DensePlan p;
     size_t parts = 0;
     bool tiled = false;      // on operands that the DMA fetches
-    ForwardPlan(int64_t M, int64_t N, int64_t K, int dtype) : p(dense_plan(DENSE_FORWARD, M, N, K, dtype)) {
+    ForwardPlan(int64_t M, int64_t N, int64_t K, int dtype, Lie x, Lie w)
+        : p(dense_plan(DENSE_FORWARD, M, N, K, dtype, x, w)) {
         if (M == 0 || N == 0 || K == 0) return;
         parts = p.bytes;
         tiled = dtype == NFLOW_DTYPE_BF16 && p.kind != DENSE_FEW;
     }
 };
+// The room for x and W that both lie in groups, or the most that it is for what `copies` says.
+size_t forward_space(int64_t M, int64_t N, int64_t K, int dtype, int copies) {
+    if (M == 0 || N == 0 || K == 0) return 0;
+    if (!copies || dtype != NFLOW_DTYPE_BF16) return ForwardPlan(M, N, K, dtype, LIE_GROUPS, LIE_GROUPS).parts;
+    const FewRows f{M, N, K, dtype};
+    DensePlan tiles{DENSE_FEW, 0, 0, 0.0};
+    size_t bytes = 0;
+    for (Lie x : {LIE_GROUPS, LIE_WORDS, LIE_ANY})
+        for (Lie w : {LIE_GROUPS, LIE_WORDS, LIE_ANY}) {
+            if (copies == 2 && (x == LIE_ANY || w == LIE_ANY)) continue;
+            if (M <= kDenseFewRows && f.faster(x, w, f.least())) continue;
+            if (tiles.kind == DENSE_FEW) tiles = tiles_plan(DENSE_FORWARD, M, N, K, dtype);
+            if (M <= kDenseFewRows && f.faster(x, w, FewRows::call(tiles))) continue;
+            bytes = std::max(bytes, tiles.bytes + f.copied(x, w));
+        }
+    return bytes;
+}
 struct BackwardPlan {
     DensePlan x, w, pair;
     size_t sums = 0, x_parts = 0, bytes;
@@ -337,8 +392,7 @@ int nflow_dense_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, int
     if (!bytes) return bad_arg(what, "null output");
     *bytes = 0;
     if (int rc = check_sizes(what, M, N, K, dtype)) return rc;
-    const ForwardPlan plan(M, N, K, dtype);
-    *bytes = plan.parts + (copies && plan.tiled ? copy_space(M, K) + copy_space(N, K) : 0);
+    *bytes = forward_space(M, N, K, dtype, copies);
     return NFLOW_OK;
 }
 
@@ -352,7 +406,7 @@ int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     if (int rc = check_act(what, activation)) return rc;
     if (ldx < K || ldw < K || ldy < N || (residual && ldr < N) || (pre && ldpre < N))
         return bad_arg(what, "row stride smaller than a row");
-    const ForwardPlan plan(M, N, K, dtype);
+    const ForwardPlan plan(M, N, K, dtype, lie_of(x, ldx, K, dtype), lie_of(W, ldw, K, dtype));
     Copies copies;
     const void *px = x, *pw = W;
     int64_t lx = ldx, lw = ldw;
