@@ -13,7 +13,9 @@
  * be recorded into a HIP graph.  The same call on the same device gives the same
  * bits.  Activations are NFLOW_DTYPE_F32 or NFLOW_DTYPE_BF16; rows are
  * contiguous, ld* the elements from one row to the next, and rows need no
- * alignment beyond that of their elements.  There is no counterpart in the
+ * alignment beyond that of their elements.  Matrices that are columns of one buffer,
+ * at one row stride, share no memory; those of different strides are taken to where
+ * the memory that they span does.  There is no counterpart in the
  * reference, whose norm is a layer norm (cpp/src/fno.cpp:1418-1438) and whose
  * linear layers run on a CPU.
  */

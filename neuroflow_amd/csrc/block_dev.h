@@ -269,6 +269,30 @@ inline bool rows_clash(const void* a, int64_t lda, const void* b, int64_t ldb, i
     return off < row || off + row > step;
 }
 
+// The memory of `rows` rows of `cols` elements (of `size` bytes), `ld` elements apart;
+// of a vector the one row.
+struct Span {
+    intptr_t p;
+    int64_t rows, row, step;    // bytes of a row, and from one to the next
+    Span(const void* at, int64_t rows_, int64_t cols, int64_t ld, size_t size)
+        : p(reinterpret_cast<intptr_t>(at)), rows(rows_), row(cols * static_cast<int64_t>(size)),
+          step(ld * static_cast<int64_t>(size)) {}
+    Span(const void* at, int64_t n, size_t size) : Span(at, 1, n, n, size) {}
+    bool empty() const { return !p || rows <= 0 || row <= 0; }
+    intptr_t end() const { return p + (rows - 1) * step + row; }
+};
+// Whether two share memory.  A row, or rows at the other's stride, may lie between
+// the other's rows; rows of different strides are compared by the memory they span.
+inline bool meet(const Span& a, const Span& b) {
+    if (a.empty() || b.empty() || b.p >= a.end() || a.p >= b.end()) return false;
+    if (a.rows > 1 && b.rows > 1 && a.step != b.step) return true;
+    if (a.rows == 1 && b.rows == 1) return true;
+    const int64_t step = a.rows > 1 ? a.step : b.step, off = ((b.p - a.p) % step + step) % step;
+    return off < a.row || off + b.row > step;
+}
+
+inline constexpr const char* kShared = "a result shares memory with an input or another result";
+
 inline size_t round16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
 
 }  // namespace nfq

@@ -317,23 +317,6 @@ int check_act(const char* what, int act) {
     return NFLOW_OK;
 }
 
-// Whether the memory that two matrices span meets.
-struct Span {
-    const void* p;
-    int64_t rows, cols, ld;
-};
-bool meet(const Span& a, const Span& b, size_t e) {
-    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.cols <= 0 || b.cols <= 0) return false;
-    auto end = [e](const Span& s) {
-        return reinterpret_cast<uintptr_t>(s.p) + (static_cast<uintptr_t>(s.rows - 1) * s.ld + s.cols) * e;
-    };
-    return reinterpret_cast<uintptr_t>(a.p) < end(b) && reinterpret_cast<uintptr_t>(b.p) < end(a);
-}
-// The same, where lying in the same rows is allowed.
-bool clash(const Span& a, const Span& b, size_t e) {
-    return a.p && b.p && a.cols > 0 && rows_clash(a.p, a.ld, b.p, b.ld, a.rows, a.cols, e);
-}
-
 // What a call launches and the room it takes.
 struct ForwardPlan {
     DensePlan p;
@@ -377,8 +360,6 @@ struct BackwardPlan {
     }
 };
 
-constexpr const char* kShared = "a result shares memory with an input or another result";
-
 }  // namespace
 }  // namespace nfq
 
@@ -419,9 +400,9 @@ int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     if (!y) return bad_arg(what, "null y");
     if (K > 0 && (!x || !W)) return bad_arg(what, "null x or W");
     const size_t e = dtype_size(dtype);
-    const Span sx{x, M, K, ldx}, sw{W, N, K, ldw}, sr{residual, M, N, ldr}, sy{y, M, N, ldy}, sp{pre, M, N, ldpre};
-    if (meet(sx, sy, e) || meet(sw, sy, e) || meet(sx, sp, e) || meet(sw, sp, e) || meet(sy, sp, e) || meet(sr, sp, e) ||
-        clash(sr, sy, e))
+    const Span sx(x, M, K, ldx, e), sw(W, N, K, ldw, e), sr(residual, M, N, ldr, e), sy(y, M, N, ldy, e), sp(pre, M, N, ldpre, e);
+    if (meet(sx, sy) || meet(sw, sy) || meet(sx, sp) || meet(sw, sp) || meet(sy, sp) || meet(sr, sp) ||
+        (residual && rows_clash(residual, ldr, y, ldy, M, N, e)))
         return bad_arg(what, kShared);
     hipStream_t st = as_stream(stream);
     if (copies.n) launch_dense_pack(copies.m, st);
@@ -469,11 +450,12 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
         if (K > 0 && ((dx && !W) || (dW && !x))) return bad_arg(what, "null x or W");
     }
     const size_t e = dtype_size(dtype);
-    const Span sdy{dy, M, N, lddy}, spr{pre, M, N, ldpre}, sdz{dz, M, N, lddz}, sx{dW ? x : nullptr, M, K, ldx},
-        sw{dx ? W : nullptr, N, K, ldw}, sdx{dx, M, K, lddx}, sdw{dW, N, K, lddw};
-    for (const Span* in : {&sdy, &spr, &sdz, &sx, &sw})
-        if (meet(*in, sdx, e) || meet(*in, sdw, e)) return bad_arg(what, kShared);
-    if (meet(sdx, sdw, e) || meet(sx, sdz, e) || meet(sw, sdz, e) || clash(sdy, sdz, e) || clash(spr, sdz, e))
+    const Span sdz(dz, M, N, lddz, e), sx(dW ? x : nullptr, M, K, ldx, e), sw(dx ? W : nullptr, N, K, ldw, e),
+        sdx(dx, M, K, lddx, e), sdw(dW, N, K, lddw, e);
+    for (const Span& m : {sx, sw, sdz, Span(dy, M, N, lddy, e), Span(pre, M, N, ldpre, e)})
+        if (meet(m, sdx) || meet(m, sdw)) return bad_arg(what, kShared);
+    if (meet(sdx, sdw) || meet(sx, sdz) || meet(sw, sdz) ||
+        (act && N > 0 && (rows_clash(dy, lddy, dz, lddz, M, N, e) || rows_clash(pre, ldpre, dz, lddz, M, N, e))))
         return bad_arg(what, kShared);
     // Every result that is wanted is empty.  (dx of no columns of dz is not: zeros.)
     if ((M == 0 || (N == 0 ? !dx : !(act || dx))) && !dW && !dbias) return NFLOW_OK;
