@@ -53,8 +53,8 @@ int nflow_rms_norm_fp8(const void* x, int dtype, int64_t M, int64_t D, int64_t l
  *   dt = rstd * (g - h * mean_D(g * h)) + dsum,   dweight = sum_M(dy * h).
  * dt is the gradient of x and of residual alike; dsum (NULL: 0) is what t has
  * from its other use, the residual stream.  weight may be NULL (ones), dweight
- * (D) NULL (not wanted).  dt may be dy, t or dsum at the same row stride.
- * M = 0 gives zero dweight. */
+ * (D) NULL (not wanted).  dt may be dy, t or dsum at the same row stride; dt and
+ * dweight share no other memory with an input or one another.  M = 0 gives zero dweight. */
 int nflow_rms_norm_backward(const void* dy, const void* t, int dtype, int64_t M, int64_t D, int64_t lddy,
                             int64_t ldt, const float* weight, const float* rstd, const void* dsum, int64_t lddsum,
                             void* dt, int64_t lddt, float* dweight, void* workspace, size_t workspace_bytes,

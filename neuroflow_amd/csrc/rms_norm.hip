@@ -437,6 +437,13 @@ int check_rms(const char* what, const RmsArgs& a, int dtype, bool* run) {
     }
     if (a.y && a.sum && (a.y == a.sum || rows_clash(a.y, a.ldy, a.sum, a.ldsum, a.M, a.D, e)))
         return bad_arg(what, "y and sum overlap");
+    // What lies alone in memory, of which weight is an input.
+    const Span w(a.weight, a.D, sizeof(float)), rs(a.rstd, a.M, sizeof(float)), c(a.codes, a.M * blk_count(a.D) * kBlk, 1),
+        sc(a.scales, a.M * blk_count(a.D), sizeof(float));
+    const Span y(a.y, a.M, a.D, a.ldy, e), s(a.sum, a.M, a.D, a.ldsum, e);
+    for (const Span& m : {Span(a.x, a.M, a.D, a.ldx, e), Span(a.r, a.M, a.D, a.ldr, e), w, y, s})
+        if (meet(m, rs) || meet(m, c) || meet(m, sc)) return bad_arg(what, kShared);
+    if (meet(w, y) || meet(w, s) || meet(rs, c) || meet(rs, sc) || meet(c, sc)) return bad_arg(what, kShared);
     *run = true;
     return NFLOW_OK;
 }
@@ -511,6 +518,10 @@ int nflow_rms_norm_backward(const void* dy, const void* t, int dtype, int64_t M,
     if (rows_clash(dy, lddy, dt, lddt, M, D, e) || rows_clash(t, ldt, dt, lddt, M, D, e) ||
         (dsum && rows_clash(dsum, lddsum, dt, lddt, M, D, e)))
         return bad_arg(what, kOverlap);
+    const Span w(weight, D, sizeof(float)), rs(rstd, M, sizeof(float)), dw(dweight, D, sizeof(float)), d(dt, M, D, lddt, e);
+    for (const Span& m : {w, rs, d, Span(dy, M, D, lddy, e), Span(t, M, D, ldt, e), Span(dsum, M, D, lddsum, e)})
+        if (meet(m, dw)) return bad_arg(what, kShared);
+    if (meet(w, d) || meet(rs, d)) return bad_arg(what, kShared);
     if (int rc = check_workspace(what, workspace, workspace_bytes, rms_grad_space(M, D))) return rc;
     hipStream_t st = as_stream(stream);
     const int64_t nb = rms_grad_blocks(M);
