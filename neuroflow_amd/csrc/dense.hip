@@ -401,7 +401,10 @@ int nflow_dense_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     if (K > 0 && (!x || !W)) return bad_arg(what, "null x or W");
     const size_t e = dtype_size(dtype);
     const Span sx(x, M, K, ldx, e), sw(W, N, K, ldw, e), sr(residual, M, N, ldr, e), sy(y, M, N, ldy, e), sp(pre, M, N, ldpre, e);
-    if (meet(sx, sy) || meet(sw, sy) || meet(sx, sp) || meet(sw, sp) || meet(sy, sp) || meet(sr, sp) ||
+    const Span sb(bias, N, sizeof(float));
+    for (const Span& m : {sx, sw, sb})
+        if (meet(m, sy) || meet(m, sp)) return bad_arg(what, kShared);
+    if (meet(sy, sp) || meet(sr, sp) ||
         (residual && rows_clash(residual, ldr, y, ldy, M, N, e)))
         return bad_arg(what, kShared);
     hipStream_t st = as_stream(stream);
@@ -451,10 +454,10 @@ int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N,
     }
     const size_t e = dtype_size(dtype);
     const Span sdz(dz, M, N, lddz, e), sx(dW ? x : nullptr, M, K, ldx, e), sw(dx ? W : nullptr, N, K, ldw, e),
-        sdx(dx, M, K, lddx, e), sdw(dW, N, K, lddw, e);
+        sdx(dx, M, K, lddx, e), sdw(dW, N, K, lddw, e), sdb(dbias, N, sizeof(float));
     for (const Span& m : {sx, sw, sdz, Span(dy, M, N, lddy, e), Span(pre, M, N, ldpre, e)})
-        if (meet(m, sdx) || meet(m, sdw)) return bad_arg(what, kShared);
-    if (meet(sdx, sdw) || meet(sx, sdz) || meet(sw, sdz) ||
+        if (meet(m, sdx) || meet(m, sdw) || meet(m, sdb)) return bad_arg(what, kShared);
+    if (meet(sdx, sdw) || meet(sdx, sdb) || meet(sdw, sdb) || meet(sx, sdz) || meet(sw, sdz) ||
         (act && N > 0 && (rows_clash(dy, lddy, dz, lddz, M, N, e) || rows_clash(pre, ldpre, dz, lddz, M, N, e))))
         return bad_arg(what, kShared);
     // Every result that is wanted is empty.  (dx of no columns of dz is not: zeros.)

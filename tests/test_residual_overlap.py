@@ -44,6 +44,24 @@ def test_rms_norm_backward():
         refused("nflow_rms_norm_backward", [DY, T, 0, M, D, D, D, w, RS, DS, D, dt, D, dw, WS, n.value, None])
 
 
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("y,pre", [(W, S), (Y, W), (W + 4 * (N - 1), S), (Y, W - 8), (W - 2 * (M * N - 2), S)])
+def test_dense_linear(dtype, y, pre):
+    """The results and the bias."""
+    n = C.c_size_t()
+    assert _lib.lib().nflow_dense_linear_workspace(M, N, K, dtype, 1, C.byref(n)) == _lib.OK
+    refused("nflow_dense_linear", [X, dtype, M, K, K, R, K, N, W, None, 0, 2, y, N, pre, N, WS, n.value, None])
+
+
+def test_dense_linear_backward():
+    """dbias and everything else."""
+    n = C.c_size_t()
+    assert _lib.lib().nflow_dense_linear_backward_workspace(M, N, K, 0, 1, C.byref(n)) == _lib.OK
+    DY, PRE, DZ, DX, DW = S, RS, Y, CODES, SCALES
+    for db in (DY, X, R, PRE, DZ, DX, DW, DX + 4 * (M * K - 1), DW - 4 * (N - 1), X + 4 * K):
+        refused("nflow_dense_linear_backward", [DY, 0, M, N, N, X, K, R, K, K, 2, PRE, N, DZ, N, DX, K, DW, K, db, WS, n.value, None])
+
+
 def test_vectors_on_rows():
     """A vector in the gap between rows, one value too far in either direction."""
     ld = 3 * D
