@@ -121,8 +121,9 @@ int nflow_grad_norm(const nflow_grad_tensor* tensors, int count, float* norm, vo
 /* The same norm, and each gradient times min(1, max_norm / norm), the factor
  * rounded to fp32.  Where that is 1, gradients clipped in place are not touched.
  * A NaN in any gradient makes all of them NaN, an infinity makes finite ones 0
- * and itself NaN (their norm says so).  An out that is not its own grad shares
- * no memory with any gradient or other out. */
+ * and itself NaN (their norm says so); with an infinite max_norm and no NaN
+ * all are left as they are.  An out that is not its own grad, and norm, share no memory with any
+ * gradient or other out. */
 int nflow_grad_clip(const nflow_grad_tensor* tensors, int count, float max_norm, float* norm, void* workspace,
                     size_t workspace_bytes, void* stream);
 

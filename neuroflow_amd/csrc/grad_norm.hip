@@ -191,15 +191,17 @@ int check_grads(const char* what, const nflow_grad_tensor* tensors, int count, b
     return NFLOW_OK;
 }
 
-// Whether memory that is written shares a byte with another tensor's, or an out
-// with its own grad in another way than as the same memory: by their places in order.
-bool tangled(const nflow_grad_tensor* tensors, int count) {
-    struct Span {
+// Whether memory that is written (outs and the norm) shares a byte with another
+// tensor's, or an out with its own grad in another way than as the same memory: by
+// their places in order.
+bool tangled(const nflow_grad_tensor* tensors, int count, const float* norm) {
+    struct Bytes {
         uintptr_t from, to;
         bool written;
     };
-    std::vector<Span> spans;
-    spans.reserve(2 * static_cast<size_t>(count));
+    std::vector<Bytes> spans;
+    spans.reserve(2 * static_cast<size_t>(count) + 1);
+    spans.push_back({reinterpret_cast<uintptr_t>(norm), reinterpret_cast<uintptr_t>(norm) + sizeof(float), true});
     for (int i = 0; i < count; ++i) {
         const nflow_grad_tensor& t = tensors[i];
         const uintptr_t n = static_cast<uintptr_t>(t.count) * dtype_size(t.dtype);
@@ -208,9 +210,9 @@ bool tangled(const nflow_grad_tensor* tensors, int count) {
         spans.push_back({o, o + n, true});
         if (o != g) spans.push_back({g, g + n, false});
     }
-    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+    std::sort(spans.begin(), spans.end(), [](const Bytes& a, const Bytes& b) { return a.from < b.from; });
     uintptr_t any = 0, written = 0;                 // ends of what came before
-    for (const Span& s : spans) {
+    for (const Bytes& s : spans) {
         if (s.from < (s.written ? any : written)) return true;
         any = std::max(any, s.to);
         if (s.written) written = std::max(written, s.to);
@@ -291,7 +293,7 @@ int nflow_grad_clip(const nflow_grad_tensor* tensors, int count, float max_norm,
         if (tensors[i].count > 0 && !tensors[i].out) return bad_arg(what, "null out");
     if (int rc = check_workspace(what, workspace, workspace_bytes, grad_space(count))) return rc;
     try {
-        if (tangled(tensors, count)) return bad_arg(what, "an out overlaps a gradient or another out");
+        if (tangled(tensors, count, norm)) return bad_arg(what, "an out or the norm overlaps a gradient or another out");
     } catch (const std::exception& e) {
         return set_error(NFLOW_INTERNAL, std::string(what) + ": " + e.what());
     }

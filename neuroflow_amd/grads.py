@@ -25,5 +25,6 @@ def clip_by_global_norm(grads: Sequence[torch.Tensor], max_norm: float,
                         out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Multiplies every gradient by min(1, max_norm / norm), in place or into the
     tensors of out, and returns the norm.  A NaN in any gradient makes all of them
-    NaN, an infinity makes the finite ones 0: the norm, NaN or infinite, tells."""
+    NaN, an infinity makes the finite ones 0: the norm, NaN or infinite, tells.  With
+    an infinite max_norm and no NaN all are left as they are."""
     return _ops().clip_by_global_norm(list(grads), float(max_norm), None if out is None else list(out))

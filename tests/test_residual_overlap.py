@@ -62,6 +62,15 @@ def test_dense_linear_backward():
         refused("nflow_dense_linear_backward", [DY, 0, M, N, N, X, K, R, K, K, 2, PRE, N, DZ, N, DX, K, DW, K, db, WS, n.value, None])
 
 
+@pytest.mark.parametrize("norm", [X, X + 396, X - 2, Y, Y + 396, S + 2])
+def test_grad_clip(norm):
+    """The norm and a gradient in place, another's out, and a bf16 one."""
+    n = C.c_size_t()
+    assert _lib.lib().nflow_grad_workspace(3, C.byref(n)) == _lib.OK
+    t = (_lib.GradTensorC * 3)(*(_lib.GradTensorC(*v) for v in ((X, X, 100, 0), (R, Y, 100, 0), (S, S, 2, 1))))
+    refused("nflow_grad_clip", [t, 3, 1.0, norm, WS, n.value, None], b"overlaps")
+
+
 def test_vectors_on_rows():
     """A vector in the gap between rows, one value too far in either direction."""
     ld = 3 * D
