@@ -35,7 +35,8 @@ extern "C" {
 
 /* t = x + residual (fp32; residual NULL: t = x), rstd = 1 / sqrt(mean_D(t^2) +
  * eps), y = t * rstd * weight over the D columns of each of M rows.  The norm is
- * of t before its rounding.  sum, of x's type, takes the rounded t; it is
+ * of t before its rounding; its squares are summed in fp32, so a row whose sum of
+ * them is past fp32's range (values from 1.8e19 on) has rstd 0.  sum, of x's type, takes the rounded t; it is
  * wanted only with a residual and may be NULL, as weight (ones) and rstd (M)
  * may.  sum and y may each be x or residual at the same row stride, but not one
  * another; memory shared in any other way is refused. */
@@ -90,7 +91,8 @@ int nflow_dense_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, int
  *   dz = dy * act'(pre) (M, N), the gradient of residual too,
  *   dx (M, K) = dz W,  dW (N, K) = dz^T x,  dbias (N, fp32) = the sum of dz's rows.
  * dz, dx and dW are of dy's type, and the products take dz as it is returned;
- * dbias sums it ahead of its rounding.  With no activation dz is dy and both
+ * dbias sums it ahead of its rounding.  In fp32 the products, and with no activation
+ * dbias too, are of three parts of each operand, as above.  With no activation dz is dy and both
  * dz and pre are NULL; with one both are required (for ReLU pre may be y).  dx,
  * dW and dbias may each be NULL (not wanted).  M = 0 gives zero dW and dbias.
  * dz may be dy or pre at the same row stride; results share no other memory
@@ -132,7 +134,8 @@ int nflow_grad_workspace(int count, size_t* bytes);
 
 /* ---- for tests: which kernel a size takes (no GPU needed: 256 CUs without one) ---- */
 
-/* The kernel of the linear layer's product at this size: 0 the few-row one, else
+/* The kernel of the linear layer's product at this size, of operands in whole 16-byte
+ * groups: 0 the few-row one, else
  * tiles of 64 x 64 (1), 128 x 64 (2, bf16), 128 x 128 (3; 4 the same with its loads
  * further ahead, bf16) or 256 x 256 (5; fp32 256 x 128); and the workgroups that
  * tiles' K steps are dealt out to, or 0 where tiles stay whole.  form: 0 forward,

@@ -35,6 +35,13 @@ __device__ __forceinline__ float act_grad(float dy, float z, int act) {
 // HBM bound beside the slope's VALU work: 65536 x 1024 bf16 with GELU 80 us (403 MB, 5.0
 // TB/s, VALU 58%).  A pass of its own: dx and dW both read dz, at tiles of 256 four
 // times each, and the slope would be taken at every read.
+//
+// dz is rounded to the activations' type, and the products take it as it is returned.
+// In bf16 that is a second rounding of half a step beside dx's and dW's own: in the
+// 2-norm they are 2.3e-3 from the formula, where a dz kept in fp32 leaves 1.7e-3.  The
+// rest of it would be a second bf16 operand, and both products (280 of the 345 us of
+// 65536 x 1024 -> 1024) twice the work.  dbias, which costs nothing more, sums dz
+// ahead of the rounding.
 constexpr int kDzCols = 256, kDzRows = 8;            // of a workgroup at a time
 struct DzArgs {
     const void* dy;
@@ -116,8 +123,12 @@ int64_t dz_runs(int64_t M, int64_t N) {
 // `tile` for what a tile does outside its K loop.  Dealt out whole, the busiest
 // CU has ceil(tiles / CUs) of them.  Dealt out to `groups` workgroups, with the K
 // steps of what is left shared evenly, every CU is as busy as the next, for the
-// shared parts' way through the caches and a second launch.  Fitted to MI355X
-// times at 256 to 1024 tiles of 16 and 64 steps.  `across`: a step of the backward
+// shared parts' way through the caches and a second launch.  The times rank the
+// cuts of one product; as times they are low where few steps leave a tile's first
+// loads and stores bare (a product of 1537 x 2021 -> 1001 10.6 us for the 22.5 of a
+// trace, dx of 65536 x 1024 -> 1024 117 for 139 to 154, 32768 x 256 -> 256 in fp32 24 for
+// 37.5).  They are those of steps at 256 to 1024 tiles of 16 and 64 steps, but for fp32
+// tiles of 64: 69 x 4864 -> 2688 and 1024 x 2048 -> 1024.  `across`: a step of the backward
 // products to one of the forward's, in fp32, whose planes of operands across k go to
 // LDS and come from it in more pieces (us, by tiles of 64, 128 and 256: 1024 x 1024 x 1024
 // backward 62, 43, 43; 83 x 1536 x 1024 31, 26, 35; 64 x 1536 x 1024 22, 24, 36).
@@ -132,7 +143,8 @@ struct Cut {
         return std::ceil(static_cast<double>(M) / bm) * std::ceil(static_cast<double>(N) / bn);
     }
     // `steps` of 64 k's evenly dealt out to `groups` workgroups, `occ` a CU, in `pieces` of
-    // tiles each, of which `parts` in all are shared, `deep` to a tile.
+    // tiles each, of which `parts` in all are shared, `deep` to a tile: a join of 32, 64 and
+    // 128 slots of 64 x 64 takes 5.0, 7.8 and 12.5 us.
     DensePlan shared(DenseForm form, int occ, int groups, double steps, double pieces, double parts, double deep) const {
         const size_t slot = static_cast<size_t>(bm) * (bn + 1) * sizeof(float);
         const double us = (steps / groups + 0.5) * step(form, occ) + pieces * occ * tile + 3.0 +
@@ -167,7 +179,9 @@ DensePlan tiles_plan(DenseForm form, int64_t M, int64_t N, int64_t K, int dtype)
         const double us = steps * c.step(form, per) + per * c.tile;
         if (us < best.us) best = DensePlan{c.kind, 0, 0, us};
         for (int occ = 1; occ <= c.per_cu; ++occ) {
-            // Every workgroup that fits, or where there is little to share some steps to each.
+            // Every workgroup that fits, or where there is little to share 8, 4 or 2 steps to
+            // each: fewer parts to join (us, every workgroup against those: 64 x 8192 -> 64 bf16 31 : 9.6,
+            // 42 x 64 -> 2792 fp32 backward 84 : 18).
             for (int least = occ == 1 ? 8 : 1; least > 0; least /= 2) {
                 const double most = least == 1 ? occ * cus : std::floor(tiles * steps / least);
                 if (most > occ * cus || (least > 1 && most <= tiles)) continue;

@@ -8,7 +8,7 @@ namespace nfq {
 // Eight fp32 values as planes h + m + l, each the rest rounded to bf16: exact from
 // 2^-110 on; below, l's rounding to a bf16 subnormal leaves out up to 2^-134.  A value
 // that would round to infinity keeps bf16's largest as its first plane; of an
-// infinity or a NaN the third is NaN.
+// infinity or a NaN the third is NaN, and so is what it is multiplied or summed into.
 __device__ __forceinline__ void dense_split(const float (&v)[8], v8bf (&p)[3]) {
     constexpr float top = 0x1.fep127f;
 #pragma unroll
