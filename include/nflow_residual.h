@@ -36,10 +36,11 @@ extern "C" {
 /* t = x + residual (fp32; residual NULL: t = x), rstd = 1 / sqrt(mean_D(t^2) +
  * eps), y = t * rstd * weight over the D columns of each of M rows.  The norm is
  * of t before its rounding; its squares are summed in fp32, so a row whose sum of
- * them is past fp32's range (values from 1.8e19 on) has rstd 0.  sum, of x's type, takes the rounded t; it is
- * wanted only with a residual and may be NULL, as weight (ones) and rstd (M)
- * may.  sum and y may each be x or residual at the same row stride, but not one
- * another; memory shared in any other way is refused. */
+ * them is past fp32's range (values from 1.8e19 on) has rstd 0.  sum, of x's type,
+ * takes the rounded t; it is wanted only with a residual and may be NULL, as weight
+ * (ones) and rstd (M) may.  sum and y may each be x or residual at the same row
+ * stride, but not one another; memory that a result shares in any other way is
+ * refused. */
 int nflow_rms_norm_forward(const void* x, int dtype, int64_t M, int64_t D, int64_t ldx, const void* residual,
                            int64_t ldr, const float* weight, float eps, void* y, int64_t ldy, void* sum,
                            int64_t ldsum, float* rstd, void* stream);
@@ -55,7 +56,8 @@ int nflow_rms_norm_fp8(const void* x, int dtype, int64_t M, int64_t D, int64_t l
  * dt is the gradient of x and of residual alike; dsum (NULL: 0) is what t has
  * from its other use, the residual stream.  weight may be NULL (ones), dweight
  * (D) NULL (not wanted).  dt may be dy, t or dsum at the same row stride; dt and
- * dweight share no other memory with an input or one another.  M = 0 gives zero dweight. */
+ * dweight share no other memory with an input or one another.  M = 0 gives zero
+ * dweight. */
 int nflow_rms_norm_backward(const void* dy, const void* t, int dtype, int64_t M, int64_t D, int64_t lddy,
                             int64_t ldt, const float* weight, const float* rstd, const void* dsum, int64_t lddsum,
                             void* dt, int64_t lddt, float* dweight, void* workspace, size_t workspace_bytes,
@@ -92,9 +94,10 @@ int nflow_dense_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, int
  *   dx (M, K) = dz W,  dW (N, K) = dz^T x,  dbias (N, fp32) = the sum of dz's rows.
  * dz, dx and dW are of dy's type, and the products take dz as it is returned;
  * dbias sums it ahead of its rounding.  In fp32 the products, and with no activation
- * dbias too, are of three parts of each operand, as above.  With no activation dz is dy and both
- * dz and pre are NULL; with one both are required (for ReLU pre may be y).  dx,
- * dW and dbias may each be NULL (not wanted).  M = 0 gives zero dW and dbias.
+ * dbias too, are of three parts of each operand, as above.  With no activation dz is
+ * dy and both dz and pre are NULL; with one both are required (for ReLU pre may be
+ * y).  dx, dW and dbias may each be NULL (not wanted).  M = 0 gives zero dW and
+ * dbias, N = 0 zero dx.
  * dz may be dy or pre at the same row stride; results share no other memory
  * with an input or one another.  `copies` as above, for dz (or dy), x and W. */
 int nflow_dense_linear_backward(const void* dy, int dtype, int64_t M, int64_t N, int64_t lddy, const void* x,
@@ -123,9 +126,9 @@ int nflow_grad_norm(const nflow_grad_tensor* tensors, int count, float* norm, vo
 /* The same norm, and each gradient times min(1, max_norm / norm), the factor
  * rounded to fp32.  Where that is 1, gradients clipped in place are not touched.
  * A NaN in any gradient makes all of them NaN, an infinity makes finite ones 0
- * and itself NaN (their norm says so); with an infinite max_norm and no NaN
- * all are left as they are.  An out that is not its own grad, and norm, share no memory with any
- * gradient or other out. */
+ * and itself NaN (their norm says so); with an infinite max_norm and no NaN all are
+ * left as they are.  An out that is not its own grad, and norm, share no memory with
+ * any gradient or other out. */
 int nflow_grad_clip(const nflow_grad_tensor* tensors, int count, float max_norm, float* norm, void* workspace,
                     size_t workspace_bytes, void* stream);
 
