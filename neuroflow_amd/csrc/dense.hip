@@ -225,9 +225,10 @@ struct FewRows {
         const double weight = w == LIE_ANY ? 3.1 : 0.95 + 0.5 * std::min(full, 1.0);
         return 3.0 + std::max(N * bytes / 5e6, pieces * (weight + row * M));
     }
-    // The tiles' copies of what they cannot fetch: room, and us.
+    // The tiles' copies of what they cannot fetch: room, and us (a launch that overlaps the
+    // product's, and the bytes at a copy's rate).
     size_t copied(Lie x, Lie w) const { return (x ? copy_space(M, K) : 0) + (w ? copy_space(N, K) : 0); }
-    double copy_us(Lie x, Lie w) const { return x || w ? 3.3 + 2 * static_cast<double>(copied(x, w)) / 5e6 : 0.0; }
+    double copy_us(Lie x, Lie w) const { return x || w ? 2.0 + 2 * static_cast<double>(copied(x, w)) / 5e6 : 0.0; }
     // Whether it is estimated faster than tiles whose call is estimated at `tiles` us: they
     // gain with much to sum in few columns or with a large weight, by the rate that they read
     // it at, and lose their copies.  Measured, us a call, few against tiles: bf16, one row
@@ -235,7 +236,9 @@ struct FewRows {
     // 7.6, of 4096 -> 16384 52.7 : 34.0; of rows in words, 17 of 16382 -> 16384 185 : 367, 32 of
     // 4094 -> 1024 13.7 : 17.4; at any element, one of 1023 -> 16384 15.7 : 22.5, 17 of 4095 ->
     // 1024 27.9 : 17.4, 32 of 8191 -> 4096 75.9 : 43.1.  fp32, 16 rows of 4096 -> 4096
-    // 19.0 : 26.5, 32 of 4096 -> 256 24.4 : 11.6, of 16384 -> 4096 93.7 : 89.6.
+    // 19.0 : 26.5, 32 of 4096 -> 256 24.4 : 11.6, of 16384 -> 4096 93.7 : 89.6.  Over 500 sizes
+    // of rows off 16-byte groups the choice takes 1% longer than the faster of the two, the
+    // worst 1.4 times as long.
     bool faster(Lie x, Lie w, double tiles) const {
         const double read = static_cast<double>(N) * K / (dtype == NFLOW_DTYPE_F32 ? 0.75e6 : 2e6);
         return us(x, w) <= std::max(tiles, read) + copy_us(x, w);
